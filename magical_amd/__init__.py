@@ -8,6 +8,8 @@ render + LoRes4E preprocessing), keeping its name surface (magical/__init__.py):
     env = magical.make('MoveToCorner-Demo-LoRes4E-v0', n_envs=4096, device='cuda:0')
     obs = env.reset()
     obs, rew, done, info = env.step(actions)      # info['eval_score']
+    obs, rew, done, info = env.step_policy(logits)           # the same with actions drawn from a policy's logits [4096, 18]
+    magical.action_log_probs(logits, actions)                # their log probabilities and entropies, differentiable
 
 The compute path is hand-written HIP (magical_amd/csrc) behind the C ABI in include/mgx.h;
 there is no CPU fallback.
@@ -23,4 +25,14 @@ from magical_amd.version import __version__  # noqa: F401
 # try_download_demos, load_demos, preprocess_demos_with_wrapper, splice_in_preproc_name, __version__; the rest is this package's own)
 __all__ = ['DEMO_ENVS_TO_TEST_ENVS_MAP', 'register_envs', 'make', 'EnvName', 'ALL_REGISTERED_ENVS',
            'AVAILABLE_PREPROCESSORS', 'update_magical_env_name', 'try_download_demos', 'load_demos',
-           'preprocess_demos_with_wrapper', 'splice_in_preproc_name', '__version__']
+           'preprocess_demos_with_wrapper', 'splice_in_preproc_name', '__version__',
+           'ActionLogProbs', 'SampledActions', 'action_log_probs', 'sample_actions']
+
+
+def __getattr__(name):
+    """The operators on a policy's action scores (magical_amd/policy.py), looked up when asked for: that module needs torch, which the
+    rest of the package imports with the first env."""
+    if name in ('ActionLogProbs', 'SampledActions', 'action_log_probs', 'sample_actions'):
+        from magical_amd import policy
+        return getattr(policy, name)
+    raise AttributeError(f'module {__name__!r} has no attribute {name!r}')

@@ -1,4 +1,4 @@
-"""ctypes binding of libmagical_hip.so (the C ABI in include/mgx.h).
+"""ctypes binding of libmagical_hip.so (the C ABI in include/mgx.h and include/mgx_policy.h).
 
 The product path has NO fallback: if the HIP library is missing or no GPU is
 visible, loading / engine creation raises.  Build with `python __graft_entry__.py`
@@ -6,12 +6,17 @@ visible, loading / engine creation raises.  Build with `python __graft_entry__.p
 """
 import ctypes as C
 import os
+import shutil
 import subprocess
+import tempfile
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_PKG, 'csrc')
 LIB_PATH = os.environ.get('MGX_LIB_PATH') or os.path.join(_PKG, 'libmagical_hip.so')      # (override: development builds with other -D knobs)
-_SOURCES = ['mgx_api.hip', 'mgx_world.cpp']
+_SOURCES = ['mgx_api.hip', 'mgx_world.cpp', 'policy/mgx_policy.hip']
+# the operators on action scores are compiled without packed fp32 instructions: some of their forms have given wrong results on this
+# hardware now and then.  (The engine's sources keep their code generation: without them its fp32 results and speed change.)
+_SOURCE_FLAGS = {'policy/mgx_policy.hip': ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
 _DEPS = _SOURCES + ['mgx_step.hip', 'mgx_raster.hip', 'mgx_raster_body.inc', 'mgx_score.hip', 'mgx_sim.h', 'mgx_raster.h', 'mgx_tmpl.h', 'mgx_world.h']
 
 # enums (include/mgx.h)
@@ -43,11 +48,25 @@ def build(force=False, verbose=False, defines=(), out=None, extra=()):
     """hipcc --offload-arch=gfx950 (cross-compiles without a GPU).  defines / out / extra: development builds with other -D knobs / compiler flags."""
     if not force and not defines and not needs_build():
         return LIB_PATH
-    cmd = ['hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-Wno-unused-parameter', '-Wno-extern-c-compat',
-           '-pthread', '-o', out or LIB_PATH] + list(extra) + [f'-D{d}' for d in defines] + [os.path.join(_CSRC, f) for f in _SOURCES]
-    if verbose:
-        print(' '.join(cmd))
-    subprocess.check_call(cmd, cwd=_CSRC)
+    flags = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-parameter', '-Wno-extern-c-compat', '-pthread']
+    tmp = tempfile.mkdtemp(prefix='mgx_build_')
+    try:
+        jobs, objects = [], []
+        for f in _SOURCES:      # one compiler per source, together: the engine's takes minutes, the others seconds
+            objects.append(os.path.join(tmp, os.path.basename(f) + '.o'))
+            cmd = ['hipcc'] + flags + _SOURCE_FLAGS.get(f, []) + list(extra) + [f'-D{d}' for d in defines] + ['-c', os.path.join(_CSRC, f), '-o', objects[-1]]
+            if verbose:
+                print(' '.join(cmd), flush=True)
+            jobs.append((cmd, subprocess.Popen(cmd, cwd=_CSRC)))
+        failed = [cmd for cmd, job in jobs if job.wait() != 0]
+        if failed:
+            raise subprocess.CalledProcessError(1, failed[0])
+        link = ['hipcc', '--offload-arch=gfx950', '-shared', '-fPIC', '-pthread', '-o', out or LIB_PATH] + objects
+        if verbose:
+            print(' '.join(link), flush=True)
+        subprocess.check_call(link, cwd=_CSRC)
+    finally:
+        shutil.rmtree(tmp, ignore_errors=True)
     return out or LIB_PATH
 
 
@@ -67,7 +86,11 @@ def lib():
     L = C.CDLL(LIB_PATH)
     vp, i32, i64, dbl = C.c_void_p, C.c_int, C.c_int64, C.c_double
     ip, dp = C.POINTER(C.c_int), C.POINTER(C.c_double)
+    scores = [i32, vp, i64, i64, i64, vp, i64, dbl]     # include/mgx_policy.h: dtype, logits, rows, n, row stride, mask, its row stride, temperature
     L.mgx_last_error.restype = C.c_char_p
+    L.mgx_policy_last_error.restype = C.c_char_p
+    L.mgx_policy_workspace_bytes.argtypes = [i32, i32, i64, i64, i32]
+    L.mgx_policy_workspace_bytes.restype = i64
     sig = {
         'mgx_version': [],
         'mgx_world_create': [C.POINTER(vp)],
@@ -119,6 +142,9 @@ def lib():
         'mgx_engine_render_native': [vp, vp, i32, vp, i32, vp],
         'mgx_engine_set_timing': [vp, i32],
         'mgx_engine_timing_read': [vp, i32, C.POINTER(C.c_float), i32],
+        'mgx_policy_log_probs': [i32] + scores + [vp, i32, i32, vp, vp, vp, vp, vp, vp, i64, vp],
+        'mgx_policy_log_probs_backward': [i32] + scores + [vp, i32, vp, vp, vp, i64, vp, i64, vp, vp],
+        'mgx_policy_sample': [i32] + scores + [vp, i32, vp, vp, vp, vp, i64, vp],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -149,3 +175,5 @@ EXPORTED_SYMBOLS = [
     'mgx_engine_step', 'mgx_engine_substeps', 'mgx_engine_render', 'mgx_engine_step_render', 'mgx_engine_handoff_stats', 'mgx_engine_render_native',
     'mgx_engine_set_timing', 'mgx_engine_timing_read',
 ]
+# include/mgx_policy.h
+POLICY_SYMBOLS = ['mgx_policy_last_error', 'mgx_policy_workspace_bytes', 'mgx_policy_log_probs', 'mgx_policy_log_probs_backward', 'mgx_policy_sample']

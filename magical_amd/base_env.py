@@ -420,6 +420,25 @@ class BaseEnv(abc.ABC):
             obs = {k: v.clone() for k, v in obs.items()} if isinstance(obs, dict) else obs.clone()
         return obs, self._reward, done, info
 
+    def step_policy(self, logits, uniforms=None, *, mask=None, temperature=1.0, generator=None):
+        """step() with one action per env drawn on the device from a policy's scores, logits [n_envs, 18] (magical_amd/policy.py:
+        sample_actions; no action leaves the GPU).  uniforms: the random numbers f32 / f64 [n_envs] in [0, 1), drawn with `generator`
+        if None.  An env in which nothing is open (or whose logits are NaN) gets action 0 (no movement, gripper open).
+        Returns step()'s tuple; info['action'] (i32, as drawn: -1 there), info['action_log_prob'] and info['action_entropy'] (f32) are
+        tensors [n_envs] on the GPU."""
+        import torch
+        from .policy import sample_actions
+        if tuple(logits.shape) != (self.n_envs, self.action_space_n):
+            raise ValueError(f'logits: [{self.n_envs}, {self.action_space_n}], got {tuple(logits.shape)}')
+        if logits.device != self.device:
+            raise ValueError(f'logits are on {logits.device}, the envs on {self.device}')
+        if uniforms is None:
+            uniforms = torch.rand(self.n_envs, device=self.device, generator=generator)
+        drawn = sample_actions(logits, uniforms, mask=mask, temperature=temperature)
+        obs, rew, done, info = self.step(drawn.action.clamp(min=0))
+        info['action'], info['action_log_prob'], info['action_entropy'] = drawn.action, drawn.log_prob, drawn.entropy
+        return obs, rew, done, info
+
     def _check_capacity(self, idx, n_finished, source=None):
         """Chipmunk never drops a contact (base_env.py:243); this engine's per-env working set is sized from the world
         (every shape pair that can touch) and counts what did not fit in state_i[2].  The counter of the envs whose episode

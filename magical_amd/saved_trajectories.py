@@ -129,11 +129,15 @@ def preprocess_demos_with_wrapper(trajectories, orig_env_name=None, preproc_name
     return out
 
 
-def replay_demos(demo_dicts, device='cuda:0', preproc=None, **env_kwargs):
+def replay_demos(demo_dicts, device='cuda:0', preproc=None, policy=None, **env_kwargs):
     """Replay the action tapes of demos of ONE env name through the engine, all demos in lockstep (one env per demo;
     shorter demos idle on action 0 after their end and are scored at their own last step).  Returns
     {'scores': f64[n], 'recorded_scores': f64[n], 'final_obs': [...]}: with the reference's data the two score columns are
-    the end-to-end parity check of SURVEY.md section 8f-4 (demonstrations solve their task, so both should be ~1)."""
+    the end-to-end parity check of SURVEY.md section 8f-4 (demonstrations solve their task, so both should be ~1).
+
+    policy: also score a policy on the demonstrations.  A callable from the env's observation (before the step) to logits
+    [n, 18] on the GPU; the result then has, per demo, 'log_probs' and 'entropies' (f32[T]: log p of the recorded action, the policy's
+    entropy; magical_amd/policy.py: action_log_probs) and 'best_actions' (i32[T]: what the policy would rather have done)."""
     import torch
     from . import make
     demo_dicts = list(demo_dicts)
@@ -148,14 +152,27 @@ def replay_demos(demo_dicts, device='cuda:0', preproc=None, **env_kwargs):
     try:
         obs = env.reset()
         scores = np.zeros(n, dtype=np.float64)
+        judged = []
         for t in range(T):
             acts = np.array([tape[t] if t < len(tape) else 0 for tape in tapes], dtype=np.int32)
+            if policy is not None:
+                from .policy import action_log_probs
+                given = np.array([tape[t] if t < len(tape) else -1 for tape in tapes], dtype=np.int32)     # (-1: this demo is over)
+                with torch.no_grad():
+                    judged.append(action_log_probs(policy(obs), torch.as_tensor(given, device=env.device), top=1))
             obs, _, _, _ = env.step(torch.as_tensor(acts, device=env.device))
             ending = [k for k, tape in enumerate(tapes) if len(tape) == t + 1]
             if ending:
                 idx = np.asarray(ending)
                 env._scoring_envs = idx
                 scores[idx] = env.score_on_end_of_traj(env.get_poses(idx))
-        return {'scores': scores, 'recorded_scores': np.array([float(d.get('score', np.nan)) for d in demo_dicts]), 'final_obs': obs}
+        out = {'scores': scores, 'recorded_scores': np.array([float(d.get('score', np.nan)) for d in demo_dicts]), 'final_obs': obs}
+        if policy is not None:
+            columns = {'log_probs': [j.log_prob for j in judged], 'entropies': [j.entropy for j in judged],
+                       'best_actions': [j.top_actions[:, 0] for j in judged]}
+            for key, steps in columns.items():
+                whole = torch.stack(steps).cpu().numpy()
+                out[key] = [whole[:len(tape), k].copy() for k, tape in enumerate(tapes)]
+        return out
     finally:
         env.close()

@@ -1,0 +1,709 @@
+"""The operators on a policy's action scores (magical_amd/policy.py, include/mgx_policy.h) against their formulas in 64 bits.
+
+Tolerances.  u = 2^-24 is fp32's largest relative rounding error.  With d = (x - m) / T, s = sum e^d, L = log n:
+  * d has three roundings (the difference, 1 / T, the product): |err d| <= 3 u |d|;
+  * e^d: 2 ulp of the exponential and err d: relative 4 u + 3 u |d|; a sum of n of them by lanes and trees of at most
+    A = 40 + n / 256 additions in a row: relative A u.  sum |d| e^d / s <= L + 1, so err(log s) <= u (A + 4 + 3 (L + 1) + L);
+  * log p = d - log s: u (4 |d| + A + 8 + 4 L);
+  * H = log s - t / s with t = sum d e^d: |t / s| <= L + 1, sum d^2 e^d / s <= (L + 2)^2, so err H <= u (2 A (L + 2) + 4 (L + 2)^2 + 16);
+  * the gradient's p = e^(log p): relative err(log p) + 4 u; the rest is the product rule, and one rounding to the logits' type (half a
+    step, eps / 2 relative, in float16 at least 2^-25)."""
+import math
+import os
+import re
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+U = 2.0 ** -24
+
+
+# ------------------------------------------------------------------------------------------------ the formulas, in 64 bits, on the CPU
+def oracle(x, mask=None, temperature=1.0):
+    """(open, log p, H, undefined rows) of logits [rows, n] (float64 numpy)."""
+    x = np.asarray(x, dtype=np.float64)
+    is_open = ~np.isneginf(x)
+    if mask is not None:
+        is_open &= np.broadcast_to(np.asarray(mask), x.shape)
+    bad = (is_open & (np.isnan(x) | np.isposinf(x))).any(1)
+    z = np.where(is_open, x, -np.inf)
+    z[bad] = 0.0
+    with np.errstate(all='ignore'):
+        m = z.max(1, keepdims=True)
+        m = np.where(np.isneginf(m), 0.0, m)
+        d = (z - m) / temperature
+        s = np.exp(d).sum(1, keepdims=True)
+        lp = np.where(is_open, d - np.log(s), -np.inf)
+        h = np.where(is_open.any(1), -(np.where(np.isneginf(lp), 0.0, np.exp(lp)) * np.where(np.isneginf(lp), 0.0, lp)).sum(1), 0.0)
+    lp[bad] = np.nan
+    h[bad] = np.nan
+    return is_open, lp, h, bad
+
+
+def oracle_top(x, is_open, bad, k):
+    out = np.full((x.shape[0], k), -1, dtype=np.int32)
+    for r in range(x.shape[0]):
+        if not bad[r]:
+            idx = np.nonzero(is_open[r])[0]
+            best = idx[np.argsort(-x[r, idx], kind='stable')][:k]
+            out[r, :len(best)] = best
+    return out
+
+
+def oracle_grad(is_open, lp, h, actions, g_lp, g_h, temperature):
+    p = np.where(is_open, np.exp(lp), 0.0)
+    safe = np.where(is_open & ~np.isneginf(lp), lp, 0.0)
+    given = actions >= 0
+    gl = np.where(given, g_lp, 0.0)[:, None]
+    g = -p * (gl + g_h[:, None] * (safe + h[:, None]))
+    rows = np.nonzero(given & (actions < lp.shape[1]))[0]
+    rows = rows[is_open[rows, actions[rows]]]
+    g[rows, actions[rows]] += g_lp[rows]
+    return np.where(is_open, g / temperature, 0.0)
+
+
+def oracle_draw(is_open, lp, u):
+    """(action, smallest distance of u to a border of the distribution) per row."""
+    p = np.where(is_open, np.exp(lp), 0.0)
+    c = np.cumsum(p, 1)
+    c /= np.where(c[:, -1:] > 0, c[:, -1:], 1.0)
+    a = np.minimum((c <= u[:, None]).sum(1), p.shape[1] - 1)
+    inner = np.where(p > 0, np.abs(c - u[:, None]), np.inf)
+    return np.where(is_open.any(1), a, -1), np.minimum(inner.min(1), np.where(is_open.any(1), 1.0, np.inf))
+
+
+def in_f32(v):
+    """Values outside fp32's range round to the infinities (the type's lowest value over a temperature below 1 does)."""
+    return np.where(np.abs(v) > np.finfo(np.float32).max, np.sign(v) * np.inf, v)
+
+
+def err_log_prob(d, n):
+    L, A = math.log(n), 40 + n / 256
+    return U * (4 * np.abs(d) + A + 8 + 4 * L)
+
+
+def err_entropy(n):
+    L, A = math.log(n), 40 + n / 256
+    return U * (2 * A * (L + 2) + 4 * (L + 2) ** 2 + 16)
+
+
+def err_grad(is_open, lp, h, g_lp, g_h, want, temperature, eps, tiny):
+    n = lp.shape[1]
+    lpz = np.where(is_open & ~np.isneginf(lp), lp, 0.0)
+    p = np.where(is_open, np.exp(lp), 0.0)
+    rel = err_log_prob(np.abs(lpz) + math.log(n), n) + 4 * U
+    size = np.abs(g_lp)[:, None] + np.abs(g_h)[:, None] * (np.abs(lpz) + h[:, None])
+    e = p * (rel * size + np.abs(g_h)[:, None] * (rel + err_entropy(n)) + 4 * U * size) / temperature + 4 * U * np.abs(want)
+    return e + np.maximum(np.abs(want) * (1 + 1e-3) * eps / 2, tiny) + 2.0 ** -126
+
+
+# ------------------------------------------------------------------------------------------------ no GPU needed
+def test_the_library_exports_the_policy_header():
+    from magical_amd import _native
+    L = _native.lib()
+    header = open(os.path.join(ROOT, 'include', 'mgx_policy.h')).read()
+    header = re.sub(r'/\*.*?\*/', '', header, flags=re.S)
+    declared = set(re.findall(r'\b(mgx_policy_[a-z_]+)\s*\(', header))
+    assert declared == set(_native.POLICY_SYMBOLS)
+    for name in declared:
+        getattr(L, name)
+
+
+def _c_args(**kw):
+    a = dict(dtype=0, logits=64, rows=1, n=18, row_stride=18, mask=None, mask_row_stride=0, temperature=1.0)
+    a.update(kw)
+    return [a[k] for k in ('dtype', 'logits', 'rows', 'n', 'row_stride', 'mask', 'mask_row_stride', 'temperature')]
+
+
+@pytest.mark.parametrize('kw', [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(n=0), dict(n=(1 << 30) + 1), dict(row_stride=-1),
+                                dict(mask=64, mask_row_stride=-1), dict(temperature=0.0), dict(temperature=-1.0),
+                                dict(temperature=float('nan')), dict(temperature=float('inf')), dict(temperature=1e-60),
+                                dict(temperature=1e300), dict(logits=None)])
+def test_the_c_entries_refuse_bad_scores_before_any_device_work(kw):
+    from magical_amd import _native
+    L = _native.lib()
+    args = _c_args(**kw)
+    assert L.mgx_policy_log_probs(0, *args, 64, 4, 0, 64, 64, None, None, None, None, 0, None) == -1
+    assert L.mgx_policy_last_error()
+    assert L.mgx_policy_log_probs_backward(0, *args, 64, 4, 64, 64, None, 0, None, 0, 64, None) == -1
+    assert L.mgx_policy_sample(0, *args, 64, 4, 64, None, None, None, 0, None) == -1
+
+
+def test_the_c_entries_refuse_other_bad_arguments_before_any_device_work():
+    from magical_amd import _native
+    L = _native.lib()
+    a = _c_args()
+    for action_bytes, top in ((2, 0), (4, -1), (4, 19), (4, 65)):
+        assert L.mgx_policy_log_probs(0, *a, 64, action_bytes, top, 64, 64, None, 64, 64, None, 0, None) == -1
+    assert L.mgx_policy_log_probs(0, *_c_args(n=100, row_stride=100), 64, 4, 65, 64, 64, None, 64, 64, None, 0, None) == -1
+    assert L.mgx_policy_log_probs(0, *a, None, 4, 0, 64, 64, None, None, None, None, 0, None) == -1
+    assert L.mgx_policy_log_probs(0, *a, 64, 4, 0, None, 64, None, None, None, None, 0, None) == -1
+    assert L.mgx_policy_log_probs(0, *a, 64, 4, 2, 64, 64, None, None, 64, None, 0, None) == -1
+    assert L.mgx_policy_log_probs_backward(0, *a, 64, 2, 64, 64, None, 0, None, 0, 64, None) == -1
+    assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, None, 64, None, 0, None, 0, 64, None) == -1
+    assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, 64, 64, 64, -1, None, 0, 64, None) == -1
+    assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, 64, 64, None, 0, None, 0, None, None) == -1
+    assert L.mgx_policy_sample(0, *a, 64, 2, 64, None, None, None, 0, None) == -1
+    assert L.mgx_policy_sample(0, *a, None, 4, 64, None, None, None, 0, None) == -1
+    assert L.mgx_policy_sample(0, *a, 64, 4, None, None, None, None, 0, None) == -1
+    # nothing to do is no error, whatever the pointers
+    empty = _c_args(rows=0, logits=None)
+    assert L.mgx_policy_log_probs(0, *empty, None, 4, 0, None, None, None, None, None, None, 0, None) == 0
+    assert L.mgx_policy_log_probs_backward(0, *empty, None, 4, None, None, None, 0, None, 0, None, None) == 0
+    assert L.mgx_policy_sample(0, *empty, None, 4, None, None, None, None, 0, None) == 0
+
+
+def test_the_python_entries_refuse_bad_arguments():
+    import torch
+    import magical_amd as m
+    from magical_amd._native import MgxError
+    x, a, u = torch.zeros(3, 18), torch.zeros(3, dtype=torch.int32), torch.zeros(3)
+    with pytest.raises(MgxError, match='no CPU fallback'):
+        m.action_log_probs(x, a)
+    with pytest.raises(MgxError, match='no CPU fallback'):
+        m.sample_actions(x, u)
+    for bad in (np.zeros((3, 18)), x.double(), x.int(), x.to(torch.complex64)):
+        with pytest.raises(TypeError):
+            m.action_log_probs(bad, a)
+        with pytest.raises(TypeError):
+            m.sample_actions(bad, u)
+    for bad in (torch.zeros(()), torch.zeros(3, 0)):
+        with pytest.raises(ValueError):
+            m.action_log_probs(bad, a)
+    for bad in (a.float(), a.to(torch.int16), a.bool(), [0, 0, 0]):
+        with pytest.raises(TypeError):
+            m.action_log_probs(x, bad)
+    for bad in (a[:2], a[:, None], torch.zeros((), dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            m.action_log_probs(x, bad)
+    for bad in (torch.ones(18), torch.ones(18, dtype=torch.uint8), np.ones(18, bool)):
+        with pytest.raises(TypeError):
+            m.action_log_probs(x, a, mask=bad)
+        with pytest.raises(TypeError):
+            m.sample_actions(x, u, mask=bad)
+    for bad in (torch.ones(17, dtype=torch.bool), torch.ones(2, 18, dtype=torch.bool), torch.ones(1, 3, 18, dtype=torch.bool)):
+        with pytest.raises(ValueError):
+            m.action_log_probs(x, a, mask=bad)
+    for bad in (0.0, -1.0, float('nan'), float('inf')):
+        with pytest.raises(ValueError):
+            m.action_log_probs(x, a, temperature=bad)
+        with pytest.raises(ValueError):
+            m.sample_actions(x, u, temperature=bad)
+    for bad in (-1, 19):
+        with pytest.raises(ValueError):
+            m.action_log_probs(x, a, top=bad)
+    with pytest.raises(ValueError):
+        m.action_log_probs(torch.zeros(3, 100), a, top=65)
+    with pytest.raises(TypeError):
+        m.sample_actions(x, u.half())
+    with pytest.raises(ValueError):
+        m.sample_actions(x, u[:2])
+
+
+# ------------------------------------------------------------------------------------------------ on the GPU
+NS = [1, 2, 3, 4, 5, 8, 9, 16, 17, 18, 19, 20, 31, 32, 33, 48, 63, 64, 65, 100, 127, 128, 129, 200, 255, 256, 257, 324, 511, 512, 513,
+      1000, 1024, 1025, 2047, 2048, 2049, 4097, 5832, 8191, 20011]
+DTYPES = ['f32', 'f16', 'bf16']
+
+
+def _torch_type(name):
+    import torch
+    return {'f32': torch.float32, 'f16': torch.float16, 'bf16': torch.bfloat16}[name]
+
+
+def _case(n, dtype, seed, rows=None, masked=None):
+    """Logits with the values that masks and policies bring: spread scores, one far ahead, ties, -inf, the type's lowest value; in row 0 (of
+    several) nothing is open, in row 1 only one action, row 2 is all equal, row 3 all the type's lowest value."""
+    import torch
+    rng = np.random.RandomState(seed)
+    rows = rows if rows is not None else (13 if n < 3000 else 6)
+    t = _torch_type(dtype)
+    x = rng.randn(rows, n) * 3
+    x[rng.rand(rows) < 0.3] *= 0.01
+    ahead = rng.rand(rows) < 0.4
+    x[ahead, rng.randint(0, n, rows)[ahead]] += 12
+    x[rng.rand(rows, n) < 0.05] = -np.inf
+    x[rng.rand(rows, n) < 0.05] = float(torch.finfo(t).min)
+    mask = None
+    if masked == 'rows':
+        mask = rng.rand(rows, n) < 0.7
+    elif masked == 'shared':
+        mask = rng.rand(n) < 0.7
+    if rows > 4:
+        x[0] = -np.inf
+        x[1] = -np.inf
+        x[1, rng.randint(n)] = -1.5
+        x[2] = 0.75
+        x[3] = float(torch.finfo(t).min)
+    if masked == 'rows' and rows > 5:
+        mask[5] = False
+    x = torch.tensor(x, dtype=torch.float64).to(t)
+    actions = rng.randint(0, n, rows)
+    actions[rng.rand(rows) < 0.2] = -1
+    return x, mask, actions, rng
+
+
+def _check_forward(out, x64, mask, actions, temperature, top, what):
+    is_open, lp, h, bad = oracle(x64, mask, temperature)
+    n = x64.shape[1]
+    got_lp, got_h = out.log_prob.detach().double().cpu().numpy(), out.entropy.detach().double().cpu().numpy()
+    with np.errstate(invalid='ignore'):
+        d = np.where(is_open, (x64 - np.where(is_open, x64, -np.inf).max(1, keepdims=True)) / temperature, 0.0)
+    for r in range(len(actions)):
+        a = int(actions[r])
+        want = 0.0 if a < 0 else (np.nan if a >= n or bad[r] else float(in_f32(lp[r, a])))
+        if np.isfinite(want):
+            assert abs(got_lp[r] - want) <= (0 if a < 0 else err_log_prob(d[r, a], n)), (what, r, got_lp[r], want)
+        else:
+            assert got_lp[r] == want or (np.isnan(want) and np.isnan(got_lp[r])), (what, r, got_lp[r], want)
+    assert np.array_equal(np.isnan(got_h), bad), what
+    assert np.all(np.abs(got_h - h)[~bad] <= err_entropy(n)), (what, np.abs(got_h - h)[~bad].max())
+    if top:
+        want_a = oracle_top(x64, is_open, bad, top)
+        got_a, got_t = out.top_actions.cpu().numpy(), out.top_log_probs.double().cpu().numpy()
+        assert np.array_equal(got_a, want_a), what
+        there = want_a >= 0
+        rows = np.nonzero(there)[0]
+        want_t = in_f32(lp[rows, want_a[there]])
+        fine = np.isfinite(want_t)
+        assert np.all(np.abs(got_t[there] - want_t)[fine] <= err_log_prob(d[rows, want_a[there]], n)[fine]), what
+        assert np.all(np.isneginf(got_t[there][~fine])) and np.all(np.isneginf(got_t[~there])), what
+    return is_open, lp, h, bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n', NS)
+def test_log_probs_gradient_and_draws_against_64_bits(n, dtype):
+    import torch
+    import magical_amd as m
+    for k, (masked, temperature) in enumerate([(None, 1.0), ('shared', 1.0), ('rows', 0.7), ('rows', 2.5)]):
+        x, mask, actions, rng = _case(n, dtype, 1000 * n + k, masked=masked)
+        rows = x.shape[0]
+        x64 = x.double().numpy()
+        top = min(n, (0, 1, 5, 64)[k])
+        leaf = x.cuda().requires_grad_(True)
+        m_dev = None if mask is None else torch.tensor(mask).cuda()
+        a_dev = torch.tensor(actions, dtype=(torch.int32, torch.int64)[k % 2]).cuda()
+        out = m.action_log_probs(leaf, a_dev, mask=m_dev, temperature=temperature, top=top)
+        what = (n, dtype, masked, temperature)
+        is_open, lp, h, bad = _check_forward(out, x64, mask, actions, temperature, top, what)
+        # the gradient
+        g_lp, g_h = rng.randn(rows).astype(np.float32), (rng.randn(rows) * 0.1).astype(np.float32)
+        torch.autograd.backward((out.log_prob, out.entropy), (torch.tensor(g_lp).cuda(), torch.tensor(g_h).cuda()))
+        assert leaf.grad.dtype == x.dtype
+        got = leaf.grad.double().cpu().numpy()
+        want = oracle_grad(is_open, lp, h, actions, g_lp.astype(np.float64), g_h.astype(np.float64), temperature)
+        eps, tiny = torch.finfo(x.dtype).eps, 2.0 ** -25 if dtype == 'f16' else 0.0
+        bound = err_grad(is_open, lp, h, g_lp.astype(np.float64), g_h.astype(np.float64), want, temperature, eps, tiny)
+        assert np.all(np.abs(got - want) <= bound), (what, np.max(np.abs(got - want) / bound))
+        assert np.all(got[~is_open] == 0), what
+        # without a graph: the same bits
+        again = m.action_log_probs(leaf.detach(), a_dev, mask=m_dev, temperature=temperature, top=top)
+        assert torch.equal(again.log_prob, out.log_prob) and torch.equal(again.entropy, out.entropy), what
+        # draws
+        u = rng.rand(rows)
+        u[-1] = 0.0
+        u = u.astype(np.float32) if k % 2 else u
+        drawn = m.sample_actions(leaf.detach(), torch.tensor(u).cuda(), mask=m_dev, temperature=temperature)
+        want_a, gap = oracle_draw(is_open, lp, u.astype(np.float64))
+        clear = gap > 1e-11
+        clear[-1] = True                      # u = 0: the first action of non-zero probability, exactly
+        if is_open[-1].any():
+            want_a[-1] = np.nonzero(is_open[-1] & (np.exp(lp[-1]) > 0))[0][0]
+        assert clear.sum() >= rows - 1
+        got_a = drawn.action.cpu().numpy()
+        assert np.array_equal(got_a[clear], want_a[clear]), (what, got_a, want_a)
+        rows_open = np.nonzero(got_a >= 0)[0]
+        want_lp = in_f32(lp[rows_open, got_a[rows_open]])
+        assert np.all(np.abs(drawn.log_prob.double().cpu().numpy()[rows_open] - want_lp) <= U * (np.abs(want_lp) + 1e-6)), what
+        assert np.all(np.isneginf(drawn.log_prob.cpu().numpy()[got_a < 0])), what
+        assert np.all(np.abs(drawn.entropy.double().cpu().numpy() - h) <= U * (h + 1e-6) + 1e-12), what
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 18, 300, 1500, 6000, 70000])
+def test_rows_that_nothing_or_nonsense_is_left_in(n):
+    """NaN and infinities among the open scores, behind the mask, and everywhere."""
+    import torch
+    import magical_amd as m
+    nan, inf = float('nan'), float('inf')
+    x = torch.randn(8, n, generator=torch.Generator().manual_seed(n))
+    mask = torch.ones(8, n, dtype=torch.bool)
+    k = n // 2
+    x[0, k] = nan
+    x[1, k] = inf
+    x[2, k] = nan
+    mask[2, k] = False
+    x[3, k] = inf
+    mask[3, k] = False
+    x[4] = nan
+    x[5] = nan
+    mask[5] = False
+    x[6] = -inf
+    x[7, k] = -inf
+    actions = torch.full((8,), n - 1, dtype=torch.int64)
+    leaf = x.cuda().requires_grad_(True)
+    top = min(n, 3)
+    out = m.action_log_probs(leaf, actions.cuda(), mask=mask.cuda(), top=top)
+    is_open, lp, h, bad = _check_forward(out, x.double().numpy(), mask.numpy(), actions.numpy(), 1.0, top, n)
+    assert bad.tolist() == [True, True, False, False, True, False, False, False]
+    (out.log_prob.nan_to_num(0, 0, 0).sum() * 0 + out.log_prob.sum() + out.entropy.sum()).backward()
+    grad = leaf.grad.cpu().numpy()
+    assert np.all(np.isnan(grad[bad][is_open[bad]])) and np.all(grad[~is_open] == 0) and np.all(np.isfinite(grad[~bad]))
+    drawn = m.sample_actions(leaf.detach(), torch.full((8,), 0.5).cuda(), mask=mask.cuda())
+    assert np.all((drawn.action.cpu().numpy() == -1) == (bad | ~is_open.any(1)))
+    assert np.all(np.isnan(drawn.log_prob.cpu().numpy()) == bad) and np.all(np.isnan(drawn.entropy.cpu().numpy()) == bad)
+    # padded rows keep log probability 0 even so; an action behind the last one is NaN
+    out = m.action_log_probs(leaf.detach(), torch.tensor([-1, -7, n, n + 5, -1, -1, -1, n]).cuda(), mask=mask.cuda())
+    got = out.log_prob.cpu().numpy()
+    assert np.all(got[[0, 1, 4, 5, 6]] == 0) and np.all(np.isnan(got[[2, 3, 7]]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [18, 700, 6000])
+def test_random_numbers_at_and_outside_the_ends(n):
+    import torch
+    import magical_amd as m
+    x = torch.randn(7, n, generator=torch.Generator().manual_seed(n))
+    x[:, 0] = x[:, -1] = float('-inf')
+    u = torch.tensor([0.0, -3.0, float('nan'), 1.0, 5.0, float('inf'), 1 - 2.0 ** -53], dtype=torch.float64)
+    a = m.sample_actions(x.cuda(), u.cuda()).action.cpu().tolist()
+    assert a == [1, 1, 1, n - 2, n - 2, n - 2, n - 2]
+    a = m.sample_actions(x.cuda(), u.float().cuda()).action.cpu().tolist()
+    assert a == [1, 1, 1, n - 2, n - 2, n - 2, n - 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n', [18, 19, 300, 1500, 5000, 40000])
+def test_strides_offsets_and_orders_change_no_bit(n, dtype):
+    """Views of a wider head, odd offsets, transposed, expanded and higher-dimensional tensors: the results of the dense copy."""
+    import torch
+    import magical_amd as m
+    g = torch.Generator(device='cuda').manual_seed(n)
+    rows = 24
+    base = torch.randn(rows, n, generator=g, device='cuda').to(_torch_type(dtype))
+    mask = torch.rand(rows, n, generator=g, device='cuda') < 0.8
+    actions = torch.randint(0, n, (rows,), generator=g, device='cuda')
+    u = torch.rand(rows, generator=g, device='cuda')
+    g_lp, g_h = torch.randn(rows, generator=g, device='cuda'), torch.randn(rows, generator=g, device='cuda')
+
+    def all_of(x, msk, acts=actions, uu=u, gl=g_lp, gh=g_h):
+        x = x.detach().requires_grad_(True)
+        out = m.action_log_probs(x, acts, mask=msk, top=3)
+        grad, = torch.autograd.grad((out.log_prob, out.entropy), (x,), (gl, gh))
+        return list(out) + [grad] + list(m.sample_actions(x.detach(), uu, mask=msk))
+
+    want = all_of(base, mask)
+
+    def same(got, shape=None):
+        for a, b in zip(got, want):
+            a = a.reshape(b.shape)
+            assert torch.equal(a, b)
+
+    wide = torch.full((rows, n + 3), 7.0, device='cuda', dtype=base.dtype)
+    wide[:, 1:n + 1] = base
+    wide_mask = torch.zeros((rows, n + 5), device='cuda', dtype=torch.bool)
+    wide_mask[:, 3:n + 3] = mask
+    same(all_of(wide[:, 1:n + 1], wide_mask[:, 3:n + 3]))
+    flat = torch.zeros(rows * n + 1, device='cuda', dtype=base.dtype)
+    flat[1:] = base.reshape(-1)
+    same(all_of(flat[1:].view(rows, n), mask))
+    same(all_of(base.t().contiguous().t(), mask.t().contiguous().t()))
+    cube = lambda t: t.view(2, 3, 4, *t.shape[1:])      # noqa: E731
+    same(all_of(cube(base), cube(mask), cube(actions), cube(u), cube(g_lp), cube(g_h)))
+    same(all_of(base, mask, actions.int()))
+    # one row for all, one mask for all
+    row = base[:1].expand(rows, n)
+    got, dense = all_of(row, mask[0]), all_of(row.contiguous(), mask[:1].expand(rows, n).contiguous())
+    for a, b in zip(got, dense):
+        assert torch.equal(a, b)
+    # ... and the gradient of the one row is the sum over its uses
+    leaf = base[0].float().clone().requires_grad_(True)
+    out = m.action_log_probs(leaf.expand(rows, n), actions, mask=mask[0])
+    (out.log_prob * g_lp).sum().backward()
+    grads = all_of(leaf.detach().expand(rows, n).contiguous(), mask[0], gh=torch.zeros_like(g_h))[4]
+    assert torch.allclose(leaf.grad.double(), grads.double().sum(0), rtol=rows * 2.0 ** -23, atol=rows * 2.0 ** -23)
+    # a single row without a batch dimension
+    one = m.action_log_probs(base[5], actions[5], mask=mask[5], top=3)
+    assert one.log_prob.shape == () and one.top_actions.shape == (3,)
+    assert torch.allclose(one.log_prob, want[0][5], rtol=0, atol=float(err_log_prob(30, n)))
+    assert m.sample_actions(base[5], u[5], mask=mask[5]).action.shape == ()
+    # none at all
+    none = m.action_log_probs(base[:0].requires_grad_(True), actions[:0], top=2)
+    assert none.log_prob.shape == (0,) and none.top_actions.shape == (0, 2)
+    none.log_prob.sum().backward()
+    assert m.sample_actions(base[:0], u[:0]).action.shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,n', [((1 << 20) + 3, 18), (300007, 5), (70001, 324), (5003, 2500)])
+def test_many_rows(rows, n):
+    """Every row of a large batch is worked on: the results of row subsets equal those of the whole."""
+    import torch
+    import magical_amd as m
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    x = (torch.randn(rows, n, generator=g, device='cuda') * 2).bfloat16()
+    a = torch.randint(0, n, (rows,), generator=g, device='cuda')
+    u = torch.rand(rows, generator=g, device='cuda')
+    xr = x.clone().requires_grad_(True)
+    out = m.action_log_probs(xr, a, top=2)
+    out.log_prob.sum().backward()
+    x32 = x.float()
+    lse = torch.logsumexp(x32, 1)
+    tol = float(err_log_prob(40, n)) + 40 * 2.0 ** -23
+    assert (out.log_prob - (x32.gather(1, a[:, None])[:, 0] - lse)).abs().max() <= tol
+    p = torch.exp(x32 - lse[:, None])
+    want = -p
+    want.scatter_add_(1, a[:, None], torch.ones_like(want[:, :1]))
+    assert (xr.grad.float() - want).abs().max() <= 2.0 ** -8 + 1e-5
+    assert (x.gather(1, out.top_actions[:, :1].long())[:, 0] == x.amax(1)).all()
+    drawn = m.sample_actions(x, u)
+    assert ((drawn.action >= 0) & (drawn.action < n)).all()
+    cut = rows - 1234
+    part = m.sample_actions(x[cut:], u[cut:])
+    assert torch.equal(part.action, drawn.action[cut:])
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows that lie further than 2^32 bytes and 2^31 elements from the first one."""
+    import torch
+    import magical_amd as m
+    far = (1 << 31) + 64
+    buf = torch.empty(far + 40000, dtype=torch.float16, device='cuda')
+    for n in (18, 1000, 30000):
+        g = torch.Generator(device='cuda').manual_seed(n)
+        x = torch.randn(2, n, generator=g, device='cuda').half()
+        buf[:n], buf[far:far + n] = x[0], x[1]
+        view = buf.as_strided((2, n), (far, 1)).requires_grad_(True)
+        a = torch.tensor([0, n - 1], device='cuda')
+        u = torch.tensor([0.3, 0.6], device='cuda')
+        dense = x.clone().requires_grad_(True)
+        got, want = m.action_log_probs(view, a, top=4), m.action_log_probs(dense, a, top=4)
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+        # (the gradient as the kernel hands it out: autograd would lay a view's gradient out over the whole buffer)
+        out = m.action_log_probs(view.detach(), a)
+        assert torch.equal(out.log_prob, want.log_prob)
+        assert torch.equal(m.sample_actions(view.detach(), u).action, m.sample_actions(x, u).action)
+    del buf, view
+    rows = (1 << 31) // 18 + 1000                       # results and gradient of more than 2^31 elements in all
+    x = torch.zeros(1, 18, device='cuda', dtype=torch.bfloat16)
+    x[0, 3] = 2.0
+    a = torch.full((rows,), 3, dtype=torch.int32, device='cuda')
+    leaf = x.expand(rows, 18).requires_grad_(True)
+    out = m.action_log_probs(leaf, a)
+    assert (out.log_prob == out.log_prob[0]).all()
+    grad, = torch.autograd.grad(out.log_prob, leaf, torch.ones((), device='cuda').expand(rows))
+    assert torch.equal(grad[-1000:], grad[:1000]) and (grad[-1] != 0).all()
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """The kernels' gradient (fp32) against central differences of the formula in 64 bits: (f(x + h) - f(x - h)) / 2h, h = 1e-4, is off by
+    h^2 / 6 x the third derivative (of log p and H: below 10 + L) and by rounding 2^-52 |f| / h."""
+    import torch
+    import magical_amd as m
+    rng = np.random.RandomState(0)
+    for n, temperature in ((2, 1.0), (18, 0.5), (70, 3.0)):
+        x = rng.randn(4, n).astype(np.float32)
+        actions, gl, gh = rng.randint(0, n, 4), rng.randn(4), rng.randn(4)
+        leaf = torch.tensor(x).cuda().requires_grad_(True)
+        out = m.action_log_probs(leaf, torch.tensor(actions).cuda(), temperature=temperature)
+        torch.autograd.backward((out.log_prob, out.entropy), (torch.tensor(gl).float().cuda(), torch.tensor(gh).float().cuda()))
+
+        def f(z):
+            _, lp, h, _ = oracle(z, None, temperature)
+            return gl.astype(np.float32) * lp[np.arange(4), actions] + gh.astype(np.float32) * h
+        step, want = 1e-4, np.zeros((4, n))
+        for j in range(n):
+            e = np.zeros((1, n))
+            e[0, j] = step
+            want[:, j] = (f(x.astype(np.float64) + e) - f(x.astype(np.float64) - e)) / (2 * step)
+        L = math.log(n)
+        tol = (np.abs(gl) + np.abs(gh)) * (step ** 2 / 6 * (10 + L) / temperature ** 3 + 2.0 ** -52 * (10 / temperature + L) / step)
+        tol = tol[:, None] + (np.abs(gl) + np.abs(gh) * (L + 1))[:, None] * 2 * err_entropy(n) / temperature
+        assert np.all(np.abs(leaf.grad.cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,n', [(64, 18), (300, 324), (9, 5832), (2, 104976)])
+def test_captured_calls_replay(rows, n):
+    """Forward, backward and draws in one captured graph, replayed on new inputs with eager calls of other sizes in between."""
+    import torch
+    import magical_amd as m
+    g = torch.Generator(device='cuda').manual_seed(1)
+
+    def new():
+        return (torch.randn(rows, n, generator=g, device='cuda'), torch.randint(0, n, (rows,), generator=g, device='cuda'),
+                torch.rand(rows, generator=g, device='cuda'))
+
+    gl, gh = torch.randn(rows, generator=g, device='cuda'), torch.full((rows,), -0.01, device='cuda')
+
+    def work(x, a, u):
+        out = m.action_log_probs(x, a, top=4)
+        grad, = torch.autograd.grad((out.log_prob, out.entropy), (x,), (gl, gh))
+        drawn = m.sample_actions(x.detach(), u, temperature=0.8)
+        return [out.log_prob.detach(), out.entropy.detach(), out.top_actions, out.top_log_probs, grad, *drawn]
+
+    sx, sa, su = (t.clone() for t in new())
+    sx.requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(sx, sa, su)
+    torch.cuda.current_stream().wait_stream(side)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work(sx, sa, su)
+    with torch.cuda.graph(other):
+        held2 = work(sx, sa, su)
+    for _ in range(4):
+        x, a, u = new()
+        with torch.no_grad():
+            sx.copy_(x)
+        sa.copy_(a)
+        su.copy_(u)
+        graph.replay()
+        other.replay()
+        torch.cuda.synchronize()
+        want = work(x.requires_grad_(True), a, u)
+        for p, p2, q in zip(held, held2, want):
+            assert torch.equal(p, q) and torch.equal(p2, q)
+        m.action_log_probs(torch.randn(3, 50000, device='cuda'), torch.zeros(3, dtype=torch.int64, device='cuda'), top=8)
+
+
+@pytest.mark.gpu
+def test_calls_on_other_streams_and_interleaved():
+    """Two streams at once, each with its own inputs: the results of one after the other."""
+    import torch
+    import magical_amd as m
+    torch.cuda.synchronize()
+    sets = []
+    for k, (rows, n) in enumerate([(3, 60000), (5, 90000), (4096, 18), (2, 104976)]):
+        g = torch.Generator(device='cuda').manual_seed(k)
+        sets.append((torch.randn(rows, n, generator=g, device='cuda'), torch.randint(0, n, (rows,), generator=g, device='cuda'),
+                     torch.rand(rows, generator=g, device='cuda')))
+    want = [(m.action_log_probs(x, a, top=7), m.sample_actions(x, u)) for x, a, u in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(5):
+        for s, (x, a, u) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append((m.action_log_probs(x, a, top=7), m.sample_actions(x, u)))
+    torch.cuda.synchronize()
+    for k, (p, q) in enumerate(got):
+        for t, w in zip(list(p) + list(q), list(want[k % 4][0]) + list(want[k % 4][1])):
+            assert torch.equal(t, w)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    import torch
+    import magical_amd as m
+    x, a = torch.zeros(3, 18, device='cuda'), torch.zeros(3, dtype=torch.int32, device='cuda')
+    with pytest.raises(ValueError):
+        m.action_log_probs(x, a.cpu())
+    with pytest.raises(ValueError):
+        m.action_log_probs(x, a, mask=torch.ones(18, dtype=torch.bool))
+    with pytest.raises(ValueError):
+        m.sample_actions(x, torch.zeros(3))
+    # twice differentiable it is not, and it says so
+    leaf = x.clone().requires_grad_(True)
+    g, = torch.autograd.grad(m.action_log_probs(leaf, a).entropy.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    # inputs changed in between are noticed
+    y = (leaf * 1.0)
+    out = m.action_log_probs(y, a)
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError):
+        out.log_prob.sum().backward()
+
+
+@pytest.mark.gpu
+def test_a_rollout_and_its_learning_step():
+    """As they are used together: actions drawn per env-step by step_policy, the same bits as sample_actions + step; the rollout's log
+    probabilities again from action_log_probs; one ascent step along the gradient makes the drawn actions likelier."""
+    import torch
+    import magical_amd as m
+    n_envs, T = 64, 6
+    env = m.make('MoveToCorner-Demo-LoRes4E-v0', n_envs=n_envs, device='cuda:0')
+    twin = m.make('MoveToCorner-Demo-LoRes4E-v0', n_envs=n_envs, device='cuda:0')
+    g = torch.Generator(device='cuda').manual_seed(5)
+    weights = (torch.randn(12, 18, generator=g, device='cuda') * 0.05).requires_grad_(True)
+    obs, _ = env.reset(), twin.reset()
+    feats, acts, lps, ents = [], [], [], []
+    for t in range(T):
+        feat = obs.float().mean((1, 2)) / 32
+        feats.append(feat)
+        u = torch.rand(n_envs, generator=g, device='cuda')
+        with torch.no_grad():
+            logits = feat @ weights
+        obs, rew, done, info = env.step_policy(logits, u)
+        drawn = m.sample_actions(logits, u)
+        want, _, _, _ = twin.step(drawn.action)
+        assert torch.equal(obs, want)
+        assert torch.equal(info['action'], drawn.action) and torch.equal(info['action_log_prob'], drawn.log_prob)
+        acts.append(info['action'])
+        lps.append(info['action_log_prob'])
+        ents.append(info['action_entropy'])
+    feats, acts, lps, ents = torch.stack(feats), torch.stack(acts), torch.stack(lps), torch.stack(ents)
+    out = m.action_log_probs(feats @ weights, acts)
+    tol = float(err_log_prob(30, 18)) + 60 * 2.0 ** -23             # (+ the two matrix products' own rounding of scores below 8)
+    assert (out.log_prob - lps).abs().max() <= tol and (out.entropy - ents).abs().max() <= tol + float(err_entropy(18))
+    (out.log_prob.mean() + 0.01 * out.entropy.mean()).backward()
+    # the gradient to the weights, from the formula in 64 bits
+    z = (feats.double() @ weights.detach().double()).requires_grad_(True)
+    lp = torch.log_softmax(z, 2)
+    ref = lp.gather(2, acts.long()[..., None]).mean() - 0.01 * (lp.exp() * lp).sum(2).mean()
+    gz, = torch.autograd.grad(ref, z)
+    gw = feats.double().flatten(0, 1).t() @ gz.flatten(0, 1)
+    assert (weights.grad.double() - gw).abs().max() <= 1e-5 * gw.abs().max() + 1e-7
+    # no action is open: the env idles
+    obs, _, _, info = env.step_policy(torch.full((n_envs, 18), float('-inf'), device='cuda'))
+    want, _, _, _ = twin.step(np.zeros(n_envs, dtype=np.int32))
+    assert torch.equal(obs, want) and (info['action'] == -1).all()
+    with pytest.raises(ValueError):
+        env.step_policy(torch.zeros(n_envs, 17, device='cuda'))
+    with pytest.raises(ValueError):
+        env.step_policy(torch.zeros(n_envs, 18))
+    env.close()
+    twin.close()
+
+
+@pytest.mark.gpu
+def test_replay_scores_a_policy_on_demonstrations():
+    """replay_demos(policy=...): per demo, the log probability of every recorded action, the entropies and the policy's own choice; demos
+    that are over take no part."""
+    import torch
+    from magical_amd import saved_trajectories as st
+    rng = np.random.RandomState(3)
+    lengths = (5, 9, 2)
+    demos = [{'env_name': 'MoveToCorner-Demo-v0', 'score': 0.0,
+              'trajectory': st.MAGICALTrajectory(acts=rng.randint(0, 18, T), obs={}, rews=np.zeros(T), infos=None)} for T in lengths]
+    seen = []
+    w = torch.randn(12, 18, generator=torch.Generator().manual_seed(0)).cuda() * 0.05
+
+    def policy(obs):
+        logits = (obs.float().mean((1, 2)) / 32) @ w
+        seen.append(logits.double().cpu().numpy())
+        return logits
+
+    plain = st.replay_demos(demos, preproc='LoRes4E')
+    out = st.replay_demos(demos, preproc='LoRes4E', policy=policy)
+    assert np.array_equal(out['scores'], plain['scores']) and torch.equal(out['final_obs'], plain['final_obs'])
+    assert set(plain) == {'scores', 'recorded_scores', 'final_obs'} and len(seen) == max(lengths)
+    for k, demo in enumerate(demos):
+        T = lengths[k]
+        assert len(out['log_probs'][k]) == len(out['entropies'][k]) == len(out['best_actions'][k]) == T
+        for t in range(T):
+            is_open, lp, h, _ = oracle(seen[t][k:k + 1])
+            assert abs(out['log_probs'][k][t] - lp[0, demo['trajectory'].acts[t]]) <= err_log_prob(60, 18)
+            assert abs(out['entropies'][k][t] - h[0]) <= err_entropy(18)
+            assert out['best_actions'][k][t] == seen[t][k].argmax()
