@@ -66,6 +66,255 @@ template <typename V, typename F> __device__ __forceinline__ V block_all(V v, V 
 // is (v, i) a better alternative than (w, k)?  Higher score first, then the lower index.
 __device__ __forceinline__ bool better(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
 
+// e^d for d <= 0 in 64 bits: d = k log 2 + r with |r| <= log 2 / 2 (log 2 in two parts, so that r is exact to 2^-53), Taylor's series to
+// the 13th power (the next term is below 2^-57), times 2^k.  NaN stays NaN, -inf gives 0.
+__device__ __forceinline__ double exp64(double d) {
+    const double k = rint(d * 1.4426950408889634);
+    double r = fma(k, -0x1.62e42fefa3800p-1, d);
+    r = fma(k, -0x1.ef35793c76730p-45, r);
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return d < -800.0 ? 0.0 : ldexp(p, (int)k);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- short rows
+// A row of up to 2048 scores stays in the registers of G lanes (4 ... 64, so that several rows share a wavefront), E a lane: one read of the
+// scores, all sums by lane exchanges, no LDS, no barrier.
+
+template <typename V, typename F> __device__ __forceinline__ V group_all(V v, int G, F f) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+        if (o < G) v = f(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ float f_max(float a, float b) { return fmaxf(a, b); }
+
+// W consecutive scores from j on, in one load where they are all there (gfx950 loads any alignment)
+template <int W, typename T> __device__ __forceinline__ void load(const Row<T> &row, int j, int n, float (&x)[W]) {
+    if (j + W <= n) {
+        T v[W];
+        __builtin_memcpy(v, row.x + j, sizeof v);
+#pragma unroll
+        for (int k = 0; k < W; k++) x[k] = to_f32(v[k]);
+        if (row.mask) {
+            uint8_t b[W];
+            __builtin_memcpy(b, row.mask + j, W);
+#pragma unroll
+            for (int k = 0; k < W; k++) x[k] = b[k] ? x[k] : NEG_INF;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < W; k++) x[k] = j + k < n ? row.at(j + k) : NEG_INF;
+    }
+}
+
+// lane g of a row's G lanes holds W-wide pieces: x[e] is score place(g, e)
+template <int G, int E> struct Spread {
+    static constexpr int W = E % 4 == 0 && G == 64 ? 4 : 1;
+    static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
+    template <typename T> static __device__ __forceinline__ void load_row(const Row<T> &row, int g, int n, float (&x)[E]) {
+#pragma unroll
+        for (int e = 0; e < E; e += W) {
+            float v[W];
+            load<W>(row, place(g, e), n, v);
+#pragma unroll
+            for (int k = 0; k < W; k++) x[e + k] = v[k];
+        }
+    }
+};
+
+template <typename T, int G, int E>
+__global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy,
+                                                           float *top_log_probs, int32_t *top_actions) {
+    using S = Spread<G, E>;
+    const int g = threadIdx.x % G, n = (int)sc.n;
+    for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
+        const Row<T> row(sc, r);
+        float x[E];
+        S::load_row(row, g, n, x);
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
+        m = group_all(m, G, f_max);
+        const bool some = m > NEG_INF;
+        const float ref = some ? m : 0.0f;
+        float s = 0, t = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const float d = (x[e] - ref) * sc.inv_t, p = expf(d);
+            s += p;
+            t += p * fmaxf(d, -1e30f);          // (not open: 0 x a finite number)
+        }
+        s = group_all(s, G, [](float a, float b) { return a + b; });
+        t = group_all(t, G, [](float a, float b) { return a + b; });
+        const bool undefined = !(s == s);
+        const float log_s = logf(s), nan = __builtin_nanf("");
+        if (g == 0) {
+            const int64_t a = actions.at(r);
+            float lp = 0.0f;
+            if (a >= n || (a >= 0 && undefined)) lp = nan;
+            else if (a >= 0) lp = some ? (row.at(a) - ref) * sc.inv_t - log_s : NEG_INF;
+            log_prob[r] = lp;
+            entropy[r] = undefined ? nan : some ? log_s - t / s : 0.0f;
+        }
+        // the best alternatives, one after the other: every lane's best of what is left, then the group's
+        for (int k = 0; k < top; k++) {
+            float v = NEG_INF;
+            int i = 0x7fffffff;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const bool b = x[e] > v;          // (a lane's places ascend: of equal scores the first)
+                v = b ? x[e] : v;
+                i = b ? S::place(g, e) : i;
+            }
+#pragma unroll
+            for (int o = 1; o < G; o <<= 1) {
+                const float ov = __shfl_xor(v, o);
+                const int oi = __shfl_xor(i, o);
+                const bool b = better(ov, oi, v, i);
+                v = b ? ov : v;
+                i = b ? oi : i;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = S::place(g, e) == i ? NEG_INF : x[e];
+            if (g == 0) {
+                const bool there = v > NEG_INF && !undefined;
+                top_actions[r * top + k] = there ? i : -1;
+                top_log_probs[r * top + k] = there ? (v - ref) * sc.inv_t - log_s : NEG_INF;
+            }
+        }
+    }
+}
+
+template <typename T, int G, int E>
+__global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions actions, const float *entropy, const float *g_lp,
+                                                          int64_t g_lp_stride, const float *g_h, int64_t g_h_stride, T *grad) {
+    using S = Spread<G, E>;
+    const int g = threadIdx.x % G, n = (int)sc.n;
+    for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
+        const Row<T> row(sc, r);
+        float x[E];
+        S::load_row(row, g, n, x);
+        const int64_t a = actions.at(r);
+        const float h = entropy[r];
+        const float gl = g_lp && a >= 0 ? g_lp[r * g_lp_stride] : 0.0f, gh = g_h ? g_h[r * g_h_stride] : 0.0f;
+        // maximum and sum again (cheaper than 8 bytes a row written and read)
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
+        m = group_all(m, G, f_max);
+        const float ref = m > NEG_INF ? m : 0.0f;
+        float s = 0;
+        float p[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            p[e] = expf((x[e] - ref) * sc.inv_t);
+            s += p[e];
+        }
+        s = group_all(s, G, [](float a, float b) { return a + b; });
+        const float inv_s = 1.0f / s, log_s = logf(s);
+        T out[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const float lp = (x[e] - ref) * sc.inv_t - log_s;
+            float v = -(p[e] * inv_s) * (gl + gh * (fmaxf(lp, -1e30f) + h));
+            if (S::place(g, e) == a) v += gl;
+            out[e] = from_f32<T>(x[e] == NEG_INF ? 0.0f : v * sc.inv_t);
+        }
+        T *to = grad + r * sc.n;
+#pragma unroll
+        for (int e = 0; e < E; e += S::W) {
+            const int j = S::place(g, e);
+            if (j + S::W <= n) __builtin_memcpy(to + j, out + e, S::W * sizeof(T));
+            else
+#pragma unroll
+                for (int k = 0; k < S::W; k++)
+                    if (j + k < n) to[j + k] = out[e + k];
+        }
+    }
+}
+
+__device__ __forceinline__ double uniform_at(const void *uniforms, int bytes, int64_t r) {
+    const double u = bytes == 8 ? ((const double *)uniforms)[r] : (double)((const float *)uniforms)[r];
+    return u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;          // (NaN: 0)
+}
+
+// Lane g holds the E consecutive scores from g * E on: a running sum in index order is a lane's sum, a scan over the lanes, and a second
+// look at the one lane in which the target lies.
+template <typename T, int G, int E>
+__global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void *uniforms, int uniform_bytes, int32_t *action,
+                                                        float *log_prob, float *entropy) {
+    constexpr int W = E % 8 == 0 ? 8 : E % 4 == 0 ? 4 : 1;
+    const int g = threadIdx.x % G, n = (int)sc.n;
+    for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
+        const Row<T> row(sc, r);
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; e += W) {
+            float v[W];
+            load<W>(row, g * E + e, n, v);
+#pragma unroll
+            for (int k = 0; k < W; k++) x[e + k] = v[k];
+        }
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
+        m = group_all(m, G, f_max);
+        const bool some = m > NEG_INF;
+        const double ref = some ? m : 0.0;
+        double p[E], s = 0, t = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const double d = ((double)x[e] - ref) * sc.inv_t64;
+            p[e] = exp64(d);
+            s += p[e];
+            t = fma(p[e], fmax(d, -1e300), t);
+        }
+        double upto = s;          // the lanes' running sum, this one's included
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) {
+            const double v = __shfl_up(upto, o, G);
+            if (g >= o) upto += v;
+        }
+        const double total = __shfl(upto, G - 1, G);
+        t = group_all(t, G, [](double a, double b) { return a + b; });
+        const bool undefined = !(total == total), none = undefined || !some;
+        const double target = uniform_at(uniforms, uniform_bytes, r) * total;
+        // the first lane that passes the target, or else (rounding; a number of 1) the last one with anything in it
+        const int first_lane = (threadIdx.x & 63) - g;
+        const uint64_t in_group = G == 64 ? ~0ull : ((1ull << (G & 63)) - 1) << first_lane;
+        const uint64_t past = __ballot(s > 0.0 && upto > target) & in_group, any = __ballot(s > 0.0) & in_group;
+        const int owner = none ? first_lane : past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)any);
+        if ((threadIdx.x & 63) == owner) {
+            double c = upto - s;
+            c = g == 0 ? 0.0 : c;
+            int a = -1;
+            bool found = false;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                c += p[e];
+                if (p[e] > 0.0 && !found) { a = g * E + e; found = c > target; }
+            }
+            action[r] = none ? -1 : a;
+            if (log_prob) log_prob[r] = undefined ? __builtin_nanf("") : some ? (float)(((double)row.at(a) - ref) * sc.inv_t64 - log(total)) : NEG_INF;
+            if (entropy) entropy[r] = undefined ? __builtin_nanf("") : some ? (float)(log(total) - t / total) : 0.0f;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- rows of any length
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_log_probs(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy, float *stats,
                                                      float *top_log_probs, int32_t *top_actions) {
@@ -254,6 +503,36 @@ template <typename... P, typename... A> int launch(void (*kernel)(P...), int64_t
     return err == hipSuccess ? (int)MGX_OK : fail(MGX_ERR_HIP, hipGetErrorString(err));
 }
 
+constexpr int SHORT_MAX = 2048;
+template <int G_, int E_> struct Shape { static constexpr int G = G_, E = E_; };
+// f(lanes a row and scores a lane) for rows of n <= SHORT_MAX: the fewest lanes that keep 4 ... 8 scores each, then a whole wavefront
+template <typename F> int by_length(int64_t n, F f) {
+    if (n <= 32)
+        switch ((n + 3) / 4) {
+            case 1: return f(Shape<4, 1>());
+            case 2: return f(Shape<4, 2>());
+            case 3: return f(Shape<4, 3>());
+            case 4: return f(Shape<4, 4>());
+            case 5: return f(Shape<4, 5>());
+            case 6: return f(Shape<4, 6>());
+            case 7: return f(Shape<4, 7>());
+            default: return f(Shape<4, 8>());
+        }
+    if (n <= 48) return f(Shape<8, 6>());
+    if (n <= 64) return f(Shape<8, 8>());
+    if (n <= 96) return f(Shape<16, 6>());
+    if (n <= 128) return f(Shape<16, 8>());
+    if (n <= 192) return f(Shape<32, 6>());
+    if (n <= 256) return f(Shape<32, 8>());
+    if (n <= 384) return f(Shape<64, 6>());
+    if (n <= 512) return f(Shape<64, 8>());
+    if (n <= 768) return f(Shape<64, 12>());
+    if (n <= 1024) return f(Shape<64, 16>());
+    if (n <= 1536) return f(Shape<64, 24>());
+    return f(Shape<64, 32>());
+}
+int64_t short_blocks(int64_t rows, int G) { return (rows * G + BLOCK - 1) / BLOCK; }
+
 // f(a value of the scores' element type)
 template <typename F> int by_dtype(int dtype, F f) {
     switch (dtype) {
@@ -285,6 +564,12 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
+        if (n <= SHORT_MAX)
+            return by_length(n, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, E = decltype(shape)::E;
+                return launch(k_log_probs_short<T, G, E>, short_blocks(rows, G), BLOCK, stream, sc, Actions{actions, action_bytes}, top,
+                              log_prob, entropy, top_log_probs, top_actions);
+            });
         return launch(k_log_probs<T>, rows, BLOCK, stream, sc, Actions{actions, action_bytes}, top, log_prob, entropy, stats, top_log_probs,
                       top_actions);
     });
@@ -305,6 +590,12 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
+        if (n <= SHORT_MAX)
+            return by_length(n, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, E = decltype(shape)::E;
+                return launch(k_backward_short<T, G, E>, short_blocks(rows, G), BLOCK, stream, sc, Actions{actions, action_bytes}, entropy,
+                              grad_log_prob, grad_log_prob_stride, grad_entropy, grad_entropy_stride, (T *)grad);
+            });
         return launch(k_log_probs_backward<T>, rows, BLOCK, stream, sc, Actions{actions, action_bytes}, stats, entropy, grad_log_prob,
                       grad_log_prob_stride, grad_entropy, grad_entropy_stride, (T *)grad);
     });
@@ -322,6 +613,12 @@ int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, i
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
+        if (n <= SHORT_MAX)
+            return by_length(n, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, E = decltype(shape)::E;
+                return launch(k_sample_short<T, G, E>, short_blocks(rows, G), BLOCK, stream, sc, uniforms, uniform_bytes, action, log_prob,
+                              entropy);
+            });
         return launch(k_sample<T>, rows, BLOCK, stream, sc, uniforms, uniform_bytes, action, log_prob, entropy);
     });
 }

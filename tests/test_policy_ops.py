@@ -75,7 +75,7 @@ def oracle_draw(is_open, lp, u):
 
 def in_f32(v):
     """Values outside fp32's range round to the infinities (the type's lowest value over a temperature below 1 does)."""
-    return np.where(np.abs(v) > np.finfo(np.float32).max, np.sign(v) * np.inf, v)
+    return np.where(np.abs(v) > np.finfo(np.float32).max, np.where(v > 0, np.inf, -np.inf), v)
 
 
 def err_log_prob(d, n):
@@ -267,7 +267,7 @@ def _check_forward(out, x64, mask, actions, temperature, top, what):
         rows = np.nonzero(there)[0]
         want_t = in_f32(lp[rows, want_a[there]])
         fine = np.isfinite(want_t)
-        assert np.all(np.abs(got_t[there] - want_t)[fine] <= err_log_prob(d[rows, want_a[there]], n)[fine]), what
+        assert np.all(np.abs(got_t[there][fine] - want_t[fine]) <= err_log_prob(d[rows, want_a[there]][fine], n)), what
         assert np.all(np.isneginf(got_t[there][~fine])) and np.all(np.isneginf(got_t[~there])), what
     return is_open, lp, h, bad
 
