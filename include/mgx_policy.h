@@ -35,8 +35,10 @@ const char *mgx_policy_last_error(void);
 /* bytes of DEVICE scratch memory (16-byte aligned) that a call of this size needs, 0 if none; it is free again once the call's work
  * has run.  Two calls that may run at the same time need memory of their own. */
 int64_t mgx_policy_workspace_bytes(int op, int dtype, int64_t rows, int64_t n, int top);
+/* bytes of `stats` that the backward call of this size needs from the forward call, 0 if none (stats may then be NULL) */
+int64_t mgx_policy_stats_bytes(int64_t rows, int64_t n);
 /* actions: i32 or i64 [rows] (action_bytes 4 or 8); < 0: none given in this row (log_prob 0); >= n: NaN.  log_prob, entropy: f32 [rows].
- * stats: NULL, or f32 [rows][2] for the backward call.  top (0 ... min(n, MGX_POLICY_MAX_TOP)): the best open actions of each row, best first,
+ * stats: NULL, or f32 of mgx_policy_stats_bytes() for the backward call.  top (0 ... min(n, MGX_POLICY_MAX_TOP)): the best open actions of each row, best first,
  * equal scores by the lower index: top_actions i32 [rows][top] (-1: there are no more), top_log_probs f32 [rows][top] (-inf there). */
 int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride, const uint8_t *mask,
                          int64_t mask_row_stride, double temperature, const void *actions, int action_bytes, int top, float *log_prob,

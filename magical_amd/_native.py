@@ -17,7 +17,10 @@ _SOURCES = ['mgx_api.hip', 'mgx_world.cpp', 'policy/mgx_policy.hip']
 # the operators on action scores are compiled without packed fp32 instructions: some of their forms have given wrong results on this
 # hardware now and then.  (The engine's sources keep their code generation: without them its fp32 results and speed change.)
 _SOURCE_FLAGS = {'policy/mgx_policy.hip': ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
-_DEPS = _SOURCES + ['mgx_step.hip', 'mgx_raster.hip', 'mgx_raster_body.inc', 'mgx_score.hip', 'mgx_sim.h', 'mgx_raster.h', 'mgx_tmpl.h', 'mgx_world.h']
+# ... and their binding to torch tensors, a Python extension module of its own (host code)
+POLICY_OPS_PATH = os.path.join(_PKG, '_policy_torch.so')
+_POLICY_OPS_SOURCE = os.path.join(_CSRC, 'policy', 'mgx_policy_torch.cpp')
+_DEPS = _SOURCES + ['policy/mgx_policy_torch.cpp', '../../include/mgx_policy.h'] + ['mgx_step.hip', 'mgx_raster.hip', 'mgx_raster_body.inc', 'mgx_score.hip', 'mgx_sim.h', 'mgx_raster.h', 'mgx_tmpl.h', 'mgx_world.h']
 
 # enums (include/mgx.h)
 MGX_F32, MGX_F64, MGX_F32_PURE = 0, 1, 2
@@ -38,10 +41,22 @@ class MgxCapacityWarning(RuntimeWarning):
 
 
 def needs_build():
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(POLICY_OPS_PATH):
         return True
-    t = os.path.getmtime(LIB_PATH)
+    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(POLICY_OPS_PATH))
     return any(os.path.getmtime(os.path.join(_CSRC, f)) > t for f in _DEPS)
+
+
+def _policy_ops_command(out):
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    libs = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    return (['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+             f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}']
+            + [a for d in cpp_extension.include_paths() + ['/opt/rocm/include', sysconfig.get_paths()['include']] for a in ('-isystem', d)]
+            + [_POLICY_OPS_SOURCE, '-o', out, '-L' + libs, '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch', '-ltorch_python'])
 
 
 def build(force=False, verbose=False, defines=(), out=None, extra=()):
@@ -58,6 +73,11 @@ def build(force=False, verbose=False, defines=(), out=None, extra=()):
             if verbose:
                 print(' '.join(cmd), flush=True)
             jobs.append((cmd, subprocess.Popen(cmd, cwd=_CSRC)))
+        if out is None:         # (a development build of the library goes with the module that is there)
+            cmd = _policy_ops_command(os.path.join(tmp, 'policy_torch.so'))
+            if verbose:
+                print(' '.join(cmd), flush=True)
+            jobs.append((cmd, subprocess.Popen(cmd, cwd=_CSRC)))
         failed = [cmd for cmd, job in jobs if job.wait() != 0]
         if failed:
             raise subprocess.CalledProcessError(1, failed[0])
@@ -65,6 +85,8 @@ def build(force=False, verbose=False, defines=(), out=None, extra=()):
         if verbose:
             print(' '.join(link), flush=True)
         subprocess.check_call(link, cwd=_CSRC)
+        if out is None:
+            shutil.move(os.path.join(tmp, 'policy_torch.so'), POLICY_OPS_PATH)
     finally:
         shutil.rmtree(tmp, ignore_errors=True)
     return out or LIB_PATH
@@ -91,6 +113,8 @@ def lib():
     L.mgx_policy_last_error.restype = C.c_char_p
     L.mgx_policy_workspace_bytes.argtypes = [i32, i32, i64, i64, i32]
     L.mgx_policy_workspace_bytes.restype = i64
+    L.mgx_policy_stats_bytes.argtypes = [i64, i64]
+    L.mgx_policy_stats_bytes.restype = i64
     sig = {
         'mgx_version': [],
         'mgx_world_create': [C.POINTER(vp)],
@@ -158,6 +182,22 @@ def lib():
     return L
 
 
+_policy_ops = None
+
+
+def policy_ops():
+    """The module of the operators on action scores for torch tensors, tied to the loaded library's entry points."""
+    global _policy_ops
+    if _policy_ops is None:
+        L = lib()
+        if not os.path.exists(POLICY_OPS_PATH):
+            raise MgxError(f'{POLICY_OPS_PATH} not found: the extension is not built (run `python __graft_entry__.py`)')
+        from . import _policy_torch
+        _policy_torch.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in POLICY_SYMBOLS}, MgxError)
+        _policy_ops = _policy_torch
+    return _policy_ops
+
+
 def check(rc):
     if rc < 0:
         raise MgxError(f'mgx error {rc}: {lib().mgx_last_error().decode()}')
@@ -176,4 +216,4 @@ EXPORTED_SYMBOLS = [
     'mgx_engine_set_timing', 'mgx_engine_timing_read',
 ]
 # include/mgx_policy.h
-POLICY_SYMBOLS = ['mgx_policy_last_error', 'mgx_policy_workspace_bytes', 'mgx_policy_log_probs', 'mgx_policy_log_probs_backward', 'mgx_policy_sample']
+POLICY_SYMBOLS = ['mgx_policy_last_error', 'mgx_policy_workspace_bytes', 'mgx_policy_stats_bytes', 'mgx_policy_log_probs', 'mgx_policy_log_probs_backward', 'mgx_policy_sample']

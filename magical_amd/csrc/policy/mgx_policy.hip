@@ -550,6 +550,8 @@ const char *mgx_policy_last_error(void) { return g_err; }
 
 int64_t mgx_policy_workspace_bytes(int, int, int64_t, int64_t, int) { return 0; }
 
+int64_t mgx_policy_stats_bytes(int64_t rows, int64_t n) { return n > SHORT_MAX ? rows * 8 : 0; }
+
 int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride, const uint8_t *mask,
                          int64_t mask_row_stride, double temperature, const void *actions, int action_bytes, int top, float *log_prob,
                          float *entropy, float *stats, float *top_log_probs, int32_t *top_actions, void *workspace,
@@ -584,7 +586,7 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
     if (action_bytes != 4 && action_bytes != 8) return fail(MGX_ERR_ARG, "action_bytes: 4 or 8");
     if (grad_log_prob_stride < 0 || grad_entropy_stride < 0) return fail(MGX_ERR_ARG, "negative stride");
     if (rows == 0) return MGX_OK;
-    if (!actions || !stats || !entropy || !grad) return fail(MGX_ERR_ARG, "NULL argument");
+    if (!actions || (!stats && mgx_policy_stats_bytes(rows, n)) || !entropy || !grad) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
     return by_dtype(dtype, [&](auto v) {

@@ -141,7 +141,8 @@ def test_the_c_entries_refuse_other_bad_arguments_before_any_device_work():
     assert L.mgx_policy_log_probs(0, *a, 64, 4, 0, None, 64, None, None, None, None, 0, None) == -1
     assert L.mgx_policy_log_probs(0, *a, 64, 4, 2, 64, 64, None, None, 64, None, 0, None) == -1
     assert L.mgx_policy_log_probs_backward(0, *a, 64, 2, 64, 64, None, 0, None, 0, 64, None) == -1
-    assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, None, 64, None, 0, None, 0, 64, None) == -1
+    assert L.mgx_policy_log_probs_backward(0, *_c_args(n=5000, row_stride=5000), 64, 4, None, 64, None, 0, None, 0, 64, None) == -1
+    assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, None, None, None, 0, None, 0, 64, None) == -1
     assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, 64, 64, 64, -1, None, 0, 64, None) == -1
     assert L.mgx_policy_log_probs_backward(0, *a, 64, 4, 64, 64, None, 0, None, 0, None, None) == -1
     assert L.mgx_policy_sample(0, *a, 64, 2, 64, None, None, None, 0, None) == -1
@@ -615,7 +616,7 @@ def test_refusals_on_the_gpu():
     # twice differentiable it is not, and it says so
     leaf = x.clone().requires_grad_(True)
     g, = torch.autograd.grad(m.action_log_probs(leaf, a).entropy.sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(RuntimeError, match='differentiable once'):
         g.sum().backward()
     # inputs changed in between are noticed
     y = (leaf * 1.0)
