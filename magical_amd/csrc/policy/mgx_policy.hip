@@ -46,18 +46,138 @@ struct Actions {
 
 constexpr int BLOCK = 256, WAVES = BLOCK / 64;
 
-template <typename V, typename F> __device__ __forceinline__ V wave_all(V v, F f) {
-    for (int o = 1; o < 64; o <<= 1) v = f(v, __shfl_xor(v, o));
+template <typename T> constexpr uint32_t neg_inf_bits = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, half> ? 0xfc00u : 0xff80u;
+
+// N pieces of W neighbouring scores of a row, as they lie in memory (16-bit scores two a word), with their mask bytes.  One load a piece and
+// one for its mask where all W are there (gfx950 loads any alignment), else one a score; what is behind the row's end is -inf.
+template <typename T, int W, int N> struct Pieces {
+    static constexpr int WORDS = W * sizeof(T) < 4 ? 1 : W * sizeof(T) / 4, MASK_WORDS = (W + 3) / 4;
+    uint32_t w[N][WORDS], open[N][MASK_WORDS];
+    using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+    __device__ __forceinline__ void fetch(const Row<T> &row, int p, int j) { __builtin_memcpy(w[p], row.x + j, W * sizeof(T)); }
+    __device__ __forceinline__ void fetch_mask(const Row<T> &row, int p, int j) { __builtin_memcpy(open[p], row.mask + j, W); }
+    __device__ __forceinline__ void fetch_ragged(const Row<T> &row, int p, int j, int n) {
+        if (j + W <= n) return fetch(row, p, j);
+        Bits bits[W];
+#pragma unroll
+        for (int k = 0; k < W; k++) bits[k] = (Bits)neg_inf_bits<T>;
+        if (j < n)
+#pragma unroll
+            for (int k = 0; k < W; k++) {
+                Bits b;
+                __builtin_memcpy(&b, row.x + (j + k < n ? j + k : n - 1), sizeof b);          // (in bounds without a branch)
+                if (j + k < n) bits[k] = b;
+            }
+#pragma unroll
+        for (int k = 0; k < WORDS; k++) w[p][k] = 0;
+#pragma unroll
+        for (int k = 0; k < W; k++) w[p][k * sizeof(T) / 4] |= (uint32_t)bits[k] << (k * sizeof(T) % 4 * 8);
+    }
+    __device__ __forceinline__ void fetch_mask_ragged(const Row<T> &row, int p, int j, int n) {
+        if (j + W <= n) return fetch_mask(row, p, j);
+#pragma unroll
+        for (int k = 0; k < MASK_WORDS; k++) open[p][k] = 0;
+        if (j < n)
+#pragma unroll
+            for (int k = 0; k < W; k++) open[p][k / 4] |= (uint32_t)row.mask[j + k < n ? j + k : n - 1] << (k % 4 * 8);
+    }
+    // piece p from place(p) on; every lane's piece below `whole` is known to be all there
+    template <typename F> __device__ __forceinline__ void load(const Row<T> &row, int n, int whole, F place) {
+#pragma unroll
+        for (int p = 0; p < N; p++)
+            if (p < whole) fetch(row, p, place(p));
+            else fetch_ragged(row, p, place(p), n);
+        if (row.mask) {
+#pragma unroll
+            for (int p = 0; p < N; p++)
+                if (p < whole) fetch_mask(row, p, place(p));
+                else fetch_mask_ragged(row, p, place(p), n);
+        }
+    }
+    __device__ __forceinline__ float score(int p, int k) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[p][k]);
+        else if constexpr (std::is_same_v<T, half>) return (float)__builtin_bit_cast(half, (uint16_t)(w[p][k / 2] >> (k % 2 * 16)));
+        else return __builtin_bit_cast(float, k % 2 ? w[p][k / 2] & 0xffff0000u : w[p][k / 2] << 16);
+    }
+    // the N * W scores in fp32, -inf where the mask rules them out
+    __device__ __forceinline__ void scores(const Row<T> &row, float *x) const {
+#pragma unroll
+        for (int p = 0; p < N; p++)
+#pragma unroll
+            for (int k = 0; k < W; k++) x[p * W + k] = score(p, k);
+        if (row.mask)
+#pragma unroll
+            for (int p = 0; p < N; p++)
+#pragma unroll
+                for (int k = 0; k < W; k++) x[p * W + k] = open[p][k / 4] >> (k % 4 * 8) & 0xff ? x[p * W + k] : NEG_INF;
+    }
+};
+
+// ---- lane exchanges in the vector unit.  Partner values of a butterfly over G lanes: quads, then half rows, rows of 16, and the two swaps of
+// gfx950 (the mirrors reach the other half, whose lanes all hold the same by then).
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ float dpp(float v) { return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(int, v))); }
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dpp<CTRL, ROWS>((int)(uint32_t)b), hi = (uint32_t)dpp<CTRL, ROWS>((int)(uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140, DPP_WAVE_SHR1 = 0x138, DPP_ROW_SHR = 0x110,
+              DPP_BCAST15 = 0x142, DPP_BCAST31 = 0x143;
+template <typename V> struct Two { V a, b; };
+// the values of this lane's and its partner's 16 (32) lanes, the lower ones' first
+__device__ __forceinline__ Two<int> swap16(int v) { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); return {(int)r[0], (int)r[1]}; }
+__device__ __forceinline__ Two<int> swap32(int v) { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); return {(int)r[0], (int)r[1]}; }
+template <int N> __device__ __forceinline__ Two<int> swap(int v) { if constexpr (N == 16) return swap16(v); else return swap32(v); }
+template <int N> __device__ __forceinline__ Two<float> swap(float v) {
+    const Two<int> r = swap<N>(__builtin_bit_cast(int, v));
+    return {__builtin_bit_cast(float, r.a), __builtin_bit_cast(float, r.b)};
+}
+template <int N> __device__ __forceinline__ Two<double> swap(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const Two<int> lo = swap<N>((int)(uint32_t)b), hi = swap<N>((int)(uint32_t)(b >> 32));
+    return {__builtin_bit_cast(double, (uint64_t)(uint32_t)hi.a << 32 | (uint32_t)lo.a), __builtin_bit_cast(double, (uint64_t)(uint32_t)hi.b << 32 | (uint32_t)lo.b)};
+}
+// f over the G lanes of a group (f commutes: all lanes get the same bits)
+template <int G, typename V, typename F> __device__ __forceinline__ V group_all(V v, F f) {
+    if constexpr (G > 1) v = f(v, dpp<DPP_XOR1>(v));
+    if constexpr (G > 2) v = f(v, dpp<DPP_XOR2>(v));
+    if constexpr (G > 4) v = f(v, dpp<DPP_HALF_MIRROR>(v));
+    if constexpr (G > 8) v = f(v, dpp<DPP_MIRROR>(v));
+    if constexpr (G > 16) { const Two<V> t = swap<16>(v); v = f(t.a, t.b); }
+    if constexpr (G > 32) { const Two<V> t = swap<32>(v); v = f(t.a, t.b); }
     return v;
 }
+template <int G> __device__ __forceinline__ float group_max(float v) { return group_all<G>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int G, typename V> __device__ __forceinline__ V group_sum(V v) { return group_all<G>(v, [](V a, V b) { return a + b; }); }
+// running sum over the G lanes of a group, this lane (number g) included
+template <int G> __device__ __forceinline__ double group_scan(double v, int g) {
+    const auto step = [&](double from, int o) { v += G >= 16 || g >= o ? from : 0.0; };          // (a row's first lanes get 0 from outside)
+    if constexpr (G > 1) step(dpp<DPP_ROW_SHR + 1>(v), 1);
+    if constexpr (G > 2) step(dpp<DPP_ROW_SHR + 2>(v), 2);
+    if constexpr (G > 4) step(dpp<DPP_ROW_SHR + 4>(v), 4);
+    if constexpr (G > 8) step(dpp<DPP_ROW_SHR + 8>(v), 8);
+    if constexpr (G > 16) v += dpp<DPP_BCAST15, 0xa>(v);
+    if constexpr (G > 32) v += dpp<DPP_BCAST31, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int first_lane(uint64_t b) { return __ffsll((unsigned long long)b) - 1; }
+__device__ __forceinline__ int last_lane(uint64_t b) { return 63 - __clzll((long long)b); }
+
 // is (v, i) a better alternative than (w, k)?  Higher score first, then the lower index.
 __device__ __forceinline__ bool better(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
 
-// 2^y for y <= 0 in 64 bits: y = k + f with |f| <= 1 / 2, a polynomial for 2^f (interpolated at the Chebyshev points of [-1/2, 1/2] in 60
-// digits: off by 3.1e-16 at most), times 2^k.  Below -1100 (and for NaN, which the callers look for themselves) it is 0.
+// 2^y for -1100 <= y <= 0 in 64 bits: y = k + f with |f| <= 1 / 2 (k by adding 1.5 * 2^52, whose last bits then are k), a polynomial for 2^f
+// (interpolated at the Chebyshev points of [-1/2, 1/2] in 60 digits: off by 3.1e-16 at most), k added to its exponent; 0 for k below -1000.
 __device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -1100.0);
-    const double k = rint(y), f = y - k;
+    const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
+    const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, shifted);
     double p = 0x1.e6063f7217bc6p-28;
     p = fma(p, f, 0x1.b675bca4eeebbp-24);
     p = fma(p, f, 0x1.62bfd47773353p-20);
@@ -69,69 +189,44 @@ __device__ __forceinline__ double exp2_64(double y) {
     p = fma(p, f, 0x1.ebfbdff82c598p-3);
     p = fma(p, f, 0x1.62e42fefa3a19p-1);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)k);
+    const uint64_t b = __builtin_bit_cast(uint64_t, p);
+    const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)k << 20);
+    return k < -1000 ? 0.0 : __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
 }
+// (x - ref) inv_t2 for it: -inf and whatever else 2^y is 0 for at -1100.  (A NaN too: the callers look for those themselves.)
+__device__ __forceinline__ double below(float x, double ref, double inv_t2) { return fmax(((double)x - ref) * inv_t2, -1100.0); }
 constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
-// A row of up to 2048 scores stays in the registers of G lanes (4 ... 64, so that several rows share a wavefront), E a lane: one read of the
-// scores, all sums by lane exchanges, no LDS, no barrier.
-
-template <typename V, typename F> __device__ __forceinline__ V group_all(V v, int G, F f) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
-        if (o < G) v = f(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float f_max(float a, float b) { return fmaxf(a, b); }
-
-// W consecutive scores from j on, in one load where they are all there (gfx950 loads any alignment)
-template <int W, typename T> __device__ __forceinline__ void load(const Row<T> &row, int j, int n, float (&x)[W]) {
-    if (j + W <= n) {
-        T v[W];
-        __builtin_memcpy(v, row.x + j, sizeof v);
-#pragma unroll
-        for (int k = 0; k < W; k++) x[k] = to_f32(v[k]);
-        if (row.mask) {
-            uint8_t b[W];
-            __builtin_memcpy(b, row.mask + j, W);
-#pragma unroll
-            for (int k = 0; k < W; k++) x[k] = b[k] ? x[k] : NEG_INF;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < W; k++) x[k] = j + k < n ? row.at(j + k) : NEG_INF;
-    }
-}
-
-// lane g of a row's G lanes holds W-wide pieces: x[e] is score place(g, e)
-template <int G, int E> struct Spread {
-    static constexpr int W = E % 4 == 0 && G == 64 ? 4 : 1;
+// A row of up to 2048 scores stays in the registers of G lanes (1 ... 64), E a lane: one read of the scores, all sums by lane exchanges, no
+// LDS, no barrier.  Lane g holds pieces of W neighbouring scores (16 bytes, or 1): x[e] is score place(g, e).
+template <int G, int E, int W> struct Spread {
     static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
     template <typename T> static __device__ __forceinline__ void load_row(const Row<T> &row, int g, int n, float (&x)[E]) {
-#pragma unroll
-        for (int e = 0; e < E; e += W) {
-            float v[W];
-            load<W>(row, place(g, e), n, v);
-#pragma unroll
-            for (int k = 0; k < W; k++) x[e + k] = v[k];
-        }
+        Pieces<T, W, E / W> p;
+        p.load(row, n, n / (G * W), [&](int k) { return place(g, k * W); });
+        p.scores(row, x);
     }
 };
+template <int E> __device__ __forceinline__ float lane_max(const float (&x)[E]) {
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
+    return m;
+}
 
-template <typename T, int G, int E>
+template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy,
                                                            float *top_log_probs, int32_t *top_actions) {
-    using S = Spread<G, E>;
+    using S = Spread<G, E, W>;
     const int g = threadIdx.x % G, n = (int)sc.n;
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
+        const int64_t a = actions.at(r);
+        float xa = a >= 0 && a < n ? row.at(a) : NEG_INF;
         float x[E];
         S::load_row(row, g, n, x);
-        float m = x[0];
-#pragma unroll
-        for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
-        m = group_all(m, G, f_max);
+        const float m = group_max<G>(lane_max(x));
         const bool some = m > NEG_INF;
         const float ref = some ? m : 0.0f;
         float s = 0, t = 0;
@@ -141,15 +236,14 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
             s += p;
             t = fmaf(p, fmaxf(d, -1e30f), t);          // (not open: 0 x a finite number)
         }
-        s = group_all(s, G, [](float a, float b) { return a + b; });
-        t = group_all(t, G, [](float a, float b) { return a + b; });
+        s = group_sum<G>(s);
+        t = group_sum<G>(t);
         const bool undefined = !(s == s);
         const float log_s = logf(s), nan = __builtin_nanf("");
         if (g == 0) {
-            const int64_t a = actions.at(r);
             float lp = 0.0f;
             if (a >= n || (a >= 0 && undefined)) lp = nan;
-            else if (a >= 0) lp = some ? (row.at(a) - ref) * sc.inv_t - log_s : NEG_INF;
+            else if (a >= 0) lp = some ? (xa - ref) * sc.inv_t - log_s : NEG_INF;
             log_prob[r] = lp;
             entropy[r] = undefined ? nan : some ? log_s - t / s * (float)LN_2 : 0.0f;
         }
@@ -163,14 +257,17 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
                 v = b ? x[e] : v;
                 i = b ? S::place(g, e) : i;
             }
-#pragma unroll
-            for (int o = 1; o < G; o <<= 1) {
-                const float ov = __shfl_xor(v, o);
-                const int oi = __shfl_xor(i, o);
+            const auto take = [&](float ov, int oi) {
                 const bool b = better(ov, oi, v, i);
                 v = b ? ov : v;
                 i = b ? oi : i;
-            }
+            };
+            if constexpr (G > 1) take(dpp<DPP_XOR1>(v), dpp<DPP_XOR1>(i));
+            if constexpr (G > 2) take(dpp<DPP_XOR2>(v), dpp<DPP_XOR2>(i));
+            if constexpr (G > 4) take(dpp<DPP_HALF_MIRROR>(v), dpp<DPP_HALF_MIRROR>(i));
+            if constexpr (G > 8) take(dpp<DPP_MIRROR>(v), dpp<DPP_MIRROR>(i));
+            if constexpr (G > 16) { const auto ov = swap<16>(v); const auto oi = swap<16>(i); take(ov.a, oi.a); take(ov.b, oi.b); }
+            if constexpr (G > 32) { const auto ov = swap<32>(v); const auto oi = swap<32>(i); take(ov.a, oi.a); take(ov.b, oi.b); }
 #pragma unroll
             for (int e = 0; e < E; e++) x[e] = S::place(g, e) == i ? NEG_INF : x[e];
             if (g == 0) {
@@ -182,49 +279,49 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
     }
 }
 
-template <typename T, int G, int E>
-__global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions actions, const float *entropy, const float *g_lp,
-                                                          int64_t g_lp_stride, const float *g_h, int64_t g_h_stride, T *grad) {
-    using S = Spread<G, E>;
+struct Upstream {          // gradients to the log probabilities and entropies, one value a row (stride 0: one for all), or NULL
+    const float *lp, *h;
+    int64_t lp_stride, h_stride;
+};
+
+template <typename T, int G, int E, int W>
+__global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions actions, const float *entropy, Upstream up, T *grad) {
+    using S = Spread<G, E, W>;
     const int g = threadIdx.x % G, n = (int)sc.n;
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
+        const int64_t a = actions.at(r);
+        const float h = entropy[r], gl = up.lp && a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
         float x[E];
         S::load_row(row, g, n, x);
-        const int64_t a = actions.at(r);
-        const float h = entropy[r];
-        const float gl = g_lp && a >= 0 ? g_lp[r * g_lp_stride] : 0.0f, gh = g_h ? g_h[r * g_h_stride] : 0.0f;
         // maximum and sum again (cheaper than 8 bytes a row written and read)
-        float m = x[0];
-#pragma unroll
-        for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
-        m = group_all(m, G, f_max);
-        const float ref = m > NEG_INF ? m : 0.0f;
-        float s = 0;
-        float p[E];
+        const float m = group_max<G>(lane_max(x)), ref = m > NEG_INF ? m : 0.0f;
+        float s = 0, p[E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
             p[e] = __builtin_amdgcn_exp2f((x[e] - ref) * sc.inv_t2);
             s += p[e];
         }
-        s = group_all(s, G, [](float a, float b) { return a + b; });
-        const float inv_s = 1.0f / s, log_s = logf(s);
+        s = group_sum<G>(s);
+        // dx = p (c0 + c1 log2 p) + 1[j = a] g_lp / T
+        const float inv_s = 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
+        const float at_a = gl * sc.inv_t;
+        const int ai = a >= 0 && a < n ? (int)a : -1;
         T out[E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const float lp = (x[e] - ref) * sc.inv_t - log_s;
-            float v = -(p[e] * inv_s) * (gl + gh * (fmaxf(lp, -1e30f) + h));
-            if (S::place(g, e) == a) v += gl;
-            out[e] = from_f32<T>(x[e] == NEG_INF ? 0.0f : v * sc.inv_t);
+            const float l2 = (x[e] - ref) * sc.inv_t2 - log2_s;
+            const float v = p[e] * fmaf(c1, fmaxf(l2, -1e30f), c0) + (S::place(g, e) == ai ? at_a : 0.0f);
+            out[e] = from_f32<T>(x[e] == NEG_INF ? 0.0f : v);
         }
         T *to = grad + r * sc.n;
 #pragma unroll
-        for (int e = 0; e < E; e += S::W) {
+        for (int e = 0; e < E; e += W) {
             const int j = S::place(g, e);
-            if (j + S::W <= n) __builtin_memcpy(to + j, out + e, S::W * sizeof(T));
+            if (j + W <= n) __builtin_memcpy(to + j, out + e, W * sizeof(T));
             else
 #pragma unroll
-                for (int k = 0; k < S::W; k++)
+                for (int k = 0; k < W; k++)
                     if (j + k < n) to[j + k] = out[e + k];
         }
     }
@@ -234,28 +331,31 @@ __device__ __forceinline__ double uniform_at(const void *uniforms, int bytes, in
     const double u = bytes == 8 ? ((const double *)uniforms)[r] : (double)((const float *)uniforms)[r];
     return u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;          // (NaN: 0)
 }
+struct Drawn {
+    int32_t *action;
+    float *log_prob, *entropy;          // either may be NULL
+    __device__ __forceinline__ void put(int64_t r, int a, float lp, float h) const {
+        action[r] = a;
+        if (log_prob) log_prob[r] = lp;
+        if (entropy) entropy[r] = h;
+    }
+};
 
 // Lane g holds the E consecutive scores from g * E on: a running sum in index order is a lane's sum, a scan over the lanes, and a second
 // look at the one lane in which the target lies.
-template <typename T, int G, int E>
-__global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void *uniforms, int uniform_bytes, int32_t *action,
-                                                        float *log_prob, float *entropy) {
-    constexpr int W = E % 8 == 0 ? 8 : E % 4 == 0 ? 4 : 1;
+template <typename T, int G, int E, int W>
+__global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out) {
     const int g = threadIdx.x % G, n = (int)sc.n;
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
+        const double u = uniform_at(uniforms, uniform_bytes, r);
         float x[E];
-#pragma unroll
-        for (int e = 0; e < E; e += W) {
-            float v[W];
-            load<W>(row, g * E + e, n, v);
-#pragma unroll
-            for (int k = 0; k < W; k++) x[e + k] = v[k];
+        {
+            Pieces<T, W, E / W> p;
+            p.load(row, n, n / (G * E) * (E / W), [&](int k) { return g * E + k * W; });
+            p.scores(row, x);
         }
-        float m = x[0];
-#pragma unroll
-        for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
-        m = group_all(m, G, f_max);
+        const float m = group_max<G>(lane_max(x));
         const bool some = m > NEG_INF;
         const double ref = some ? m : 0.0;
         double p[E], s = 0, t = 0;
@@ -263,40 +363,34 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 #pragma unroll
         for (int e = 0; e < E; e++) {
             nan |= x[e] != x[e];
-            const double d = fmax(((double)x[e] - ref) * sc.inv_t2_64, -1100.0);
+            const double d = below(x[e], ref, sc.inv_t2_64);
             p[e] = exp2_64(d);
             s += p[e];
             t = fma(p[e], d, t);
         }
-        double upto = s;          // the lanes' running sum, this one's included
-#pragma unroll
-        for (int o = 1; o < G; o <<= 1) {
-            const double v = __shfl_up(upto, o, G);
-            if (g >= o) upto += v;
-        }
-        const double total = __shfl(upto, G - 1, G);
-        t = group_all(t, G, [](double a, double b) { return a + b; });
-        const int first_lane = (threadIdx.x & 63) - g;
-        const uint64_t in_group = G == 64 ? ~0ull : ((1ull << (G & 63)) - 1) << first_lane;
+        const double upto = group_scan<G>(s, g), total = __shfl(upto, G - 1, G);
+        t = group_sum<G>(t);
+        const int group = (threadIdx.x & 63) - g;
+        const uint64_t in_group = G == 64 ? ~0ull : ((1ull << (G & 63)) - 1) << group;
         const bool undefined = (__ballot(nan) & in_group) || m == -NEG_INF, none = undefined || !some;
-        const double target = uniform_at(uniforms, uniform_bytes, r) * total;
+        const double target = u * total;
         // the first lane that passes the target, or else (rounding; a number of 1) the last one with anything in it
         const uint64_t past = __ballot(s > 0.0 && upto > target) & in_group, any = __ballot(s > 0.0) & in_group;
-        const int owner = none ? first_lane : past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)any);
+        const int owner = none ? group : past ? first_lane(past) : last_lane(any);
         if ((threadIdx.x & 63) == owner) {
-            double c = upto - s;
-            c = g == 0 ? 0.0 : c;
+            double c = g == 0 ? 0.0 : upto - s;
             int a = -1;
+            float xa = 0;
             bool found = false;
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 c += p[e];
-                if (p[e] > 0.0 && !found) { a = g * E + e; found = c > target; }
+                if (p[e] > 0.0 && !found) { a = g * E + e; xa = x[e]; found = c > target; }
             }
-            action[r] = none ? -1 : a;
-            if (log_prob)
-                log_prob[r] = undefined ? __builtin_nanf("") : some ? (float)(((double)row.at(a) - ref) * sc.inv_t2_64 * LN_2 - log(total)) : NEG_INF;
-            if (entropy) entropy[r] = undefined ? __builtin_nanf("") : some ? (float)(log(total) - t / total * LN_2) : 0.0f;
+            const double log_s = log(total);
+            const float nil = undefined ? __builtin_nanf("") : NEG_INF;
+            out.put(r, none ? -1 : a, none ? nil : (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s),
+                    undefined ? nil : some ? (float)(log_s - t / total * LN_2) : 0.0f);
         }
     }
 }
@@ -309,15 +403,9 @@ template <typename T> struct Tile {
     static constexpr int V = 16 / sizeof(T), U = 4, SIZE = BLOCK * U * V;
     // vector u of a tile in this thread: a wavefront's 64 vectors are neighbours, and its places ascend with the tile and u
     static __device__ __forceinline__ int64_t place(int64_t tile, int u) { return tile * SIZE + (u * BLOCK + (int)threadIdx.x) * V; }
-    static __device__ __forceinline__ void load_tile(const Row<T> &row, int64_t tile, int n, float (&x)[U][V]) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t j = place(tile, u);
-            if (j < n) load<V>(row, (int)j, n, x[u]);
-            else
-#pragma unroll
-                for (int k = 0; k < V; k++) x[u][k] = NEG_INF;
-        }
+    Pieces<T, V, U> p;
+    __device__ __forceinline__ void load(const Row<T> &row, int64_t tile, int n) {
+        p.load(row, n, (tile + 1) * SIZE <= n ? U : 0, [&](int u) { return (int)place(tile, u); });
     }
 };
 
@@ -337,31 +425,79 @@ struct Softmax {
         s += o.s;
         t += o.t;
     }
+    __device__ __forceinline__ void join_wave(float inv_t2) {
+        const float top = group_max<64>(m);
+        if (top > NEG_INF) to(top, inv_t2);
+        s = group_sum<64>(s);
+        t = group_sum<64>(t);
+    }
 };
 
-// The best k <= 64 scores a wavefront has seen, lane i the i-th best (score, index); -inf and -1 where there are fewer.
-struct Best {
-    float v = NEG_INF, last_v = NEG_INF;
-    int i = -1, last_i = -1, k;          // last: the k-th
-    __device__ explicit Best(int k_) : k(k_) {}
-    __device__ __forceinline__ bool wants(float x, int j) const { return better(x, j, last_v, last_i); }
-    // every lane offers one score (-inf: none)
-    __device__ __forceinline__ void offer(float x, int j) {
-        uint64_t who = __ballot(wants(x, j));
-        while (who) {
-            const int lane = __ffsll((unsigned long long)who) - 1;
-            const float cv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
-            const int ci = __builtin_amdgcn_readlane(j, lane);
-            const int at = __popcll(__ballot(better(v, i, cv, ci)));
-            const float sv = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x138, 0xf, 0xf, false));
-            const int si = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xf, 0xf, false);          // (one lane up)
-            const int me = threadIdx.x & 63;
-            v = me < at ? v : me == at ? cv : sv;
-            i = me < at ? i : me == at ? ci : si;
-            last_v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), k - 1));
-            last_i = __builtin_amdgcn_readlane(i, k - 1);
-            who &= ~(1ull << lane);
-            who &= __ballot(wants(x, j));
+// The best alternatives a wavefront has seen, as 64-bit keys: the score's order in the upper half (larger is better), the index's complement in
+// the lower (equal scores: the lower index).  0 is none.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);          // (+ 0: the two zeros are one score)
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float score_of(uint32_t order) { return __builtin_bit_cast(float, order ^ (order >> 31 ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ uint64_t key_of(float x, int j) { return x > NEG_INF ? (uint64_t)order_of(x) << 32 | (uint32_t)~j : 0; }
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+// It collects, in LDS and unsorted, whatever beats the k-th best it knows (k <= 64); when that gets full, and at the end, every key's rank is
+// counted and the k best stay, in order.  (Keeping a sorted list and pushing scores in one by one took five times as long: a chain of
+// dependent exchanges for each, and unrolled over a tile's 32 scores a lane more code than the instruction cache likes.)
+struct Top {
+    static constexpr int CAPACITY = 128;
+    uint64_t *keys;          // LDS [CAPACITY], the wavefront's own
+    uint64_t bound = 0;      // what a key has to exceed
+    int count = 0, k;
+    __device__ Top(uint64_t *lds, int k_) : keys(lds), k(k_) {}
+    // Before the first offers: `x` is one score that each lane is going to offer.  The k-th best of these 64 bounds the k-th best of all from
+    // below; found bit by bit (16 of them: the bound may be lower), it keeps most of the scores out that would not last.
+    __device__ __forceinline__ void expect(float x) {
+        const uint32_t order = x > NEG_INF ? order_of(x) >> 16 : 0;
+        uint32_t at_least = 0;
+        for (uint32_t bit = 0x8000; bit; bit >>= 1)
+            if (__popcll(__ballot(order >= (at_least | bit))) >= k) at_least |= bit;
+        if (at_least) bound = ((uint64_t)at_least << 48) - 1;
+    }
+    __device__ __forceinline__ float bound_score() const { return bound ? score_of((uint32_t)(bound >> 32)) : NEG_INF; }          // (none above it: no key beats it)
+    __device__ __forceinline__ static void sync() {          // LDS between the lanes of one wavefront
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    // every lane offers one key (0: none)
+    __device__ __forceinline__ void offer(uint64_t key) {
+        uint64_t who = __ballot(key > bound);
+        if (!who) return;
+        if (count + __popcll(who) > CAPACITY) {
+            sort();
+            who = __ballot(key > bound);
+        }
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        if (key > bound) keys[count + before] = key;
+        count += __popcll(who);
+        sync();
+    }
+    // the k best in order
+    __device__ __forceinline__ void sort() {
+        const int lane = threadIdx.x & 63;
+        const uint64_t a = lane < count ? keys[lane] : 0, b = lane + 64 < count ? keys[lane + 64] : 0;
+        int rank_a = 0, rank_b = 0;
+#pragma unroll 4
+        for (int c = 0; c < count; c++) {
+            const uint64_t other = keys[c];
+            rank_a += other > a;
+            rank_b += other > b;
+        }
+        sync();
+        if (a && rank_a < k) keys[rank_a] = a;
+        if (b && rank_b < k) keys[rank_b] = b;
+        sync();
+        if (count >= k) {
+            count = k;
+            bound = keys[k - 1];
         }
     }
 };
@@ -372,9 +508,9 @@ struct LogProbOut {
     int top;
 };
 
-// a row's results from its sums (one lane) and its best (one wavefront)
-template <typename T> __device__ void finish_row(const Scores<T> &sc, int64_t r, const Actions &actions, const Softmax &all, const Best &best,
-                                                 const LogProbOut &out) {
+// a row's results from its sums (one lane) and its best (one wavefront; sorted)
+template <typename T> __device__ __forceinline__ void finish_row(const Scores<T> &sc, int64_t r, const Actions &actions, const Softmax &all,
+                                                                 const Top &best, const LogProbOut &out) {
     const int lane = threadIdx.x & 63, n = (int)sc.n;
     const bool some = all.m > NEG_INF, undefined = !(all.s == all.s);
     const float ref = some ? all.m : 0.0f, log_s = logf(all.s), nan = __builtin_nanf("");
@@ -389,70 +525,67 @@ template <typename T> __device__ void finish_row(const Scores<T> &sc, int64_t r,
         if (out.stats) { out.stats[2 * r] = ref; out.stats[2 * r + 1] = log2f(all.s); }
     }
     if (lane < out.top) {
-        const bool there = best.i >= 0 && !undefined;
-        out.top_actions[r * out.top + lane] = there ? best.i : -1;
-        out.top_log_probs[r * out.top + lane] = there ? (best.v - ref) * sc.inv_t - log_s : NEG_INF;
+        const bool there = lane < best.count && !undefined;
+        const uint64_t key = there ? best.keys[lane] : 0;
+        out.top_actions[r * out.top + lane] = there ? index_of(key) : -1;
+        out.top_log_probs[r * out.top + lane] = there ? (score_of((uint32_t)(key >> 32)) - ref) * sc.inv_t - log_s : NEG_INF;
     }
 }
 
-// what one part of a row leaves for the join: its sums, and `top` best behind them
-__device__ __forceinline__ int part_words(int top) { return 4 + 2 * top; }
+// What the parts of a row leave for the join: [rows][parts][top] keys and [rows][parts][4] sums.
+struct Partials {
+    uint64_t *keys;
+    float *sums;
+};
 
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions actions, LogProbOut out, int parts, int64_t part_tiles,
-                                                          float *workspace) {
+// SPLIT: b-th part of part_tiles tiles of a row each, else whole rows
+template <typename T, bool TOP, bool SPLIT>
+__global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions actions, LogProbOut out, int parts, int part_tiles, Partials to) {
     using L = Tile<T>;
     __shared__ float lds[WAVES][3];
-    __shared__ float lds_v[WAVES][64];
-    __shared__ int lds_i[WAVES][64];
-    const int n = (int)sc.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, top = out.top;
-    for (int64_t b = blockIdx.x; b < sc.rows * parts; b += gridDim.x) {
-        const int64_t r = b / parts, part = b % parts;
+    __shared__ uint64_t lds_keys[TOP ? WAVES : 1][TOP ? Top::CAPACITY : 1];
+    __shared__ int lds_count[WAVES];
+    const int n = (int)sc.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, top = TOP ? out.top : 0;
+    const int tiles = (int)(((int64_t)n + L::SIZE - 1) / L::SIZE);
+    for (int64_t b = blockIdx.x; b < (SPLIT ? sc.rows * parts : sc.rows); b += gridDim.x) {
+        const int64_t r = SPLIT ? b / parts : b;
+        const int first = SPLIT ? (int)(b % parts) * part_tiles : 0, behind = SPLIT ? min(first + part_tiles, tiles) : tiles;
         const Row<T> row(sc, r);
-        const int64_t tiles = (n + L::SIZE - 1) / L::SIZE, first = part * part_tiles, behind = first + part_tiles < tiles ? first + part_tiles : tiles;
         Softmax a;
-        Best best(top ? top : 1);
-        for (int64_t tile = first; tile < behind; tile++) {
-            float x[L::U][L::V], um[L::U];
-            L::load_tile(row, tile, n, x);
-            float m = NEG_INF;
-#pragma unroll
-            for (int u = 0; u < L::U; u++) {
-                um[u] = x[u][0];
-#pragma unroll
-                for (int k = 1; k < L::V; k++) um[u] = fmaxf(um[u], x[u][k]);
-                m = fmaxf(m, um[u]);
-            }
+        Top best(lds_keys[TOP ? wave : 0], TOP ? top : 1);
+        for (int tile = first; tile < behind; tile++) {
+            L now;
+            now.load(row, tile, n);
+            float x[L::U * L::V], m;
+            now.p.scores(row, x);
+            m = lane_max(x);
             if (m > a.m) a.to(m, sc.inv_t2);
             const float ref = a.m > NEG_INF ? a.m : 0.0f;
 #pragma unroll
-            for (int u = 0; u < L::U; u++)
+            for (int k = 0; k < L::U * L::V; k++) {
+                const float d = (x[k] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
+                a.s += p;
+                a.t = fmaf(p, fmaxf(d, -1e30f), a.t);
+            }
+            if constexpr (TOP) {
+                if (tile == first) best.expect(m);
+                // (the wavefront's places ascend: a later tile's score that only equals the k-th best is behind it)
+                const float bound = best.bound_score();
+                if (__ballot(tile == first ? m >= bound : m > bound)) {
+                    uint32_t mine = 0;          // which of the lane's scores are in question; read again one by one, few as they are
 #pragma unroll
-                for (int k = 0; k < L::V; k++) {
-                    const float d = (x[u][k] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
-                    a.s += p;
-                    a.t = fmaf(p, fmaxf(d, -1e30f), a.t);
+                    for (int k = 0; k < L::U * L::V; k++) mine |= x[k] >= bound && x[k] > NEG_INF ? 1u << k : 0;          // (what is behind the end is -inf)
+                    while (__ballot(mine != 0)) {
+                        const int k = __ffs((int)mine) - 1, j = (int)L::place(tile, k / L::V) + k % L::V;
+                        best.offer(mine ? key_of(row.at(j), j) : 0);
+                        mine &= mine - 1;
+                    }
                 }
-            // (a later score that only equals the k-th best is behind it)
-            if (top && __ballot(m > best.last_v)) {
-#pragma unroll
-                for (int u = 0; u < L::U; u++)
-                    if (__ballot(um[u] > best.last_v))
-#pragma unroll
-                        for (int k = 0; k < L::V; k++) best.offer(x[u][k], (int)(L::place(tile, u) + k));
             }
         }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            Softmax other;
-            other.m = __shfl_xor(a.m, o);
-            other.s = __shfl_xor(a.s, o);
-            other.t = __shfl_xor(a.t, o);
-            a.join(other, sc.inv_t2);
-        }
+        a.join_wave(sc.inv_t2);
         __syncthreads();
-        if (lane == 0) { lds[wave][0] = a.m; lds[wave][1] = a.s; lds[wave][2] = a.t; }
-        if (top) { lds_v[wave][lane] = best.v; lds_i[wave][lane] = best.i; }
+        if (lane == 0) { lds[wave][0] = a.m; lds[wave][1] = a.s; lds[wave][2] = a.t; lds_count[wave] = best.count; }
         __syncthreads();
         if (wave == 0) {
             for (int w = 1; w < WAVES; w++) {
@@ -461,71 +594,65 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                 o.s = lds[w][1];
                 o.t = lds[w][2];
                 a.join(o, sc.inv_t2);
-                if (top) best.offer(lane < top ? lds_v[w][lane] : NEG_INF, lds_i[w][lane]);
+                if constexpr (TOP)
+                    for (int c = 0; c < lds_count[w]; c += 64) best.offer(c + lane < lds_count[w] ? lds_keys[w][c + lane] : 0);
             }
-            if (parts == 1) finish_row(sc, r, actions, a, best, out);
-            else {
-                float *to = workspace + b * part_words(top);
-                if (lane == 0) { to[0] = a.m; to[1] = a.s; to[2] = a.t; }
-                if (lane < top) { to[4 + lane] = best.v; to[4 + top + lane] = __builtin_bit_cast(float, best.i); }
-            }
+            if constexpr (TOP) best.sort();
+            if constexpr (SPLIT) {
+                if (lane == 0) { to.sums[b * 4] = a.m; to.sums[b * 4 + 1] = a.s; to.sums[b * 4 + 2] = a.t; }
+                if (lane < top) to.keys[b * top + lane] = lane < best.count ? best.keys[lane] : 0;
+            } else finish_row(sc, r, actions, a, best, out);
         }
+        __syncthreads();
     }
 }
 
 // one wavefront a row: the parts' sums and best
 template <typename T>
-__global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions actions, LogProbOut out, int parts, const float *workspace) {
+__global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions actions, LogProbOut out, int parts, Partials from) {
+    __shared__ uint64_t lds_keys[Top::CAPACITY];
     const int lane = threadIdx.x, top = out.top;
     for (int64_t r = blockIdx.x; r < sc.rows; r += gridDim.x) {
-        const float *from = workspace + r * parts * part_words(top);
+        const uint64_t *keys = from.keys + r * parts * top;
+        const float *sums = from.sums + r * parts * 4;
         Softmax a;
         for (int p = lane; p < parts; p += 64) {
-            const float *f = from + (int64_t)p * part_words(top);
             Softmax o;
-            o.m = f[0];
-            o.s = f[1];
-            o.t = f[2];
+            o.m = sums[p * 4];
+            o.s = sums[p * 4 + 1];
+            o.t = sums[p * 4 + 2];
             a.join(o, sc.inv_t2);
         }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            Softmax other;
-            other.m = __shfl_xor(a.m, o);
-            other.s = __shfl_xor(a.s, o);
-            other.t = __shfl_xor(a.t, o);
-            a.join(other, sc.inv_t2);
-        }
-        Best best(top ? top : 1);
-        for (int64_t c0 = 0; c0 < (int64_t)parts * top; c0 += 64) {
-            const int64_t c = c0 + lane;
-            float v = NEG_INF;
-            int i = -1;
-            if (c < (int64_t)parts * top) {
-                const float *f = from + c / top * part_words(top) + 4;
-                v = f[c % top];
-                i = __builtin_bit_cast(int, f[top + c % top]);
-            }
-            best.offer(v, i);
+        a.join_wave(sc.inv_t2);
+        Top best(lds_keys, top ? top : 1);
+        if (top) {
+            uint64_t most = 0;
+            for (int c = lane; c < parts * top; c += 64) most = keys[c] > most ? keys[c] : most;
+            best.expect(most ? score_of((uint32_t)(most >> 32)) : NEG_INF);
+            for (int c = 0; c < parts * top; c += 64) best.offer(c + lane < parts * top ? keys[c + lane] : 0);
+            best.sort();
         }
         finish_row(sc, r, actions, a, best, out);
+        Top::sync();
     }
 }
 
 template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions actions, const float *stats, const float *entropy, const float *g_lp,
-                                                         int64_t g_lp_stride, const float *g_h, int64_t g_h_stride, T *grad) {
+__global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions actions, const float *stats, const float *entropy, Upstream up,
+                                                         T *grad) {
     using L = Tile<T>;
     const int n = (int)sc.n;
     for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
         const Row<T> row(sc, r);
+        L tile;
+        tile.load(row, blockIdx.x, n);
         const int64_t a = actions.at(r);
         const float ref = stats[2 * r], log2_s = stats[2 * r + 1], h = entropy[r];
-        const float gl = g_lp && a >= 0 ? g_lp[r * g_lp_stride] : 0.0f, gh = g_h ? g_h[r * g_h_stride] : 0.0f;
+        const float gl = up.lp && a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
         // dx = p (c0 + c1 log2 p) + 1[j = a] g_lp / T
-        const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t;
-        float x[L::U][L::V];
-        L::load_tile(row, blockIdx.x, n, x);
+        const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t, at_a = gl * sc.inv_t;
+        float x[L::U * L::V];
+        tile.p.scores(row, x);
         T *to = grad + r * sc.n;
 #pragma unroll
         for (int u = 0; u < L::U; u++) {
@@ -534,10 +661,10 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
             T v[L::V];
 #pragma unroll
             for (int k = 0; k < L::V; k++) {
-                const float lp = (x[u][k] - ref) * sc.inv_t2 - log2_s, p = __builtin_amdgcn_exp2f(lp);
-                float g = p * fmaf(c1, fmaxf(lp, -1e30f), c0);
-                if (k == given) g += gl * sc.inv_t;
-                v[k] = from_f32<T>(x[u][k] == NEG_INF ? 0.0f : g);
+                const float xk = x[u * L::V + k], l2 = (xk - ref) * sc.inv_t2 - log2_s, p = __builtin_amdgcn_exp2f(l2);
+                float g = p * fmaf(c1, fmaxf(l2, -1e30f), c0);
+                if (k == given) g += at_a;
+                v[k] = from_f32<T>(xk == NEG_INF ? 0.0f : g);
             }
             if (j + L::V <= n) __builtin_memcpy(to + j, v, sizeof v);
             else
@@ -554,53 +681,47 @@ struct Segment {
     float m;            // its maximum (-inf: nothing open)
     int nan;
 };
-__device__ __forceinline__ double wave_sum(double v) { return wave_all(v, [](double a, double b) { return a + b; }); }
+constexpr int LDS_SEGMENTS = 512;          // as many are looked at in LDS
 
 // the four segments of a wavefront's part of a tile: (tile, u, wave) is segment (tile * U + u) * WAVES + wave
 template <typename T> __device__ __forceinline__ void sum_segments(const Scores<T> &sc, const Row<T> &row, int64_t tile, int64_t segments, Segment *to) {
     using L = Tile<T>;
     const int n = (int)sc.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float x[L::U][L::V];
-    L::load_tile(row, tile, n, x);
-    float m = NEG_INF;
+    L now;
+    now.load(row, tile, n);
+    float x[L::U * L::V];
+    now.p.scores(row, x);
     bool nan = false;
 #pragma unroll
-    for (int u = 0; u < L::U; u++)
-#pragma unroll
-        for (int k = 0; k < L::V; k++) {
-            m = fmaxf(m, x[u][k]);
-            nan |= x[u][k] != x[u][k];
-        }
-    m = wave_all(m, f_max);
+    for (int k = 0; k < L::U * L::V; k++) nan |= x[k] != x[k];
+    const float m = group_max<64>(lane_max(x));
     const double ref = m > NEG_INF ? m : 0.0;
     double t = 0;
     const int any_nan = __ballot(nan) != 0;
+    int64_t last = -1;
 #pragma unroll
     for (int u = 0; u < L::U; u++) {
+        const int64_t seg = (tile * L::U + u) * WAVES + wave;
+        if (seg >= segments) break;
         double s = 0;
 #pragma unroll
         for (int k = 0; k < L::V; k++) {
-            const double d = fmax(((double)x[u][k] - ref) * sc.inv_t2_64, -1100.0), p = exp2_64(d);
+            const double d = below(x[u * L::V + k], ref, sc.inv_t2_64), p = exp2_64(d);
             s += p;
             t = fma(p, d, t);
         }
-        s = wave_sum(s);
-        if (u == L::U - 1) t = wave_sum(t);
-        const int64_t seg = (tile * L::U + u) * WAVES + wave;
-        // (the tile's t, all against one maximum, goes with its last segment that there is)
-        if (lane == 0 && seg < segments) to[seg] = {s, 0.0, m, any_nan};
+        s = group_sum<64>(s);
+        if (lane == 0) to[seg] = {s, 0.0, m, any_nan};
+        last = seg;
     }
-    if (lane == 0) {
-        int64_t seg = (tile * L::U + L::U - 1) * WAVES + wave;
-        while (seg >= segments) seg -= WAVES;
-        if (seg >= tile * L::U * WAVES) to[seg].t = t;
-    }
+    // (t of the four, all against one maximum, goes with the last of them)
+    t = group_sum<64>(t);
+    if (lane == 0 && last >= 0) to[last].t = t;
 }
 
 // One wavefront: the row's action from its segments.
 template <typename T>
-__device__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t segments, const void *uniforms, int uniform_bytes, int32_t *action,
-                     float *log_prob, float *entropy) {
+__device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t segments, double u, const Drawn &out) {
     constexpr int V = Tile<T>::V;
     const int lane = threadIdx.x & 63, n = (int)sc.n;
     const Row<T> row(sc, r);
@@ -609,19 +730,15 @@ __device__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t
     float m = NEG_INF;
     int nan = 0;
     for (int64_t g = lo; g < hi; g++) { m = fmaxf(m, seg[g].m); nan |= seg[g].nan; }
-    m = wave_all(m, f_max);
+    m = group_max<64>(m);
     const bool some = m > NEG_INF, undefined = __ballot(nan) || m == -NEG_INF;
     if (undefined || !some) {
-        if (lane == 0) {
-            action[r] = -1;
-            if (log_prob) log_prob[r] = undefined ? __builtin_nanf("") : NEG_INF;
-            if (entropy) entropy[r] = undefined ? __builtin_nanf("") : 0.0f;
-        }
+        if (lane == 0) out.put(r, -1, undefined ? __builtin_nanf("") : NEG_INF, undefined ? __builtin_nanf("") : 0.0f);
         return;
     }
     const double ref = m;
     const auto weight = [&](const Segment &g, double &d) {
-        d = fmax(((double)g.m - ref) * sc.inv_t2_64, -1100.0);
+        d = below(g.m, ref, sc.inv_t2_64);
         return exp2_64(d);
     };
     double s = 0, t = 0;
@@ -631,21 +748,16 @@ __device__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t
         s += w * seg[g].s;
         t += w * fma(d, seg[g].s, seg[g].t);
     }
-    double upto = s;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(upto, o);
-        if (lane >= o) upto += v;
-    }
-    const double total = __shfl(upto, 63);
-    t = wave_sum(t);
-    const double target = uniform_at(uniforms, uniform_bytes, r) * total;
+    double upto = group_scan<64>(s, lane);
+    const double total = lane_of(upto, 63);
+    t = group_sum<64>(t);
+    const double target = u * total;
     // the first run that passes the target, or else (rounding; a number of 1) the last one with anything in it; then the segment in it
     uint64_t past = __ballot(s > 0.0 && upto > target), any = __ballot(s > 0.0);
-    const int run = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)any);
-    double before = __shfl(lane == 0 ? 0.0 : upto - s, run);
-    int64_t found = -1;
-    double found_before = 0;
-    for (int64_t g = run * each; g < (run + 1) * each && g < segments; g++) {
+    const int run = past ? first_lane(past) : last_lane(any);
+    double before = lane_of(lane == 0 ? 0.0 : upto - s, run), found_before = 0;
+    int64_t found = run * each;
+    for (int64_t g = found; g < (run + 1) * each && g < segments; g++) {
         double d;
         const double w = weight(seg[g], d) * seg[g].s;
         if (w > 0.0) { found = g; found_before = before; }
@@ -653,24 +765,19 @@ __device__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t
         if (w > 0.0 && before > target) break;
     }
     // ... and the action in the segment
-    float x[V];
     const int64_t j = (found * 64 + lane) * V;
-    if (j < n) load<V>(row, (int)j, n, x);
-    else
-#pragma unroll
-        for (int k = 0; k < V; k++) x[k] = NEG_INF;
+    Pieces<T, V, 1> piece;
+    piece.load(row, n, 0, [&](int) { return (int)j; });
+    float x[V];
+    piece.scores(row, x);
     double p[V];
     s = 0;
 #pragma unroll
     for (int k = 0; k < V; k++) {
-        p[k] = exp2_64(((double)x[k] - ref) * sc.inv_t2_64);
+        p[k] = exp2_64(below(x[k], ref, sc.inv_t2_64));
         s += p[k];
     }
-    upto = s;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(upto, o);
-        if (lane >= o) upto += v;
-    }
+    upto = group_scan<64>(s, lane);
     past = __ballot(s > 0.0 && found_before + upto > target);
     any = __ballot(s > 0.0);
     const bool tiny = !any;          // (the segment's sum is above 0 and all its terms round to it: the first one that is open)
@@ -680,7 +787,7 @@ __device__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t
         for (int k = 0; k < V; k++) open |= x[k] > NEG_INF;
         past = __ballot(open);
     }
-    const int owner = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)any);
+    const int owner = past ? first_lane(past) : last_lane(any);
     if (lane == owner) {
         double c = found_before + (lane == 0 ? 0.0 : upto - s);
         int a = -1;
@@ -691,34 +798,44 @@ __device__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t
             c += p[k];
             if ((tiny ? x[k] > NEG_INF : p[k] > 0.0) && !done) { a = (int)j + k; xa = x[k]; done = tiny || c > target; }
         }
-        action[r] = a;
-        if (log_prob) log_prob[r] = (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log(total));
-        if (entropy) entropy[r] = (float)(log(total) - t / total * LN_2);
+        const double log_s = log(total);
+        out.put(r, a, (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s), (float)(log_s - t / total * LN_2));
     }
 }
 
 // parts == 1: a workgroup sums a row's segments and its first wavefront draws; else only the sums, for k_draw
 template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_sample_long(Scores<T> sc, const void *uniforms, int uniform_bytes, int32_t *action, float *log_prob,
-                                                       float *entropy, int parts, int64_t part_tiles, int64_t segments, Segment *workspace) {
+__global__ __launch_bounds__(BLOCK, 4) void k_sample_long(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out, int parts,
+                                                          int part_tiles, int64_t segments, Segment *workspace) {
     using L = Tile<T>;
+    __shared__ Segment lds[LDS_SEGMENTS];
     const int64_t tiles = (sc.n + L::SIZE - 1) / L::SIZE;
     for (int64_t b = blockIdx.x; b < sc.rows * parts; b += gridDim.x) {
         const int64_t r = b / parts, first = b % parts * part_tiles, behind = first + part_tiles < tiles ? first + part_tiles : tiles;
         const Row<T> row(sc, r);
-        Segment *seg = workspace + r * segments;
+        Segment *seg = workspace ? workspace + r * segments : lds;
         for (int64_t tile = first; tile < behind; tile++) sum_segments(sc, row, tile, segments, seg);
         if (parts == 1) {
             __syncthreads();
-            if (threadIdx.x < 64) draw(sc, r, seg, segments, uniforms, uniform_bytes, action, log_prob, entropy);
+            if (threadIdx.x < 64) draw(sc, r, seg, segments, uniform_at(uniforms, uniform_bytes, r), out);
+            __syncthreads();
         }
     }
 }
 template <typename T>
-__global__ __launch_bounds__(64) void k_draw(Scores<T> sc, const void *uniforms, int uniform_bytes, int32_t *action, float *log_prob, float *entropy,
-                                             int64_t segments, const Segment *workspace) {
-    for (int64_t r = blockIdx.x; r < sc.rows; r += gridDim.x)
-        draw(sc, r, workspace + r * segments, segments, uniforms, uniform_bytes, action, log_prob, entropy);
+__global__ __launch_bounds__(BLOCK) void k_draw(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out, int64_t segments,
+                                                const Segment *workspace) {
+    __shared__ Segment lds[LDS_SEGMENTS];
+    for (int64_t r = blockIdx.x; r < sc.rows; r += gridDim.x) {
+        const Segment *seg = workspace + r * segments;
+        if (segments <= LDS_SEGMENTS) {
+            for (int g = threadIdx.x; g < segments; g += BLOCK) lds[g] = seg[g];
+            seg = lds;
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) draw(sc, r, seg, segments, uniform_at(uniforms, uniform_bytes, r), out);
+        __syncthreads();
+    }
 }
 
 thread_local char g_err[256] = "";          // (no allocation: nothing may throw across the C boundary)
@@ -766,46 +883,71 @@ template <typename... P, typename... A> int launch(void (*kernel)(P...), int64_t
 }
 
 constexpr int SHORT_MAX = 2048;
-template <int G_, int E_> struct Shape { static constexpr int G = G_, E = E_; };
-// f(lanes a row and scores a lane) for rows of n <= SHORT_MAX: the fewest lanes that keep 4 ... 8 scores each, then a whole wavefront
-template <typename F> int by_length(int64_t n, F f) {
-    if (n <= 32)
-        switch ((n + 3) / 4) {
-            case 1: return f(Shape<4, 1>());
-            case 2: return f(Shape<4, 2>());
-            case 3: return f(Shape<4, 3>());
-            case 4: return f(Shape<4, 4>());
-            case 5: return f(Shape<4, 5>());
-            case 6: return f(Shape<4, 6>());
-            case 7: return f(Shape<4, 7>());
-            default: return f(Shape<4, 8>());
-        }
-    if (n <= 48) return f(Shape<8, 6>());
-    if (n <= 64) return f(Shape<8, 8>());
-    if (n <= 96) return f(Shape<16, 6>());
-    if (n <= 128) return f(Shape<16, 8>());
-    if (n <= 192) return f(Shape<32, 6>());
-    if (n <= 256) return f(Shape<32, 8>());
-    if (n <= 384) return f(Shape<64, 6>());
-    if (n <= 512) return f(Shape<64, 8>());
-    if (n <= 768) return f(Shape<64, 12>());
-    if (n <= 1024) return f(Shape<64, 16>());
-    if (n <= 1536) return f(Shape<64, 24>());
-    return f(Shape<64, 32>());
+template <int G_, int E_, int W_> struct Shape { static constexpr int G = G_, E = E_, W = W_; };
+// f(lanes a row, scores a lane, scores a load) for rows of n <= SHORT_MAX: up to 32 scores in one lane (no exchanges at all); beyond, the
+// fewest lanes that hold the row in four 16-byte pieces each, or all 64.
+template <typename T, int G, typename F> int by_pieces(int64_t n, F f) {
+    constexpr int W = 16 / sizeof(T);
+    const int64_t c = (n + G * W - 1) / (G * W);
+    if constexpr (G == 4) if (c <= 2) return f(Shape<G, 2 * W, W>());
+    if (c <= 3) return f(Shape<G, 3 * W, W>());
+    if constexpr (G < 64 || sizeof(T) == 2) return f(Shape<G, 4 * W, W>());
+    else {
+        if (c <= 4) return f(Shape<G, 4 * W, W>());
+        if (c <= 6) return f(Shape<G, 6 * W, W>());
+        return f(Shape<G, 8 * W, W>());
+    }
+}
+template <typename T, typename F> int by_lanes(int64_t n, F f) {
+    const int64_t lanes = (n + 64 / sizeof(T) - 1) / (64 / sizeof(T));
+    if (lanes <= 4) return by_pieces<T, 4>(n, f);
+    if (lanes <= 8) return by_pieces<T, 8>(n, f);
+    if (lanes <= 16) return by_pieces<T, 16>(n, f);
+    if (lanes <= 32) return by_pieces<T, 32>(n, f);
+    return by_pieces<T, 64>(n, f);
+}
+template <typename T, typename F> int by_length(int64_t n, F f) {
+    constexpr int W = 16 / sizeof(T);
+    if (n > 32) return by_lanes<T>(n, f);
+    if (n <= 8) return f(Shape<1, 8, W>());
+    if constexpr (W == 4) if (n <= 12) return f(Shape<1, 12, W>());
+    if (n <= 16) return f(Shape<1, 16, W>());
+    if constexpr (W == 4) if (n <= 20) return f(Shape<1, 20, W>());
+    if (n <= 24) return f(Shape<1, 24, W>());
+    if constexpr (W == 4) if (n <= 28) return f(Shape<1, 28, W>());
+    return f(Shape<1, 32, W>());
+}
+// Drawing: up to 32 scores over four lanes (64-bit exponentials take twenty times what an exchange takes)
+template <typename T, typename F> int by_length_64(int64_t n, F f) {
+    if (n > 32) return by_lanes<T>(n, f);
+    switch ((n + 3) / 4) {
+        case 1: return f(Shape<4, 1, 1>());
+        case 2: return f(Shape<4, 2, 1>());
+        case 3: return f(Shape<4, 3, 1>());
+        case 4: return f(Shape<4, 4, 1>());
+        case 5: return f(Shape<4, 5, 1>());
+        case 6: return f(Shape<4, 6, 1>());
+        case 7: return f(Shape<4, 7, 1>());
+        default: return f(Shape<4, 8, 1>());
+    }
 }
 // How many workgroups share a long row: enough to give every one of the 256 CUs some, no more than the row has tiles.
 struct Split {
-    int parts;
-    int64_t part_tiles;
+    int parts, part_tiles;
 };
 Split split(int dtype, int64_t rows, int64_t n) {
     const int64_t size = dtype == MGX_REAL_F32 ? Tile<float>::SIZE : Tile<half>::SIZE, tiles = (n + size - 1) / size;
     const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(tiles, 1024 / std::max<int64_t>(rows, 1))), each = (tiles + wanted - 1) / wanted;
-    return {(int)((tiles + each - 1) / each), each};
+    return {(int)((tiles + each - 1) / each), (int)each};
 }
 int64_t n_segments(int dtype, int64_t n) {
     const int64_t size = 64 * (dtype == MGX_REAL_F32 ? Tile<float>::V : Tile<half>::V);
     return (n + size - 1) / size;
+}
+
+int64_t sample_workspace(int dtype, int64_t rows, int64_t n) {
+    const int64_t segments = n_segments(dtype, n);
+    return split(dtype, rows, n).parts == 1 && segments <= LDS_SEGMENTS ? 0 : rows * segments * (int64_t)sizeof(Segment);
 }
 
 int64_t short_blocks(int64_t rows, int G) { return (rows * G + BLOCK - 1) / BLOCK; }
@@ -827,9 +969,9 @@ const char *mgx_policy_last_error(void) { return g_err; }
 
 int64_t mgx_policy_workspace_bytes(int op, int dtype, int64_t rows, int64_t n, int top) {
     if (n <= SHORT_MAX || rows <= 0) return 0;
-    if (op == MGX_POLICY_SAMPLE) return rows * n_segments(dtype, n) * (int64_t)sizeof(Segment);
+    if (op == MGX_POLICY_SAMPLE) return sample_workspace(dtype, rows, n);
     const Split sp = split(dtype, rows, n);
-    return sp.parts == 1 ? 0 : rows * sp.parts * (4 + 2 * (int64_t)top) * 4;
+    return sp.parts == 1 ? 0 : rows * sp.parts * (16 + 8 * (int64_t)top);
 }
 
 int64_t mgx_policy_stats_bytes(int64_t rows, int64_t n) { return n > SHORT_MAX ? rows * 8 : 0; }
@@ -847,21 +989,25 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
     if (!actions || !log_prob || !entropy || (top && (!top_log_probs || !top_actions))) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
+    const Actions given{actions, action_bytes};
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (n <= SHORT_MAX)
-            return by_length(n, [&](auto shape) {
-                constexpr int G = decltype(shape)::G, E = decltype(shape)::E;
-                return launch(k_log_probs_short<T, G, E>, short_blocks(rows, G), BLOCK, stream, sc, Actions{actions, action_bytes}, top,
+            return by_length<T>(n, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
+                return launch(k_log_probs_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, top,
                               log_prob, entropy, top_log_probs, top_actions);
             });
         const Split sp = split(dtype, rows, n);
         const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_actions, top};
-        const Actions given{actions, action_bytes};
-        const int rc = launch(k_log_probs_long<T>, rows * sp.parts, BLOCK, stream, sc, given, out, sp.parts, sp.part_tiles, (float *)workspace);
-        if (rc || sp.parts == 1) return rc;
-        return launch(k_log_probs_join<T>, rows, 64, stream, sc, given, out, sp.parts, (const float *)workspace);
+        const Partials partials{(uint64_t *)workspace, workspace ? (float *)((uint64_t *)workspace + rows * sp.parts * top) : nullptr};
+        if (sp.parts == 1)
+            return launch(top ? k_log_probs_long<T, true, false> : k_log_probs_long<T, false, false>, rows, BLOCK, stream, sc, given, out, 1, 0, partials);
+        if (const int rc = launch(top ? k_log_probs_long<T, true, true> : k_log_probs_long<T, false, true>, rows * sp.parts, BLOCK, stream, sc, given,
+                                  out, sp.parts, sp.part_tiles, partials))
+            return rc;
+        return launch(k_log_probs_join<T>, rows, 64, stream, sc, given, out, sp.parts, partials);
     });
 }
 
@@ -877,18 +1023,18 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
     if (!actions || (!stats && mgx_policy_stats_bytes(rows, n)) || !entropy || !grad) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
+    const Actions given{actions, action_bytes};
+    const Upstream up{grad_log_prob, grad_entropy, grad_log_prob_stride, grad_entropy_stride};
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (n <= SHORT_MAX)
-            return by_length(n, [&](auto shape) {
-                constexpr int G = decltype(shape)::G, E = decltype(shape)::E;
-                return launch(k_backward_short<T, G, E>, short_blocks(rows, G), BLOCK, stream, sc, Actions{actions, action_bytes}, entropy,
-                              grad_log_prob, grad_log_prob_stride, grad_entropy, grad_entropy_stride, (T *)grad);
+            return by_length_64<T>(n, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
+                return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad);
             });
         return launch(k_backward_long<T>, dim3((unsigned)((n + Tile<T>::SIZE - 1) / Tile<T>::SIZE), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
-                      stream, sc, Actions{actions, action_bytes}, stats, entropy, grad_log_prob, grad_log_prob_stride, grad_entropy,
-                      grad_entropy_stride, (T *)grad);
+                      stream, sc, given, stats, entropy, up, (T *)grad);
     });
 }
 
@@ -903,21 +1049,21 @@ int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, i
     if (!uniforms || !action) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
+    const Drawn out{action, log_prob, entropy};
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (n <= SHORT_MAX)
-            return by_length(n, [&](auto shape) {
-                constexpr int G = decltype(shape)::G, E = decltype(shape)::E;
-                return launch(k_sample_short<T, G, E>, short_blocks(rows, G), BLOCK, stream, sc, uniforms, uniform_bytes, action, log_prob,
-                              entropy);
+            return by_length_64<T>(n, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
+                return launch(k_sample_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, uniforms, uniform_bytes, out);
             });
         const Split sp = split(dtype, rows, n);
         const int64_t segments = n_segments(dtype, n);
-        const int rc = launch(k_sample_long<T>, rows * sp.parts, BLOCK, stream, sc, uniforms, uniform_bytes, action, log_prob, entropy, sp.parts,
-                              sp.part_tiles, segments, (Segment *)workspace);
+        Segment *const ws = sample_workspace(dtype, rows, n) ? (Segment *)workspace : nullptr;
+        const int rc = launch(k_sample_long<T>, rows * sp.parts, BLOCK, stream, sc, uniforms, uniform_bytes, out, sp.parts, sp.part_tiles, segments, ws);
         if (rc || sp.parts == 1) return rc;
-        return launch(k_draw<T>, rows, 64, stream, sc, uniforms, uniform_bytes, action, log_prob, entropy, segments, (const Segment *)workspace);
+        return launch(k_draw<T>, rows, BLOCK, stream, sc, uniforms, uniform_bytes, out, segments, (const Segment *)ws);
     });
 }
 
