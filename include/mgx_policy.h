@@ -10,7 +10,7 @@
  *
  * The scores: `logits` points at element (0, 0) of rows x n values of type `dtype` (mgx_real), value (r, j) at r * row_stride + j
  * (elements; any stride >= 0: rows may overlap or coincide, as an expanded tensor's do; no alignment beyond the element's).  `mask`:
- * NULL, or u8 at r * mask_row_stride + j, 0 = action j is ruled out in row r.  An action is OPEN if its mask is not 0 and its
+ * NULL, or u8 at r * mask_row_stride + j: 1, or 0 = action j is ruled out in row r.  An action is OPEN if its mask is not 0 and its
  * score is not -inf.  With the open scores x, m = max x, T = temperature:
  *     d_j = (x_j - m) / T,  s = sum e^d_j,   log p_j = d_j - log s,   entropy H = -sum p_j log p_j = log s - (sum d_j e^d_j) / s
  *   - an action that is not open has log p = -inf, takes no part in H and gets gradient 0;
@@ -53,7 +53,7 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
                                   int64_t grad_log_prob_stride, const float *grad_entropy, int64_t grad_entropy_stride, void *grad,
                                   void *stream);
 /* one action per row: the first j with p_0 + ... + p_j > u, u = uniforms[r] (f32 or f64: uniform_bytes 4 or 8) in [0, 1); a u below 0
- * or NaN counts as 0, a u of 1 or more draws the last action of non-zero probability.  action: i32 [rows]; log_prob, entropy: f32 [rows]
+ * or NaN counts as 0, a u of 1 or more draws the last action that can be drawn.  A probability below 2^-990 is none.  action: i32 [rows]; log_prob, entropy: f32 [rows]
  * (either may be NULL). */
 int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride, const uint8_t *mask,
                       int64_t mask_row_stride, double temperature, const void *uniforms, int uniform_bytes, int32_t *action,

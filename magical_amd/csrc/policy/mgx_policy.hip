@@ -38,6 +38,9 @@ template <typename T> struct Row {
     }
 };
 
+// The larger of two; a NaN wins.  (fmaxf would quiet each operand first, an instruction a score; two of these are one on gfx950.)
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 struct Actions {
     const void *p;
     int bytes;
@@ -99,17 +102,27 @@ template <typename T, int W, int N> struct Pieces {
         else if constexpr (std::is_same_v<T, half>) return (float)__builtin_bit_cast(half, (uint16_t)(w[p][k / 2] >> (k % 2 * 16)));
         else return __builtin_bit_cast(float, k % 2 ? w[p][k / 2] & 0xffff0000u : w[p][k / 2] << 16);
     }
-    // the N * W scores in fp32, -inf where the mask rules them out
-    __device__ __forceinline__ void scores(const Row<T> &row, float *x) const {
-#pragma unroll
-        for (int p = 0; p < N; p++)
-#pragma unroll
-            for (int k = 0; k < W; k++) x[p * W + k] = score(p, k);
+    // the N * W scores in fp32, -inf where the mask rules them out (its bytes are 0 or 1: spread to all bits, they select)
+    __device__ __forceinline__ void scores(const Row<T> &row, float *x) {
         if (row.mask)
 #pragma unroll
             for (int p = 0; p < N; p++)
 #pragma unroll
-                for (int k = 0; k < W; k++) x[p * W + k] = open[p][k / 4] >> (k % 4 * 8) & 0xff ? x[p * W + k] : NEG_INF;
+                for (int k = 0; k < WORDS; k++) {
+                    uint32_t all;
+                    if constexpr (sizeof(T) == 4) all = (uint32_t)((int32_t)(open[p][k / 4] << (31 - k % 4 * 8)) >> 31);
+                    else {
+                        using Two16 = short __attribute__((ext_vector_type(2)));
+                        const Two16 ones = __builtin_bit_cast(Two16, __builtin_amdgcn_perm(0, open[p][k / 2], k % 2 ? 0x0c030c02 : 0x0c010c00));
+                        all = __builtin_bit_cast(uint32_t, -ones);
+                    }
+                    constexpr uint32_t closed = sizeof(T) == 4 ? neg_inf_bits<T> : neg_inf_bits<T> << 16 | neg_inf_bits<T>;
+                    w[p][k] = (all & w[p][k]) | (~all & closed);
+                }
+#pragma unroll
+        for (int p = 0; p < N; p++)
+#pragma unroll
+            for (int k = 0; k < W; k++) x[p * W + k] = score(p, k);
     }
 };
 
@@ -148,7 +161,7 @@ template <int G, typename V, typename F> __device__ __forceinline__ V group_all(
     if constexpr (G > 32) { const Two<V> t = swap<32>(v); v = f(t.a, t.b); }
     return v;
 }
-template <int G> __device__ __forceinline__ float group_max(float v) { return group_all<G>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int G> __device__ __forceinline__ float group_max(float v) { return group_all<G>(v, [](float a, float b) { return max_of(a, b); }); }
 template <int G, typename V> __device__ __forceinline__ V group_sum(V v) { return group_all<G>(v, [](V a, V b) { return a + b; }); }
 // running sum over the G lanes of a group, this lane (number g) included
 template <int G> __device__ __forceinline__ double group_scan(double v, int g) {
@@ -173,28 +186,40 @@ __device__ __forceinline__ int last_lane(uint64_t b) { return 63 - __clzll((long
 // is (v, i) a better alternative than (w, k)?  Higher score first, then the lower index.
 __device__ __forceinline__ bool better(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
 
-// 2^y for -1100 <= y <= 0 in 64 bits: y = k + f with |f| <= 1 / 2 (k by adding 1.5 * 2^52, whose last bits then are k), a polynomial for 2^f
-// (interpolated at the Chebyshev points of [-1/2, 1/2] in 60 digits: off by 3.1e-16 at most), k added to its exponent; 0 for k below -1000.
-__device__ __forceinline__ double exp2_64(double y) {
-    const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
-    const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, shifted);
-    double p = 0x1.e6063f7217bc6p-28;
-    p = fma(p, f, 0x1.b675bca4eeebbp-24);
-    p = fma(p, f, 0x1.62bfd47773353p-20);
-    p = fma(p, f, 0x1.ffcb54062e698p-17);
-    p = fma(p, f, 0x1.430913096fd9fp-13);
-    p = fma(p, f, 0x1.5d87fe9d7a584p-10);
-    p = fma(p, f, 0x1.3b2ab6fba1ddap-7);
-    p = fma(p, f, 0x1.c6b08d703ce49p-5);
-    p = fma(p, f, 0x1.ebfbdff82c598p-3);
-    p = fma(p, f, 0x1.62e42fefa3a19p-1);
-    p = fma(p, f, 1.0);
-    const uint64_t b = __builtin_bit_cast(uint64_t, p);
-    const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)k << 20);
-    return k < -1000 ? 0.0 : __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
+// a * b + c with c in scalar registers.  (The compiler would copy the constant into vector registers first, two moves a step.)
+__device__ __forceinline__ double fma_64(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
 }
-// (x - ref) inv_t2 for it: -inf and whatever else 2^y is 0 for at -1100.  (A NaN too: the callers look for those themselves.)
-__device__ __forceinline__ double below(float x, double ref, double inv_t2) { return fmax(((double)x - ref) * inv_t2, -1100.0); }
+// For drawing: scores as differences to a maximum, in 64 bits, and 2^(d * inv_t2) of them.  A difference below 2^-1000's counts as that, -inf
+// and NaN too (the callers look for NaN themselves), and what is below NOTHING as no probability at all.
+constexpr double NOTHING = 0x1p-990;
+struct Exp64 {
+    double inv_t2, least;
+    __device__ __forceinline__ explicit Exp64(double inv_t2_) : inv_t2(inv_t2_), least(-1000.0 / inv_t2_) {}
+    __device__ __forceinline__ double below(float x, double ref) const { return fmax((double)x - ref, least); }
+    // y = d * inv_t2 = k + f with |f| <= 1 / 2 (k by adding 1.5 * 2^52, whose last bits then are k); a polynomial for 2^f (interpolated at the
+    // Chebyshev points of [-1/2, 1/2] in 60 digits: off by 3.1e-16 at most); k added to its exponent
+    __device__ __forceinline__ double operator()(double d) const {
+        const double shifted = fma_64(d, inv_t2, 0x1.8p52), f = fma(d, inv_t2, 0x1.8p52 - shifted);
+        using Words = uint32_t __attribute__((ext_vector_type(2)));
+        double p = 0x1.e6063f7217bc6p-28;
+        p = fma_64(p, f, 0x1.b675bca4eeebbp-24);
+        p = fma_64(p, f, 0x1.62bfd47773353p-20);
+        p = fma_64(p, f, 0x1.ffcb54062e698p-17);
+        p = fma_64(p, f, 0x1.430913096fd9fp-13);
+        p = fma_64(p, f, 0x1.5d87fe9d7a584p-10);
+        p = fma_64(p, f, 0x1.3b2ab6fba1ddap-7);
+        p = fma_64(p, f, 0x1.c6b08d703ce49p-5);
+        p = fma_64(p, f, 0x1.ebfbdff82c598p-3);
+        p = fma_64(p, f, 0x1.62e42fefa3a19p-1);
+        p = fma_64(p, f, 1.0);
+        Words w = __builtin_bit_cast(Words, p);
+        w.y += __builtin_bit_cast(Words, shifted).x << 20;
+        return __builtin_bit_cast(double, w);
+    }
+};
 constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
@@ -211,7 +236,7 @@ template <int G, int E, int W> struct Spread {
 template <int E> __device__ __forceinline__ float lane_max(const float (&x)[E]) {
     float m = x[0];
 #pragma unroll
-    for (int e = 1; e < E; e++) m = fmaxf(m, x[e]);
+    for (int e = 1; e < E; e++) m = max_of(m, x[e]);
     return m;
 }
 
@@ -279,6 +304,8 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
     }
 }
 
+__device__ __forceinline__ bool finite(float a, float b) { return fabsf(a) < __builtin_inff() && fabsf(b) < __builtin_inff(); }
+
 struct Upstream {          // gradients to the log probabilities and entropies, one value a row (stride 0: one for all), or NULL
     const float *lp, *h;
     int64_t lp_stride, h_stride;
@@ -303,26 +330,28 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
             s += p[e];
         }
         s = group_sum<G>(s);
-        // dx = p (c0 + c1 log2 p) + 1[j = a] g_lp / T
+        // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a
         const float inv_s = 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
-        const float at_a = gl * sc.inv_t;
-        const int ai = a >= 0 && a < n ? (int)a : -1;
-        T out[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const float l2 = (x[e] - ref) * sc.inv_t2 - log2_s;
-            const float v = p[e] * fmaf(c1, fmaxf(l2, -1e30f), c0) + (S::place(g, e) == ai ? at_a : 0.0f);
-            out[e] = from_f32<T>(x[e] == NEG_INF ? 0.0f : v);
-        }
         T *to = grad + r * sc.n;
 #pragma unroll
         for (int e = 0; e < E; e += W) {
+            T out[W];
+#pragma unroll
+            for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf((x[e + k] - ref) * sc.inv_t2 - log2_s, -1e30f), c0));
             const int j = S::place(g, e);
-            if (j + W <= n) __builtin_memcpy(to + j, out + e, W * sizeof(T));
+            if (e / W < n / (G * W) || j + W <= n) __builtin_memcpy(to + j, out, sizeof out);
             else
 #pragma unroll
                 for (int k = 0; k < W; k++)
-                    if (j + k < n) to[j + k] = out[e + k];
+                    if (j + k < n) to[j + k] = out[k];
+        }
+        if (!finite(c0, c1))          // NaN, but for the places that are not open
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (S::place(g, e) < n && x[e] == NEG_INF) to[S::place(g, e)] = from_f32<T>(0.0f);
+        if (a >= 0 && a < n && (int)(a / W) % G == g) {          // (the lane that has just written this place)
+            const float xa = row.at(a), d = (xa - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
+            to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, -1e30f), c0), gl * sc.inv_t));
         }
     }
 }
@@ -358,13 +387,14 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const float m = group_max<G>(lane_max(x));
         const bool some = m > NEG_INF;
         const double ref = some ? m : 0.0;
+        const Exp64 exp64(sc.inv_t2_64);
         double p[E], s = 0, t = 0;
         bool nan = false;
 #pragma unroll
         for (int e = 0; e < E; e++) {
             nan |= x[e] != x[e];
-            const double d = below(x[e], ref, sc.inv_t2_64);
-            p[e] = exp2_64(d);
+            const double d = exp64.below(x[e], ref);
+            p[e] = exp64(d);
             s += p[e];
             t = fma(p[e], d, t);
         }
@@ -375,7 +405,7 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const bool undefined = (__ballot(nan) & in_group) || m == -NEG_INF, none = undefined || !some;
         const double target = u * total;
         // the first lane that passes the target, or else (rounding; a number of 1) the last one with anything in it
-        const uint64_t past = __ballot(s > 0.0 && upto > target) & in_group, any = __ballot(s > 0.0) & in_group;
+        const uint64_t past = __ballot(s > NOTHING && upto > target) & in_group, any = __ballot(s > NOTHING) & in_group;
         const int owner = none ? group : past ? first_lane(past) : last_lane(any);
         if ((threadIdx.x & 63) == owner) {
             double c = g == 0 ? 0.0 : upto - s;
@@ -385,12 +415,12 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 c += p[e];
-                if (p[e] > 0.0 && !found) { a = g * E + e; xa = x[e]; found = c > target; }
+                if (p[e] > NOTHING && !found) { a = g * E + e; xa = x[e]; found = c > target; }
             }
             const double log_s = log(total);
             const float nil = undefined ? __builtin_nanf("") : NEG_INF;
             out.put(r, none ? -1 : a, none ? nil : (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s),
-                    undefined ? nil : some ? (float)(log_s - t / total * LN_2) : 0.0f);
+                    undefined ? nil : some ? (float)(log_s - t / total * sc.inv_t2_64 * LN_2) : 0.0f);
         }
     }
 }
@@ -522,7 +552,7 @@ template <typename T> __device__ __forceinline__ void finish_row(const Scores<T>
         else if (a >= 0) lp = some ? (row.at(a) - ref) * sc.inv_t - log_s : NEG_INF;
         out.log_prob[r] = lp;
         out.entropy[r] = undefined ? nan : some ? log_s - all.t / all.s * (float)LN_2 : 0.0f;
-        if (out.stats) { out.stats[2 * r] = ref; out.stats[2 * r + 1] = log2f(all.s); }
+        if (out.stats) { out.stats[2 * r] = ref; out.stats[2 * r + 1] = all.s == 0 ? 0.0f : log2f(all.s); }
     }
     if (lane < out.top) {
         const bool there = lane < best.count && !undefined;
@@ -649,35 +679,40 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
         const int64_t a = actions.at(r);
         const float ref = stats[2 * r], log2_s = stats[2 * r + 1], h = entropy[r];
         const float gl = up.lp && a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
-        // dx = p (c0 + c1 log2 p) + 1[j = a] g_lp / T
-        const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t, at_a = gl * sc.inv_t;
+        // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a
+        const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t;
         float x[L::U * L::V];
         tile.p.scores(row, x);
         T *to = grad + r * sc.n;
 #pragma unroll
         for (int u = 0; u < L::U; u++) {
             const int64_t j = L::place(blockIdx.x, u);
-            const int given = a >= j && a < j + L::V ? (int)(a - j) : -1;
             T v[L::V];
 #pragma unroll
             for (int k = 0; k < L::V; k++) {
-                const float xk = x[u * L::V + k], l2 = (xk - ref) * sc.inv_t2 - log2_s, p = __builtin_amdgcn_exp2f(l2);
-                float g = p * fmaf(c1, fmaxf(l2, -1e30f), c0);
-                if (k == given) g += at_a;
-                v[k] = from_f32<T>(xk == NEG_INF ? 0.0f : g);
+                const float l2 = fmaf(x[u * L::V + k] - ref, sc.inv_t2, -log2_s);
+                v[k] = from_f32<T>(__builtin_amdgcn_exp2f(l2) * fmaf(c1, fmaxf(l2, -1e30f), c0));
             }
             if (j + L::V <= n) __builtin_memcpy(to + j, v, sizeof v);
             else
 #pragma unroll
                 for (int k = 0; k < L::V; k++)
                     if (j + k < n) to[j + k] = v[k];
+            if (!finite(c0, c1))          // NaN, but for the places that are not open
+#pragma unroll
+                for (int k = 0; k < L::V; k++)
+                    if (j + k < n && x[u * L::V + k] == NEG_INF) to[j + k] = from_f32<T>(0.0f);
+            if (a >= j && a < j + L::V && a < n) {          // (the lane that has just written this place)
+                const float xa = row.at(a), l2 = fmaf(xa - ref, sc.inv_t2, -log2_s);
+                to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(__builtin_amdgcn_exp2f(l2), fmaf(c1, fmaxf(l2, -1e30f), c0), gl * sc.inv_t));
+            }
         }
     }
 }
 
 // ---- drawing: the row's segments of 64 vectors (one a lane), each with its own maximum and 64-bit sums, then the one segment the target lies in
 struct Segment {
-    double s, t;        // sum 2^d, sum d 2^d
+    double s, t;        // sums of the exponentials, and of these times their differences to the maximum
     float m;            // its maximum (-inf: nothing open)
     int nan;
 };
@@ -696,6 +731,7 @@ template <typename T> __device__ __forceinline__ void sum_segments(const Scores<
     for (int k = 0; k < L::U * L::V; k++) nan |= x[k] != x[k];
     const float m = group_max<64>(lane_max(x));
     const double ref = m > NEG_INF ? m : 0.0;
+    const Exp64 exp64(sc.inv_t2_64);
     double t = 0;
     const int any_nan = __ballot(nan) != 0;
     int64_t last = -1;
@@ -706,7 +742,7 @@ template <typename T> __device__ __forceinline__ void sum_segments(const Scores<
         double s = 0;
 #pragma unroll
         for (int k = 0; k < L::V; k++) {
-            const double d = below(x[u * L::V + k], ref, sc.inv_t2_64), p = exp2_64(d);
+            const double d = exp64.below(x[u * L::V + k], ref), p = exp64(d);
             s += p;
             t = fma(p, d, t);
         }
@@ -729,7 +765,7 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     const int64_t each = (segments + 63) / 64, lo = lane * each < segments ? lane * each : segments, hi = lo + each < segments ? lo + each : segments;
     float m = NEG_INF;
     int nan = 0;
-    for (int64_t g = lo; g < hi; g++) { m = fmaxf(m, seg[g].m); nan |= seg[g].nan; }
+    for (int64_t g = lo; g < hi; g++) { m = max_of(m, seg[g].m); nan |= seg[g].nan; }
     m = group_max<64>(m);
     const bool some = m > NEG_INF, undefined = __ballot(nan) || m == -NEG_INF;
     if (undefined || !some) {
@@ -737,9 +773,10 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
         return;
     }
     const double ref = m;
+    const Exp64 exp64(sc.inv_t2_64);
     const auto weight = [&](const Segment &g, double &d) {
-        d = below(g.m, ref, sc.inv_t2_64);
-        return exp2_64(d);
+        d = exp64.below(g.m, ref);
+        return exp64(d);
     };
     double s = 0, t = 0;
     for (int64_t g = lo; g < hi; g++) {
@@ -753,16 +790,16 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     t = group_sum<64>(t);
     const double target = u * total;
     // the first run that passes the target, or else (rounding; a number of 1) the last one with anything in it; then the segment in it
-    uint64_t past = __ballot(s > 0.0 && upto > target), any = __ballot(s > 0.0);
+    uint64_t past = __ballot(s > NOTHING && upto > target), any = __ballot(s > NOTHING);
     const int run = past ? first_lane(past) : last_lane(any);
     double before = lane_of(lane == 0 ? 0.0 : upto - s, run), found_before = 0;
     int64_t found = run * each;
     for (int64_t g = found; g < (run + 1) * each && g < segments; g++) {
         double d;
         const double w = weight(seg[g], d) * seg[g].s;
-        if (w > 0.0) { found = g; found_before = before; }
+        if (w > NOTHING) { found = g; found_before = before; }
         before += w;
-        if (w > 0.0 && before > target) break;
+        if (w > NOTHING && before > target) break;
     }
     // ... and the action in the segment
     const int64_t j = (found * 64 + lane) * V;
@@ -774,13 +811,13 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     s = 0;
 #pragma unroll
     for (int k = 0; k < V; k++) {
-        p[k] = exp2_64(below(x[k], ref, sc.inv_t2_64));
+        p[k] = exp64(exp64.below(x[k], ref));
         s += p[k];
     }
     upto = group_scan<64>(s, lane);
-    past = __ballot(s > 0.0 && found_before + upto > target);
-    any = __ballot(s > 0.0);
-    const bool tiny = !any;          // (the segment's sum is above 0 and all its terms round to it: the first one that is open)
+    past = __ballot(s > NOTHING && found_before + upto > target);
+    any = __ballot(s > NOTHING);
+    const bool tiny = !any;          // (the segment's sum is above NOTHING and none of its terms: the first one that is open)
     if (tiny) {
         bool open = false;
 #pragma unroll
@@ -796,10 +833,10 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
 #pragma unroll
         for (int k = 0; k < V; k++) {
             c += p[k];
-            if ((tiny ? x[k] > NEG_INF : p[k] > 0.0) && !done) { a = (int)j + k; xa = x[k]; done = tiny || c > target; }
+            if ((tiny ? x[k] > NEG_INF : p[k] > NOTHING) && !done) { a = (int)j + k; xa = x[k]; done = tiny || c > target; }
         }
         const double log_s = log(total);
-        out.put(r, a, (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s), (float)(log_s - t / total * LN_2));
+        out.put(r, a, (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s), (float)(log_s - t / total * sc.inv_t2_64 * LN_2));
     }
 }
 
