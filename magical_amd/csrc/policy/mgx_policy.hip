@@ -52,49 +52,107 @@ constexpr int BLOCK = 256, WAVES = BLOCK / 64;
 template <typename T> constexpr uint32_t neg_inf_bits = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, half> ? 0xfc00u : 0xff80u;
 
 // N pieces of W neighbouring scores of a row, as they lie in memory (16-bit scores two a word), with their mask bytes.  One load a piece and
-// one for its mask where all W are there (gfx950 loads any alignment), else one a score; what is behind the row's end is -inf.
-template <typename T, int W, int N> struct Pieces {
-    static constexpr int WORDS = W * sizeof(T) < 4 ? 1 : W * sizeof(T) / 4, MASK_WORDS = (W + 3) / 4;
+// one for its mask (gfx950 loads any alignment); what is behind the row's end is -inf.  SMALL: n may be less than W.
+template <typename T, int W, int N, bool SMALL = false> struct Pieces {
+    static constexpr int BITS = 8 * sizeof(T), WORDS = W * BITS < 32 ? 1 : W * BITS / 32, MASK_WORDS = (W + 3) / 4;
     uint32_t w[N][WORDS], open[N][MASK_WORDS];
+    static_assert(W == 1 || W >= 4);
     using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
-    __device__ __forceinline__ void fetch(const Row<T> &row, int p, int j) { __builtin_memcpy(w[p], row.x + j, W * sizeof(T)); }
-    __device__ __forceinline__ void fetch_mask(const Row<T> &row, int p, int j) { __builtin_memcpy(open[p], row.mask + j, W); }
-    __device__ __forceinline__ void fetch_ragged(const Row<T> &row, int p, int j, int n) {
-        if (j + W <= n) return fetch(row, p, j);
-        Bits bits[W];
-#pragma unroll
-        for (int k = 0; k < W; k++) bits[k] = (Bits)neg_inf_bits<T>;
-        if (j < n)
-#pragma unroll
-            for (int k = 0; k < W; k++) {
-                Bits b;
-                __builtin_memcpy(&b, row.x + (j + k < n ? j + k : n - 1), sizeof b);          // (in bounds without a branch)
-                if (j + k < n) bits[k] = b;
-            }
-#pragma unroll
-        for (int k = 0; k < WORDS; k++) w[p][k] = 0;
-#pragma unroll
-        for (int k = 0; k < W; k++) w[p][k * sizeof(T) / 4] |= (uint32_t)bits[k] << (k * sizeof(T) % 4 * 8);
+    static constexpr uint32_t CLOSED = sizeof(T) == 4 ? neg_inf_bits<T> : neg_inf_bits<T> << 16 | neg_inf_bits<T>;
+    // v shifted down by `bits` (0 ... 64 * words), zeros from above
+    static __device__ __forceinline__ uint64_t down(uint64_t v, int bits) { return bits < 64 ? v >> bits : 0; }
+    template <int M> static __device__ __forceinline__ void shift_down(uint32_t (&v)[M], int bits) {
+        if constexpr (M == 1) v[0] = bits < 32 ? v[0] >> bits : 0;
+        else if constexpr (M == 2) {
+            const uint64_t r = down((uint64_t)v[1] << 32 | v[0], bits);
+            v[0] = (uint32_t)r;
+            v[1] = (uint32_t)(r >> 32);
+        } else {
+            static_assert(M == 4);
+            const uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+            const uint64_t low = bits < 64 ? lo >> bits | hi << 1 << (63 - bits) : down(hi, bits - 64), high = down(hi, bits);
+            v[0] = (uint32_t)low;
+            v[1] = (uint32_t)(low >> 32);
+            v[2] = (uint32_t)high;
+            v[3] = (uint32_t)(high >> 32);
+        }
     }
-    __device__ __forceinline__ void fetch_mask_ragged(const Row<T> &row, int p, int j, int n) {
-        if (j + W <= n) return fetch_mask(row, p, j);
+    // Piece p from place j on.  Where the row ends inside it (or before it), the row's last W scores are loaded instead and shifted down.
+    __device__ __forceinline__ void fetch(const Row<T> &row, int p, int j, int n, bool whole) {
+        if (W == 1) {
+            Bits b;
+            __builtin_memcpy(&b, row.x + (j < n ? j : n - 1), sizeof b);
+            w[p][0] = j < n ? b : neg_inf_bits<T>;
+        } else if (whole) __builtin_memcpy(w[p], row.x + j, W * sizeof(T));
+        else if (!SMALL || n >= W) {
+            const int from = j < n - W ? j : n - W, bits = (j - from < W ? j - from : W) * BITS;
+            __builtin_memcpy(w[p], row.x + from, W * sizeof(T));
 #pragma unroll
-        for (int k = 0; k < MASK_WORDS; k++) open[p][k] = 0;
-        if (j < n)
+            for (int k = 0; k < WORDS; k++) w[p][k] ^= CLOSED;
+            shift_down(w[p], bits);
 #pragma unroll
-            for (int k = 0; k < W; k++) open[p][k / 4] |= (uint32_t)row.mask[j + k < n ? j + k : n - 1] << (k % 4 * 8);
+            for (int k = 0; k < WORDS; k++) w[p][k] ^= CLOSED;
+        } else {
+#pragma unroll
+            for (int k = 0; k < WORDS; k++) w[p][k] = CLOSED;
+#pragma unroll
+            for (int k = 0; k < W; k++)
+                if (j + k < n) {
+                    Bits b;
+                    __builtin_memcpy(&b, row.x + j + k, sizeof b);
+                    w[p][k * BITS / 32] = BITS == 32 ? b : (k % 2 ? (w[p][k / 2] & 0xffff) | (uint32_t)b << 16 : (w[p][k / 2] & 0xffff0000u) | b);
+                }
+        }
     }
-    // piece p from place(p) on; every lane's piece below `whole` is known to be all there
-    template <typename F> __device__ __forceinline__ void load(const Row<T> &row, int n, int whole, F place) {
+    __device__ __forceinline__ void fetch_mask(const Row<T> &row, int p, int j, int n, bool whole) {
+        if (W == 1) open[p][0] = row.mask[j < n ? j : n - 1];
+        else if (whole) __builtin_memcpy(open[p], row.mask + j, W);
+        else if (!SMALL || n >= W) {
+            const int from = j < n - W ? j : n - W;
+            __builtin_memcpy(open[p], row.mask + from, W);
+            shift_down(open[p], (j - from < W ? j - from : W) * 8);
+        } else {
+#pragma unroll
+            for (int k = 0; k < MASK_WORDS; k++) open[p][k] = 0;
+#pragma unroll
+            for (int k = 0; k < W; k++)
+                if (j + k < n) open[p][k / 4] |= (uint32_t)row.mask[j + k] << (k % 4 * 8);
+        }
+    }
+    // piece p from place(p) on.  The wavefront's pieces below `whole` are all there in every lane, those from `live` on in none.
+    template <typename F> __device__ __forceinline__ void load(const Row<T> &row, int n, int whole, int live, F place) {
 #pragma unroll
         for (int p = 0; p < N; p++)
-            if (p < whole) fetch(row, p, place(p));
-            else fetch_ragged(row, p, place(p), n);
+            if (p < live) fetch(row, p, place(p), n, p < whole);
+            else
+#pragma unroll
+                for (int k = 0; k < WORDS; k++) w[p][k] = CLOSED;
         if (row.mask) {
 #pragma unroll
             for (int p = 0; p < N; p++)
-                if (p < whole) fetch_mask(row, p, place(p));
-                else fetch_mask_ragged(row, p, place(p), n);
+                if (p < live) fetch_mask(row, p, place(p), n, p < whole);
+                else
+#pragma unroll
+                    for (int k = 0; k < MASK_WORDS; k++) open[p][k] = 0;
+        }
+    }
+    // W values of type T to `to` from place j on, as far as the row goes
+    static __device__ __forceinline__ void store(T *to, int j, int n, bool whole, const T (&v)[W]) {
+        if (whole || j + W <= n) { __builtin_memcpy(to + j, v, sizeof v); return; }
+        if constexpr (W == 1) return;
+        uint32_t q[WORDS];
+        __builtin_memcpy(q, v, sizeof v);
+        int left = n - j;
+        if (left <= 0) return;
+#pragma unroll
+        for (int half = W / 2; half >= 1; half /= 2) {          // 4, 2 and 1 of them, as many as are left
+            const int words = half * BITS / 32;
+            if (left & half) {
+                __builtin_memcpy(to + j, q, half * sizeof(T));
+                j += half;
+#pragma unroll
+                for (int k = 0; k < words; k++) q[k] = q[words + k];
+            }
         }
     }
     __device__ __forceinline__ float score(int p, int k) const {
@@ -116,8 +174,7 @@ template <typename T, int W, int N> struct Pieces {
                         const Two16 ones = __builtin_bit_cast(Two16, __builtin_amdgcn_perm(0, open[p][k / 2], k % 2 ? 0x0c030c02 : 0x0c010c00));
                         all = __builtin_bit_cast(uint32_t, -ones);
                     }
-                    constexpr uint32_t closed = sizeof(T) == 4 ? neg_inf_bits<T> : neg_inf_bits<T> << 16 | neg_inf_bits<T>;
-                    w[p][k] = (all & w[p][k]) | (~all & closed);
+                    w[p][k] = (all & w[p][k]) | (~all & CLOSED);
                 }
 #pragma unroll
         for (int p = 0; p < N; p++)
@@ -128,7 +185,11 @@ template <typename T, int W, int N> struct Pieces {
 
 // ---- lane exchanges in the vector unit.  Partner values of a butterfly over G lanes: quads, then half rows, rows of 16, and the two swaps of
 // gfx950 (the mirrors reach the other half, whose lanes all hold the same by then).
-template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+// (lanes without a source get 0; where only some rows take part, so do the others)
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ int dpp(int v) {
+    if constexpr (ROWS == 0xf) return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+    else return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
 template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ float dpp(float v) { return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(int, v))); }
 template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -228,8 +289,8 @@ constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 template <int G, int E, int W> struct Spread {
     static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
     template <typename T> static __device__ __forceinline__ void load_row(const Row<T> &row, int g, int n, float (&x)[E]) {
-        Pieces<T, W, E / W> p;
-        p.load(row, n, n / (G * W), [&](int k) { return place(g, k * W); });
+        Pieces<T, W, E / W, G == 1> p;
+        p.load(row, n, n / (G * W), E / W, [&](int k) { return place(g, k * W); });
         p.scores(row, x);
     }
 };
@@ -240,6 +301,13 @@ template <int E> __device__ __forceinline__ float lane_max(const float (&x)[E]) 
     return m;
 }
 
+struct Given {          // a row's action and its score
+    int64_t a;
+    float x;
+    template <typename T> __device__ __forceinline__ Given(const Actions &actions, const Row<T> &row, int64_t r, int n)
+        : a(actions.at(r)), x(a >= 0 && a < n ? row.at(a) : NEG_INF) {}
+};
+
 template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy,
                                                            float *top_log_probs, int32_t *top_actions) {
@@ -247,8 +315,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
     const int g = threadIdx.x % G, n = (int)sc.n;
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
-        const int64_t a = actions.at(r);
-        float xa = a >= 0 && a < n ? row.at(a) : NEG_INF;
+        const Given given(actions, row, r, n);
         float x[E];
         S::load_row(row, g, n, x);
         const float m = group_max<G>(lane_max(x));
@@ -267,8 +334,8 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
         const float log_s = logf(s), nan = __builtin_nanf("");
         if (g == 0) {
             float lp = 0.0f;
-            if (a >= n || (a >= 0 && undefined)) lp = nan;
-            else if (a >= 0) lp = some ? (xa - ref) * sc.inv_t - log_s : NEG_INF;
+            if (given.a >= n || (given.a >= 0 && undefined)) lp = nan;
+            else if (given.a >= 0) lp = some ? (given.x - ref) * sc.inv_t - log_s : NEG_INF;
             log_prob[r] = lp;
             entropy[r] = undefined ? nan : some ? log_s - t / s * (float)LN_2 : 0.0f;
         }
@@ -293,8 +360,9 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
             if constexpr (G > 8) take(dpp<DPP_MIRROR>(v), dpp<DPP_MIRROR>(i));
             if constexpr (G > 16) { const auto ov = swap<16>(v); const auto oi = swap<16>(i); take(ov.a, oi.a); take(ov.b, oi.b); }
             if constexpr (G > 32) { const auto ov = swap<32>(v); const auto oi = swap<32>(i); take(ov.a, oi.a); take(ov.b, oi.b); }
+            if (k + 1 < top)
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = S::place(g, e) == i ? NEG_INF : x[e];
+                for (int e = 0; e < E; e++) x[e] = S::place(g, e) == i ? NEG_INF : x[e];
             if (g == 0) {
                 const bool there = v > NEG_INF && !undefined;
                 top_actions[r * top + k] = there ? i : -1;
@@ -338,12 +406,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
             T out[W];
 #pragma unroll
             for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf((x[e + k] - ref) * sc.inv_t2 - log2_s, -1e30f), c0));
-            const int j = S::place(g, e);
-            if (e / W < n / (G * W) || j + W <= n) __builtin_memcpy(to + j, out, sizeof out);
-            else
-#pragma unroll
-                for (int k = 0; k < W; k++)
-                    if (j + k < n) to[j + k] = out[k];
+            Pieces<T, W, 1>::store(to, S::place(g, e), n, e / W < n / (G * W), out);
         }
         if (!finite(c0, c1))          // NaN, but for the places that are not open
 #pragma unroll
@@ -381,7 +444,7 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         float x[E];
         {
             Pieces<T, W, E / W> p;
-            p.load(row, n, n / (G * E) * (E / W), [&](int k) { return g * E + k * W; });
+            p.load(row, n, n / (G * E) * (E / W), E / W, [&](int k) { return g * E + k * W; });
             p.scores(row, x);
         }
         const float m = group_max<G>(lane_max(x));
@@ -389,10 +452,8 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const double ref = some ? m : 0.0;
         const Exp64 exp64(sc.inv_t2_64);
         double p[E], s = 0, t = 0;
-        bool nan = false;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            nan |= x[e] != x[e];
             const double d = exp64.below(x[e], ref);
             p[e] = exp64(d);
             s += p[e];
@@ -402,7 +463,7 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         t = group_sum<G>(t);
         const int group = (threadIdx.x & 63) - g;
         const uint64_t in_group = G == 64 ? ~0ull : ((1ull << (G & 63)) - 1) << group;
-        const bool undefined = (__ballot(nan) & in_group) || m == -NEG_INF, none = undefined || !some;
+        const bool undefined = m != m || m == -NEG_INF, none = undefined || !some;
         const double target = u * total;
         // the first lane that passes the target, or else (rounding; a number of 1) the last one with anything in it
         const uint64_t past = __ballot(s > NOTHING && upto > target) & in_group, any = __ballot(s > NOTHING) & in_group;
@@ -435,7 +496,12 @@ template <typename T> struct Tile {
     static __device__ __forceinline__ int64_t place(int64_t tile, int u) { return tile * SIZE + (u * BLOCK + (int)threadIdx.x) * V; }
     Pieces<T, V, U> p;
     __device__ __forceinline__ void load(const Row<T> &row, int64_t tile, int n) {
-        p.load(row, n, (tile + 1) * SIZE <= n ? U : 0, [&](int u) { return (int)place(tile, u); });
+        p.load(row, n, (int)((n - tile * SIZE) / (BLOCK * V)), live(tile, n), [&](int u) { return (int)place(tile, u); });
+    }
+    // how many of its U vectors begin inside the row in some lane of this wavefront
+    static __device__ __forceinline__ int live(int64_t tile, int n) {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        return (int)((n - tile * SIZE - wave * 64 * V + BLOCK * V - 1) / (BLOCK * V));
     }
 };
 
@@ -539,17 +605,15 @@ struct LogProbOut {
 };
 
 // a row's results from its sums (one lane) and its best (one wavefront; sorted)
-template <typename T> __device__ __forceinline__ void finish_row(const Scores<T> &sc, int64_t r, const Actions &actions, const Softmax &all,
+template <typename T> __device__ __forceinline__ void finish_row(const Scores<T> &sc, int64_t r, const Given &given, const Softmax &all,
                                                                  const Top &best, const LogProbOut &out) {
     const int lane = threadIdx.x & 63, n = (int)sc.n;
     const bool some = all.m > NEG_INF, undefined = !(all.s == all.s);
     const float ref = some ? all.m : 0.0f, log_s = logf(all.s), nan = __builtin_nanf("");
     if (lane == 0) {
-        const int64_t a = actions.at(r);
-        const Row<T> row(sc, r);
         float lp = 0.0f;
-        if (a >= n || (a >= 0 && undefined)) lp = nan;
-        else if (a >= 0) lp = some ? (row.at(a) - ref) * sc.inv_t - log_s : NEG_INF;
+        if (given.a >= n || (given.a >= 0 && undefined)) lp = nan;
+        else if (given.a >= 0) lp = some ? (given.x - ref) * sc.inv_t - log_s : NEG_INF;
         out.log_prob[r] = lp;
         out.entropy[r] = undefined ? nan : some ? log_s - all.t / all.s * (float)LN_2 : 0.0f;
         if (out.stats) { out.stats[2 * r] = ref; out.stats[2 * r + 1] = all.s == 0 ? 0.0f : log2f(all.s); }
@@ -581,6 +645,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
         const int64_t r = SPLIT ? b / parts : b;
         const int first = SPLIT ? (int)(b % parts) * part_tiles : 0, behind = SPLIT ? min(first + part_tiles, tiles) : tiles;
         const Row<T> row(sc, r);
+        const Given given(actions, row, r, n);
         Softmax a;
         Top best(lds_keys[TOP ? wave : 0], TOP ? top : 1);
         for (int tile = first; tile < behind; tile++) {
@@ -591,12 +656,16 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
             m = lane_max(x);
             if (m > a.m) a.to(m, sc.inv_t2);
             const float ref = a.m > NEG_INF ? a.m : 0.0f;
+            const int live = L::live(tile, n);
 #pragma unroll
-            for (int k = 0; k < L::U * L::V; k++) {
-                const float d = (x[k] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
-                a.s += p;
-                a.t = fmaf(p, fmaxf(d, -1e30f), a.t);
-            }
+            for (int u = 0; u < L::U; u++)
+                if (u < live)
+#pragma unroll
+                    for (int k = u * L::V; k < (u + 1) * L::V; k++) {
+                        const float d = (x[k] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
+                        a.s += p;
+                        a.t = fmaf(p, fmaxf(d, -1e30f), a.t);
+                    }
             if constexpr (TOP) {
                 if (tile == first) best.expect(m);
                 // (the wavefront's places ascend: a later tile's score that only equals the k-th best is behind it)
@@ -631,7 +700,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
             if constexpr (SPLIT) {
                 if (lane == 0) { to.sums[b * 4] = a.m; to.sums[b * 4 + 1] = a.s; to.sums[b * 4 + 2] = a.t; }
                 if (lane < top) to.keys[b * top + lane] = lane < best.count ? best.keys[lane] : 0;
-            } else finish_row(sc, r, actions, a, best, out);
+            } else finish_row(sc, r, given, a, best, out);
         }
         __syncthreads();
     }
@@ -645,6 +714,7 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
     for (int64_t r = blockIdx.x; r < sc.rows; r += gridDim.x) {
         const uint64_t *keys = from.keys + r * parts * top;
         const float *sums = from.sums + r * parts * 4;
+        const Given given(actions, Row<T>(sc, r), r, (int)sc.n);
         Softmax a;
         for (int p = lane; p < parts; p += 64) {
             Softmax o;
@@ -662,7 +732,7 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
             for (int c = 0; c < parts * top; c += 64) best.offer(c + lane < parts * top ? keys[c + lane] : 0);
             best.sort();
         }
-        finish_row(sc, r, actions, a, best, out);
+        finish_row(sc, r, given, a, best, out);
         Top::sync();
     }
 }
@@ -684,8 +754,10 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
         float x[L::U * L::V];
         tile.p.scores(row, x);
         T *to = grad + r * sc.n;
+        const int live = L::live(blockIdx.x, n);
 #pragma unroll
         for (int u = 0; u < L::U; u++) {
+            if (u >= live) break;
             const int64_t j = L::place(blockIdx.x, u);
             T v[L::V];
 #pragma unroll
@@ -693,11 +765,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
                 const float l2 = fmaf(x[u * L::V + k] - ref, sc.inv_t2, -log2_s);
                 v[k] = from_f32<T>(__builtin_amdgcn_exp2f(l2) * fmaf(c1, fmaxf(l2, -1e30f), c0));
             }
-            if (j + L::V <= n) __builtin_memcpy(to + j, v, sizeof v);
-            else
-#pragma unroll
-                for (int k = 0; k < L::V; k++)
-                    if (j + k < n) to[j + k] = v[k];
+            if (j < n) Pieces<T, L::V, 1>::store(to, (int)j, n, false, v);
             if (!finite(c0, c1))          // NaN, but for the places that are not open
 #pragma unroll
                 for (int k = 0; k < L::V; k++)
@@ -713,8 +781,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
 // ---- drawing: the row's segments of 64 vectors (one a lane), each with its own maximum and 64-bit sums, then the one segment the target lies in
 struct Segment {
     double s, t;        // sums of the exponentials, and of these times their differences to the maximum
-    float m;            // its maximum (-inf: nothing open)
-    int nan;
+    float m;            // its maximum (-inf: nothing open; NaN: there is one)
 };
 constexpr int LDS_SEGMENTS = 512;          // as many are looked at in LDS
 
@@ -726,14 +793,10 @@ template <typename T> __device__ __forceinline__ void sum_segments(const Scores<
     now.load(row, tile, n);
     float x[L::U * L::V];
     now.p.scores(row, x);
-    bool nan = false;
-#pragma unroll
-    for (int k = 0; k < L::U * L::V; k++) nan |= x[k] != x[k];
     const float m = group_max<64>(lane_max(x));
     const double ref = m > NEG_INF ? m : 0.0;
     const Exp64 exp64(sc.inv_t2_64);
     double t = 0;
-    const int any_nan = __ballot(nan) != 0;
     int64_t last = -1;
 #pragma unroll
     for (int u = 0; u < L::U; u++) {
@@ -747,7 +810,7 @@ template <typename T> __device__ __forceinline__ void sum_segments(const Scores<
             t = fma(p, d, t);
         }
         s = group_sum<64>(s);
-        if (lane == 0) to[seg] = {s, 0.0, m, any_nan};
+        if (lane == 0) to[seg] = {s, 0.0, m};
         last = seg;
     }
     // (t of the four, all against one maximum, goes with the last of them)
@@ -764,10 +827,9 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     // every lane has a run of neighbouring segments
     const int64_t each = (segments + 63) / 64, lo = lane * each < segments ? lane * each : segments, hi = lo + each < segments ? lo + each : segments;
     float m = NEG_INF;
-    int nan = 0;
-    for (int64_t g = lo; g < hi; g++) { m = max_of(m, seg[g].m); nan |= seg[g].nan; }
+    for (int64_t g = lo; g < hi; g++) m = max_of(m, seg[g].m);
     m = group_max<64>(m);
-    const bool some = m > NEG_INF, undefined = __ballot(nan) || m == -NEG_INF;
+    const bool some = m > NEG_INF, undefined = m != m || m == -NEG_INF;
     if (undefined || !some) {
         if (lane == 0) out.put(r, -1, undefined ? __builtin_nanf("") : NEG_INF, undefined ? __builtin_nanf("") : 0.0f);
         return;
@@ -804,7 +866,7 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     // ... and the action in the segment
     const int64_t j = (found * 64 + lane) * V;
     Pieces<T, V, 1> piece;
-    piece.load(row, n, 0, [&](int) { return (int)j; });
+    piece.load(row, n, 0, 1, [&](int) { return (int)j; });
     float x[V];
     piece.scores(row, x);
     double p[V];
@@ -944,15 +1006,17 @@ template <typename T, typename F> int by_lanes(int64_t n, F f) {
     return by_pieces<T, 64>(n, f);
 }
 template <typename T, typename F> int by_length(int64_t n, F f) {
-    constexpr int W = 16 / sizeof(T);
     if (n > 32) return by_lanes<T>(n, f);
-    if (n <= 8) return f(Shape<1, 8, W>());
-    if constexpr (W == 4) if (n <= 12) return f(Shape<1, 12, W>());
-    if (n <= 16) return f(Shape<1, 16, W>());
-    if constexpr (W == 4) if (n <= 20) return f(Shape<1, 20, W>());
-    if (n <= 24) return f(Shape<1, 24, W>());
-    if constexpr (W == 4) if (n <= 28) return f(Shape<1, 28, W>());
-    return f(Shape<1, 32, W>());
+    switch ((n + 3) / 4) {
+        case 1: return f(Shape<1, 4, 4>());
+        case 2: return f(Shape<1, 8, 4>());
+        case 3: return f(Shape<1, 12, 4>());
+        case 4: return f(Shape<1, 16, 4>());
+        case 5: return f(Shape<1, 20, 4>());
+        case 6: return f(Shape<1, 24, 4>());
+        case 7: return f(Shape<1, 28, 4>());
+        default: return f(Shape<1, 32, 4>());
+    }
 }
 // Drawing: up to 32 scores over four lanes (64-bit exponentials take twenty times what an exchange takes)
 template <typename T, typename F> int by_length_64(int64_t n, F f) {
