@@ -490,19 +490,20 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 // A workgroup goes over a row, or over one part of it where there are few rows, in tiles of U 16-byte vectors a lane: running maximum, sum and
 // weighted sum per lane, joined at the end.
 
-template <typename T> struct Tile {
-    static constexpr int V = 16 / sizeof(T), U = 4, SIZE = BLOCK * U * V;
-    // vector u of a tile in this thread: a wavefront's 64 vectors are neighbours, and its places ascend with the tile and u
-    static __device__ __forceinline__ int64_t place(int64_t tile, int u) { return tile * SIZE + (u * BLOCK + (int)threadIdx.x) * V; }
+// ROW_WAVES: wavefronts that go over the tile together (1, or the workgroup's 4)
+template <typename T, int ROW_WAVES> struct Tile {
+    static constexpr int V = 16 / sizeof(T), U = 4, LANES = 64 * ROW_WAVES, SIZE = LANES * U * V;
+    static __device__ __forceinline__ int lane() { return (int)threadIdx.x % LANES; }
+    static __device__ __forceinline__ int wave() { return ROW_WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+    // vector u of a tile in this lane: a wavefront's 64 vectors are neighbours, and its places ascend with the tile and u
+    static __device__ __forceinline__ int64_t place(int64_t tile, int u) { return tile * SIZE + (u * LANES + lane()) * V; }
     Pieces<T, V, U> p;
     __device__ __forceinline__ void load(const Row<T> &row, int64_t tile, int n) {
-        p.load(row, n, (int)((n - tile * SIZE) / (BLOCK * V)), live(tile, n), [&](int u) { return (int)place(tile, u); });
+        p.load(row, n, (int)((n - tile * SIZE) / (LANES * V)), live(tile, n), [&](int u) { return (int)place(tile, u); });
     }
     // how many of its U vectors begin inside the row in some lane of this wavefront
-    static __device__ __forceinline__ int live(int64_t tile, int n) {
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        return (int)((n - tile * SIZE - wave * 64 * V + BLOCK * V - 1) / (BLOCK * V));
-    }
+    static __device__ __forceinline__ int live(int64_t tile, int n) { return (int)((n - tile * SIZE - wave() * 64 * V + LANES * V - 1) / (LANES * V)); }
+    static __host__ __device__ __forceinline__ int count(int64_t n) { return (int)((n + SIZE - 1) / SIZE); }
 };
 
 // Maximum m, s = sum 2^d, t = sum d 2^d with d = (x - m) inv_t2, of scores seen so far (none: m = -inf, s = t = 0).  A NaN or +inf among
@@ -632,18 +633,18 @@ struct Partials {
     float *sums;
 };
 
-// SPLIT: b-th part of part_tiles tiles of a row each, else whole rows
-template <typename T, bool TOP, bool SPLIT>
-__global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions actions, LogProbOut out, int parts, int part_tiles, Partials to) {
-    using L = Tile<T>;
+// One wavefront (ROW_WAVES 1) or workgroup (4) goes over a row; SPLIT: a workgroup over blockIdx.x-th part of part_tiles tiles of it.
+template <typename T, bool TOP, int ROW_WAVES, bool SPLIT>
+__global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions actions, LogProbOut out, int part_tiles, Partials to) {
+    using L = Tile<T, ROW_WAVES>;
     __shared__ float lds[WAVES][3];
     __shared__ uint64_t lds_keys[TOP ? WAVES : 1][TOP ? Top::CAPACITY : 1];
     __shared__ int lds_count[WAVES];
-    const int n = (int)sc.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, top = TOP ? out.top : 0;
-    const int tiles = (int)(((int64_t)n + L::SIZE - 1) / L::SIZE);
-    for (int64_t b = blockIdx.x; b < (SPLIT ? sc.rows * parts : sc.rows); b += gridDim.x) {
-        const int64_t r = SPLIT ? b / parts : b;
-        const int first = SPLIT ? (int)(b % parts) * part_tiles : 0, behind = SPLIT ? min(first + part_tiles, tiles) : tiles;
+    const int n = (int)sc.n, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), top = TOP ? out.top : 0;
+    const int first = SPLIT ? (int)blockIdx.x * part_tiles : 0, behind = SPLIT ? min(first + part_tiles, L::count(n)) : L::count(n);
+    constexpr int ROWS = WAVES / ROW_WAVES;          // of a workgroup
+    const int64_t r0 = (SPLIT ? blockIdx.y : (int64_t)blockIdx.x * ROWS) + (ROW_WAVES == 1 ? wave : 0);
+    for (int64_t r = r0; r < sc.rows; r += SPLIT ? gridDim.y : (int64_t)gridDim.x * ROWS) {
         const Row<T> row(sc, r);
         const Given given(actions, row, r, n);
         Softmax a;
@@ -683,26 +684,33 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
             }
         }
         a.join_wave(sc.inv_t2);
-        __syncthreads();
-        if (lane == 0) { lds[wave][0] = a.m; lds[wave][1] = a.s; lds[wave][2] = a.t; lds_count[wave] = best.count; }
-        __syncthreads();
-        if (wave == 0) {
-            for (int w = 1; w < WAVES; w++) {
-                Softmax o;
-                o.m = lds[w][0];
-                o.s = lds[w][1];
-                o.t = lds[w][2];
-                a.join(o, sc.inv_t2);
-                if constexpr (TOP)
-                    for (int c = 0; c < lds_count[w]; c += 64) best.offer(c + lane < lds_count[w] ? lds_keys[w][c + lane] : 0);
-            }
+        if constexpr (ROW_WAVES == 1) {
             if constexpr (TOP) best.sort();
-            if constexpr (SPLIT) {
-                if (lane == 0) { to.sums[b * 4] = a.m; to.sums[b * 4 + 1] = a.s; to.sums[b * 4 + 2] = a.t; }
-                if (lane < top) to.keys[b * top + lane] = lane < best.count ? best.keys[lane] : 0;
-            } else finish_row(sc, r, given, a, best, out);
+            finish_row(sc, r, given, a, best, out);
+            Top::sync();
+        } else {
+            __syncthreads();
+            if (lane == 0) { lds[wave][0] = a.m; lds[wave][1] = a.s; lds[wave][2] = a.t; lds_count[wave] = best.count; }
+            __syncthreads();
+            if (wave == 0) {
+                for (int w = 1; w < WAVES; w++) {
+                    Softmax o;
+                    o.m = lds[w][0];
+                    o.s = lds[w][1];
+                    o.t = lds[w][2];
+                    a.join(o, sc.inv_t2);
+                    if constexpr (TOP)
+                        for (int c = 0; c < lds_count[w]; c += 64) best.offer(c + lane < lds_count[w] ? lds_keys[w][c + lane] : 0);
+                }
+                if constexpr (TOP) best.sort();
+                if constexpr (SPLIT) {
+                    const int64_t b = r * gridDim.x + blockIdx.x;
+                    if (lane == 0) { to.sums[b * 4] = a.m; to.sums[b * 4 + 1] = a.s; to.sums[b * 4 + 2] = a.t; }
+                    if (lane < top) to.keys[b * top + lane] = lane < best.count ? best.keys[lane] : 0;
+                } else finish_row(sc, r, given, a, best, out);
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -740,7 +748,7 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions actions, const float *stats, const float *entropy, Upstream up,
                                                          T *grad) {
-    using L = Tile<T>;
+    using L = Tile<T, WAVES>;
     const int n = (int)sc.n;
     for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
         const Row<T> row(sc, r);
@@ -783,25 +791,23 @@ struct Segment {
     double s, t;        // sums of the exponentials, and of these times their differences to the maximum
     float m;            // its maximum (-inf: nothing open; NaN: there is one)
 };
-constexpr int LDS_SEGMENTS = 512;          // as many are looked at in LDS
 
-// the four segments of a wavefront's part of a tile: (tile, u, wave) is segment (tile * U + u) * WAVES + wave
-template <typename T> __device__ __forceinline__ void sum_segments(const Scores<T> &sc, const Row<T> &row, int64_t tile, int64_t segments, Segment *to) {
-    using L = Tile<T>;
-    const int n = (int)sc.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The segments of a wavefront's vectors of a tile: (tile, u, wave) is segment (tile * U + u) * ROW_WAVES + wave.  put(segment, its sums) for
+// each that there is; t of all of them, against one maximum, comes with the last.
+template <typename T, int ROW_WAVES, typename F>
+__device__ __forceinline__ void sum_segments(const Scores<T> &sc, const Row<T> &row, const Exp64 &exp64, int tile, F put) {
+    using L = Tile<T, ROW_WAVES>;
+    const int n = (int)sc.n, live = min(L::live(tile, n), (int)L::U);
     L now;
     now.load(row, tile, n);
     float x[L::U * L::V];
     now.p.scores(row, x);
     const float m = group_max<64>(lane_max(x));
     const double ref = m > NEG_INF ? m : 0.0;
-    const Exp64 exp64(sc.inv_t2_64);
     double t = 0;
-    int64_t last = -1;
 #pragma unroll
     for (int u = 0; u < L::U; u++) {
-        const int64_t seg = (tile * L::U + u) * WAVES + wave;
-        if (seg >= segments) break;
+        if (u >= live) break;
         double s = 0;
 #pragma unroll
         for (int k = 0; k < L::V; k++) {
@@ -810,24 +816,19 @@ template <typename T> __device__ __forceinline__ void sum_segments(const Scores<
             t = fma(p, d, t);
         }
         s = group_sum<64>(s);
-        if (lane == 0) to[seg] = {s, 0.0, m};
-        last = seg;
+        if (u + 1 == live) t = group_sum<64>(t);
+        put((tile * L::U + u) * ROW_WAVES + L::wave(), Segment{s, u + 1 == live ? t : 0.0, m});
     }
-    // (t of the four, all against one maximum, goes with the last of them)
-    t = group_sum<64>(t);
-    if (lane == 0 && last >= 0) to[last].t = t;
 }
 
-// One wavefront: the row's action from its segments.
-template <typename T>
-__device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segment *seg, int64_t segments, double u, const Drawn &out) {
-    constexpr int V = Tile<T>::V;
+// One wavefront: the row's action.  Every lane has a run of `each` neighbouring segments from lane * each on; of(k) is its k-th, and
+// again(run, k) the k-th of another lane's.
+template <typename T, typename F, typename A>
+__device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, const Exp64 &exp64, int64_t r, int each, F of, A again, double u, const Drawn &out) {
+    constexpr int V = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, n = (int)sc.n;
-    const Row<T> row(sc, r);
-    // every lane has a run of neighbouring segments
-    const int64_t each = (segments + 63) / 64, lo = lane * each < segments ? lane * each : segments, hi = lo + each < segments ? lo + each : segments;
     float m = NEG_INF;
-    for (int64_t g = lo; g < hi; g++) m = max_of(m, seg[g].m);
+    for (int k = 0; k < each; k++) m = max_of(m, of(k).m);
     m = group_max<64>(m);
     const bool some = m > NEG_INF, undefined = m != m || m == -NEG_INF;
     if (undefined || !some) {
@@ -835,17 +836,12 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
         return;
     }
     const double ref = m;
-    const Exp64 exp64(sc.inv_t2_64);
-    const auto weight = [&](const Segment &g, double &d) {
-        d = exp64.below(g.m, ref);
-        return exp64(d);
-    };
     double s = 0, t = 0;
-    for (int64_t g = lo; g < hi; g++) {
-        double d;
-        const double w = weight(seg[g], d);
-        s += w * seg[g].s;
-        t += w * fma(d, seg[g].s, seg[g].t);
+    for (int k = 0; k < each; k++) {
+        const Segment g = of(k);
+        const double d = exp64.below(g.m, ref), w = exp64(d);
+        s = fma(w, g.s, s);
+        t = fma(w, fma(d, g.s, g.t), t);
     }
     double upto = group_scan<64>(s, lane);
     const double total = lane_of(upto, 63);
@@ -854,17 +850,18 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     // the first run that passes the target, or else (rounding; a number of 1) the last one with anything in it; then the segment in it
     uint64_t past = __ballot(s > NOTHING && upto > target), any = __ballot(s > NOTHING);
     const int run = past ? first_lane(past) : last_lane(any);
-    double before = lane_of(lane == 0 ? 0.0 : upto - s, run), found_before = 0;
-    int64_t found = run * each;
-    for (int64_t g = found; g < (run + 1) * each && g < segments; g++) {
-        double d;
-        const double w = weight(seg[g], d) * seg[g].s;
-        if (w > NOTHING) { found = g; found_before = before; }
-        before += w;
-        if (w > NOTHING && before > target) break;
-    }
+    double before = lane_of(lane == 0 ? 0.0 : upto - s, run), found_before = before;
+    int found = run * each;
+    if (each > 1)
+        for (int k = 0; k < each; k++) {
+            const Segment g = again(run, k);
+            const double w = exp64(exp64.below(g.m, ref)) * g.s;
+            if (w > NOTHING) { found = run * each + k; found_before = before; }
+            before += w;
+            if (w > NOTHING && before > target) break;
+        }
     // ... and the action in the segment
-    const int64_t j = (found * 64 + lane) * V;
+    const int64_t j = ((int64_t)found * 64 + lane) * V;
     Pieces<T, V, 1> piece;
     piece.load(row, n, 0, 1, [&](int) { return (int)j; });
     float x[V];
@@ -902,37 +899,57 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, int64_t r, const Segme
     }
 }
 
-// parts == 1: a workgroup sums a row's segments and its first wavefront draws; else only the sums, for k_draw
+// rows of up to 64 segments: one wavefront each, lane i keeps the i-th segment's sums
 template <typename T>
-__global__ __launch_bounds__(BLOCK, 4) void k_sample_long(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out, int parts,
-                                                          int part_tiles, int64_t segments, Segment *workspace) {
-    using L = Tile<T>;
-    __shared__ Segment lds[LDS_SEGMENTS];
-    const int64_t tiles = (sc.n + L::SIZE - 1) / L::SIZE;
-    for (int64_t b = blockIdx.x; b < sc.rows * parts; b += gridDim.x) {
-        const int64_t r = b / parts, first = b % parts * part_tiles, behind = first + part_tiles < tiles ? first + part_tiles : tiles;
+__global__ __launch_bounds__(BLOCK, 4) void k_sample_wave(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const Exp64 exp64(sc.inv_t2_64);
+    for (int64_t r = (int64_t)blockIdx.x * WAVES + wave; r < sc.rows; r += (int64_t)gridDim.x * WAVES) {
         const Row<T> row(sc, r);
-        Segment *seg = workspace ? workspace + r * segments : lds;
-        for (int64_t tile = first; tile < behind; tile++) sum_segments(sc, row, tile, segments, seg);
-        if (parts == 1) {
-            __syncthreads();
-            if (threadIdx.x < 64) draw(sc, r, seg, segments, uniform_at(uniforms, uniform_bytes, r), out);
-            __syncthreads();
-        }
+        const double u = uniform_at(uniforms, uniform_bytes, r);
+        Segment mine{0, 0, NEG_INF};
+        for (int tile = 0; tile < Tile<T, 1>::count(sc.n); tile++)
+            sum_segments<T, 1>(sc, row, exp64, tile, [&](int g, const Segment &v) {
+                mine.s = lane == g ? v.s : mine.s;
+                mine.t = lane == g ? v.t : mine.t;
+                mine.m = lane == g ? v.m : mine.m;
+            });
+        draw(sc, row, exp64, r, 1, [&](int) { return mine; }, [&](int, int) { return mine; }, u, out);
     }
 }
+
+// longer rows: workgroups sum parts of part_tiles tiles each, a wavefront draws
 template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_draw(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out, int64_t segments,
-                                                const Segment *workspace) {
+__global__ __launch_bounds__(BLOCK, 4) void k_sample_parts(Scores<T> sc, int part_tiles, int segments, Segment *workspace) {
+    using L = Tile<T, WAVES>;
+    const Exp64 exp64(sc.inv_t2_64);
+    const int first = (int)blockIdx.x * part_tiles, behind = min(first + part_tiles, L::count(sc.n));
+    for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
+        const Row<T> row(sc, r);
+        Segment *to = workspace + r * segments;
+        for (int tile = first; tile < behind; tile++)
+            sum_segments<T, WAVES>(sc, row, exp64, tile, [&](int g, const Segment &v) { if ((threadIdx.x & 63) == 0) to[g] = v; });
+    }
+}
+constexpr int LDS_SEGMENTS = 512;          // as many are looked at in LDS
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_draw(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out, int segments, const Segment *workspace) {
     __shared__ Segment lds[LDS_SEGMENTS];
+    const Exp64 exp64(sc.inv_t2_64);
     for (int64_t r = blockIdx.x; r < sc.rows; r += gridDim.x) {
+        const double u = uniform_at(uniforms, uniform_bytes, r);
         const Segment *seg = workspace + r * segments;
         if (segments <= LDS_SEGMENTS) {
             for (int g = threadIdx.x; g < segments; g += BLOCK) lds[g] = seg[g];
             seg = lds;
         }
         __syncthreads();
-        if (threadIdx.x < 64) draw(sc, r, seg, segments, uniform_at(uniforms, uniform_bytes, r), out);
+        const int lane = threadIdx.x, each = (segments + 63) / 64;
+        const auto at = [&](int run, int k) {
+            const int g = run * each + k;
+            return g < segments ? seg[g] : Segment{0, 0, NEG_INF};
+        };
+        if (threadIdx.x < 64) draw(sc, Row<T>(sc, r), exp64, r, each, [&](int k) { return at(lane, k); }, at, u, out);
         __syncthreads();
     }
 }
@@ -1032,23 +1049,21 @@ template <typename T, typename F> int by_length_64(int64_t n, F f) {
         default: return f(Shape<4, 8, 1>());
     }
 }
-// How many workgroups share a long row: enough to give every one of the 256 CUs some, no more than the row has tiles.
+// How a long row is shared out.  4096 rows or more: a wavefront each (four for every SIMD; no exchange between wavefronts).  Fewer: a workgroup
+// each, or several where that leaves CUs without one, no more than the row has tiles.
 struct Split {
-    int parts, part_tiles;
+    int row_waves, parts, part_tiles;
 };
-Split split(int dtype, int64_t rows, int64_t n) {
-    const int64_t size = dtype == MGX_REAL_F32 ? Tile<float>::SIZE : Tile<half>::SIZE, tiles = (n + size - 1) / size;
-    const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(tiles, 1024 / std::max<int64_t>(rows, 1))), each = (tiles + wanted - 1) / wanted;
-    return {(int)((tiles + each - 1) / each), (int)each};
+template <typename T> Split split(int64_t rows, int64_t n) {
+    if (rows >= 4096) return {1, 1, 0};
+    const int64_t tiles = Tile<T, WAVES>::count(n), wanted = std::max<int64_t>(1, std::min<int64_t>(tiles, 1024 / std::max<int64_t>(rows, 1)));
+    const int64_t each = (tiles + wanted - 1) / wanted;
+    return {WAVES, (int)((tiles + each - 1) / each), (int)each};
 }
-int64_t n_segments(int dtype, int64_t n) {
-    const int64_t size = 64 * (dtype == MGX_REAL_F32 ? Tile<float>::V : Tile<half>::V);
-    return (n + size - 1) / size;
-}
-
-int64_t sample_workspace(int dtype, int64_t rows, int64_t n) {
-    const int64_t segments = n_segments(dtype, n);
-    return split(dtype, rows, n).parts == 1 && segments <= LDS_SEGMENTS ? 0 : rows * segments * (int64_t)sizeof(Segment);
+template <typename T> int n_segments(int64_t n) { return (int)((n + 64 * (16 / sizeof(T)) - 1) / (64 * (16 / sizeof(T)))); }
+// Drawing: a wavefront a row up to four tiles, or up to 64 segments if there are rows enough
+template <typename T> bool sample_by_waves(int64_t rows, int64_t n) {
+    return Tile<T, 1>::count(n) <= 4 || (rows >= 1024 && n_segments<T>(n) <= 64);
 }
 
 int64_t short_blocks(int64_t rows, int G) { return (rows * G + BLOCK - 1) / BLOCK; }
@@ -1070,9 +1085,13 @@ const char *mgx_policy_last_error(void) { return g_err; }
 
 int64_t mgx_policy_workspace_bytes(int op, int dtype, int64_t rows, int64_t n, int top) {
     if (n <= SHORT_MAX || rows <= 0) return 0;
-    if (op == MGX_POLICY_SAMPLE) return sample_workspace(dtype, rows, n);
-    const Split sp = split(dtype, rows, n);
-    return sp.parts == 1 ? 0 : rows * sp.parts * (16 + 8 * (int64_t)top);
+    const auto bytes = [&](auto v) -> int64_t {
+        using T = decltype(v);
+        if (op == MGX_POLICY_SAMPLE) return sample_by_waves<T>(rows, n) ? 0 : rows * n_segments<T>(n) * (int64_t)sizeof(Segment);
+        const Split sp = split<T>(rows, n);
+        return sp.parts == 1 ? 0 : rows * sp.parts * (16 + 8 * (int64_t)top);
+    };
+    return dtype == MGX_REAL_F32 ? bytes(float()) : bytes(half());
 }
 
 int64_t mgx_policy_stats_bytes(int64_t rows, int64_t n) { return n > SHORT_MAX ? rows * 8 : 0; }
@@ -1100,13 +1119,17 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
                 return launch(k_log_probs_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, top,
                               log_prob, entropy, top_log_probs, top_actions);
             });
-        const Split sp = split(dtype, rows, n);
+        const Split sp = split<T>(rows, n);
         const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_actions, top};
         const Partials partials{(uint64_t *)workspace, workspace ? (float *)((uint64_t *)workspace + rows * sp.parts * top) : nullptr};
+        if (sp.row_waves == 1)
+            return launch(top ? k_log_probs_long<T, true, 1, false> : k_log_probs_long<T, false, 1, false>, (rows + WAVES - 1) / WAVES, BLOCK, stream,
+                          sc, given, out, 0, partials);
         if (sp.parts == 1)
-            return launch(top ? k_log_probs_long<T, true, false> : k_log_probs_long<T, false, false>, rows, BLOCK, stream, sc, given, out, 1, 0, partials);
-        if (const int rc = launch(top ? k_log_probs_long<T, true, true> : k_log_probs_long<T, false, true>, rows * sp.parts, BLOCK, stream, sc, given,
-                                  out, sp.parts, sp.part_tiles, partials))
+            return launch(top ? k_log_probs_long<T, true, WAVES, false> : k_log_probs_long<T, false, WAVES, false>, rows, BLOCK, stream, sc, given,
+                          out, 0, partials);
+        if (const int rc = launch(top ? k_log_probs_long<T, true, WAVES, true> : k_log_probs_long<T, false, WAVES, true>,
+                                  dim3((unsigned)sp.parts, (unsigned)rows), BLOCK, stream, sc, given, out, sp.part_tiles, partials))
             return rc;
         return launch(k_log_probs_join<T>, rows, 64, stream, sc, given, out, sp.parts, partials);
     });
@@ -1134,7 +1157,7 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
                 return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad);
             });
-        return launch(k_backward_long<T>, dim3((unsigned)((n + Tile<T>::SIZE - 1) / Tile<T>::SIZE), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
+        return launch(k_backward_long<T>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
                       stream, sc, given, stats, entropy, up, (T *)grad);
     });
 }
@@ -1159,12 +1182,14 @@ int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, i
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
                 return launch(k_sample_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, uniforms, uniform_bytes, out);
             });
-        const Split sp = split(dtype, rows, n);
-        const int64_t segments = n_segments(dtype, n);
-        Segment *const ws = sample_workspace(dtype, rows, n) ? (Segment *)workspace : nullptr;
-        const int rc = launch(k_sample_long<T>, rows * sp.parts, BLOCK, stream, sc, uniforms, uniform_bytes, out, sp.parts, sp.part_tiles, segments, ws);
-        if (rc || sp.parts == 1) return rc;
-        return launch(k_draw<T>, rows, BLOCK, stream, sc, uniforms, uniform_bytes, out, segments, (const Segment *)ws);
+        if (sample_by_waves<T>(rows, n))
+            return launch(k_sample_wave<T>, (rows + WAVES - 1) / WAVES, BLOCK, stream, sc, uniforms, uniform_bytes, out);
+        // (parts of up to four tiles: with many rows a workgroup's start is worth that much)
+        const int tiles = Tile<T, WAVES>::count(n), each = rows >= 256 ? 4 : 1, segments = n_segments<T>(n);
+        if (const int rc = launch(k_sample_parts<T>, dim3((unsigned)((tiles + each - 1) / each), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK, stream,
+                                  sc, each, segments, (Segment *)workspace))
+            return rc;
+        return launch(k_draw<T>, rows, BLOCK, stream, sc, uniforms, uniform_bytes, out, segments, (const Segment *)workspace);
     });
 }
 
