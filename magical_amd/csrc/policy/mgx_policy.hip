@@ -49,6 +49,20 @@ struct Actions {
 
 constexpr int BLOCK = 256, WAVES = BLOCK / 64;
 
+// A whole vector of results.  stream: it is not kept in the caches (STREAM_BYTES below).
+template <typename T, int W> __device__ __forceinline__ void store_bytes(T *to, const T (&v)[W], bool stream) {
+    if constexpr (sizeof v == 16) {
+        using Words = uint32_t __attribute__((ext_vector_type(4), aligned(2)));
+        if (stream) {
+            Words w;
+            __builtin_memcpy(&w, v, 16);
+            __builtin_nontemporal_store(w, (Words *)to);
+            return;
+        }
+    }
+    __builtin_memcpy(to, v, sizeof v);
+}
+
 template <typename T> constexpr uint32_t neg_inf_bits = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, half> ? 0xfc00u : 0xff80u;
 
 // N pieces of W neighbouring scores of a row, as they lie in memory (16-bit scores two a word), with their mask bytes.  One load a piece and
@@ -137,8 +151,8 @@ template <typename T, int W, int N, bool SMALL = false> struct Pieces {
         }
     }
     // W values of type T to `to` from place j on, as far as the row goes
-    static __device__ __forceinline__ void store(T *to, int j, int n, bool whole, const T (&v)[W]) {
-        if (whole || j + W <= n) { __builtin_memcpy(to + j, v, sizeof v); return; }
+    static __device__ __forceinline__ void store(T *to, int j, int n, bool whole, const T (&v)[W], bool stream) {
+        if (whole || j + W <= n) return store_bytes(to + j, v, stream);
         if constexpr (W == 1) return;
         uint32_t q[WORDS];
         __builtin_memcpy(q, v, sizeof v);
@@ -243,6 +257,13 @@ __device__ __forceinline__ double lane_of(double v, int lane) {
 }
 __device__ __forceinline__ int first_lane(uint64_t b) { return __ffsll((unsigned long long)b) - 1; }
 __device__ __forceinline__ int last_lane(uint64_t b) { return 63 - __clzll((long long)b); }
+
+// what lanes of a wavefront have written to LDS is there for its others
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // is (v, i) a better alternative than (w, k)?  Higher score first, then the lower index.
 __device__ __forceinline__ bool better(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
@@ -380,7 +401,7 @@ struct Upstream {          // gradients to the log probabilities and entropies, 
 };
 
 template <typename T, int G, int E, int W>
-__global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions actions, const float *entropy, Upstream up, T *grad) {
+__global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions actions, const float *entropy, Upstream up, T *grad, bool stream) {
     using S = Spread<G, E, W>;
     const int g = threadIdx.x % G, n = (int)sc.n;
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
@@ -406,7 +427,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
             T out[W];
 #pragma unroll
             for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf((x[e + k] - ref) * sc.inv_t2 - log2_s, -1e30f), c0));
-            Pieces<T, W, 1>::store(to, S::place(g, e), n, e / W < n / (G * W), out);
+            Pieces<T, W, 1>::store(to, S::place(g, e), n, e / W < n / (G * W), out, stream);
         }
         if (!finite(c0, c1))          // NaN, but for the places that are not open
 #pragma unroll
@@ -416,6 +437,58 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
             const float xa = row.at(a), d = (xa - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
             to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, -1e30f), c0), gl * sc.inv_t));
         }
+    }
+}
+
+// Up to 32 scores a row, a lane each.  The gradients of a wavefront's 64 rows are one run of memory: they are put together in LDS and stored in 16-byte
+// vectors, neighbours by neighbours (a lane storing its own row writes 16 bytes every 72: 59 us where this takes 30; four lanes a row, a score
+// a store: 38; 983040 rows of 18 fp32).
+template <typename T, int G, int E, int W>
+__global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions actions, const float *entropy, Upstream up, T *grad, bool stream) {
+    static_assert(G == 1);
+    extern __shared__ __align__(16) unsigned char lds_bytes[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (int)sc.n;
+    T *const mine = (T *)lds_bytes + (wave * 64 + lane) * n;
+    const unsigned char *const run = lds_bytes + wave * 64 * n * sizeof(T);
+    for (int64_t r0 = ((int64_t)blockIdx.x * WAVES + wave) * 64; r0 < sc.rows; r0 += (int64_t)gridDim.x * BLOCK) {
+        const int64_t r = r0 + lane;
+        if (r < sc.rows) {
+            const Row<T> row(sc, r);
+            const Given given(actions, row, r, n);
+            const float h = entropy[r], gl = up.lp && given.a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
+            float x[E];
+            Spread<1, E, W>::load_row(row, 0, n, x);
+            const float m = lane_max(x), ref = m > NEG_INF ? m : 0.0f;
+            float s = 0, p[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                p[e] = __builtin_amdgcn_exp2f((x[e] - ref) * sc.inv_t2);
+                s += p[e];
+            }
+            const float inv_s = 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
+            const bool nan = !finite(c0, c1);          // NaN, but for the places that are not open
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (e < n) {
+                    const float v = p[e] * fmaf(c1, fmaxf((x[e] - ref) * sc.inv_t2 - log2_s, -1e30f), c0);
+                    mine[e] = from_f32<T>(nan && x[e] == NEG_INF ? 0.0f : v);
+                }
+            if (given.a >= 0 && given.a < n) {
+                const float d = (given.x - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
+                mine[given.a] = from_f32<T>(given.x == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, -1e30f), c0), gl * sc.inv_t));
+            }
+        }
+        wave_sync();
+        const int bytes = (int)(sc.rows - r0 < 64 ? sc.rows - r0 : 64) * n * (int)sizeof(T);
+        unsigned char *const to = (unsigned char *)(grad + r0 * n);
+        for (int at = lane * 16; at + 16 <= bytes; at += 1024) {
+            uint32_t v[4];
+            __builtin_memcpy(v, __builtin_assume_aligned(run + at, 16), 16);
+            store_bytes((uint32_t *)(to + at), v, stream);
+        }
+        const int at = (bytes & ~15) + lane * (int)sizeof(T);
+        if (at < bytes) __builtin_memcpy(to + at, run + at, sizeof(T));
+        wave_sync();
     }
 }
 
@@ -559,11 +632,6 @@ struct Top {
         if (at_least) bound = ((uint64_t)at_least << 48) - 1;
     }
     __device__ __forceinline__ float bound_score() const { return bound ? score_of((uint32_t)(bound >> 32)) : NEG_INF; }          // (none above it: no key beats it)
-    __device__ __forceinline__ static void sync() {          // LDS between the lanes of one wavefront
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
     // every lane offers one key (0: none)
     __device__ __forceinline__ void offer(uint64_t key) {
         uint64_t who = __ballot(key > bound);
@@ -575,7 +643,7 @@ struct Top {
         const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
         if (key > bound) keys[count + before] = key;
         count += __popcll(who);
-        sync();
+        wave_sync();
     }
     // the k best in order
     __device__ __forceinline__ void sort() {
@@ -588,10 +656,10 @@ struct Top {
             rank_a += other > a;
             rank_b += other > b;
         }
-        sync();
+        wave_sync();
         if (a && rank_a < k) keys[rank_a] = a;
         if (b && rank_b < k) keys[rank_b] = b;
-        sync();
+        wave_sync();
         if (count >= k) {
             count = k;
             bound = keys[k - 1];
@@ -687,7 +755,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
         if constexpr (ROW_WAVES == 1) {
             if constexpr (TOP) best.sort();
             finish_row(sc, r, given, a, best, out);
-            Top::sync();
+            wave_sync();
         } else {
             __syncthreads();
             if (lane == 0) { lds[wave][0] = a.m; lds[wave][1] = a.s; lds[wave][2] = a.t; lds_count[wave] = best.count; }
@@ -734,20 +802,33 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
         a.join_wave(sc.inv_t2);
         Top best(lds_keys, top ? top : 1);
         if (top) {
-            uint64_t most = 0;
-            for (int c = lane; c < parts * top; c += 64) most = keys[c] > most ? keys[c] : most;
-            best.expect(most ? score_of((uint32_t)(most >> 32)) : NEG_INF);
-            for (int c = 0; c < parts * top; c += 64) best.offer(c + lane < parts * top ? keys[c + lane] : 0);
+            for (int c0 = 0; c0 < parts * top; c0 += 512) {          // eight keys a lane at a time
+                uint64_t key[8], most = 0;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int c = c0 + k * 64 + lane;
+                    key[k] = c < parts * top ? keys[c] : 0;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) most = key[k] > most ? key[k] : most;
+                if (c0 == 0) best.expect(most ? score_of((uint32_t)(most >> 32)) : NEG_INF);
+                for (int k = 0; k < 8; k++) {
+                    uint64_t v = key[0];
+#pragma unroll
+                    for (int i = 0; i < 7; i++) key[i] = key[i + 1];
+                    best.offer(v);
+                }
+            }
             best.sort();
         }
         finish_row(sc, r, given, a, best, out);
-        Top::sync();
+        wave_sync();
     }
 }
 
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions actions, const float *stats, const float *entropy, Upstream up,
-                                                         T *grad) {
+                                                         T *grad, bool stream) {
     using L = Tile<T, WAVES>;
     const int n = (int)sc.n;
     for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
@@ -773,7 +854,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
                 const float l2 = fmaf(x[u * L::V + k] - ref, sc.inv_t2, -log2_s);
                 v[k] = from_f32<T>(__builtin_amdgcn_exp2f(l2) * fmaf(c1, fmaxf(l2, -1e30f), c0));
             }
-            if (j < n) Pieces<T, L::V, 1>::store(to, (int)j, n, false, v);
+            if (j < n) Pieces<T, L::V, 1>::store(to, (int)j, n, false, v, stream);
             if (!finite(c0, c1))          // NaN, but for the places that are not open
 #pragma unroll
                 for (int k = 0; k < L::V; k++)
@@ -795,11 +876,9 @@ struct Segment {
 // The segments of a wavefront's vectors of a tile: (tile, u, wave) is segment (tile * U + u) * ROW_WAVES + wave.  put(segment, its sums) for
 // each that there is; t of all of them, against one maximum, comes with the last.
 template <typename T, int ROW_WAVES, typename F>
-__device__ __forceinline__ void sum_segments(const Scores<T> &sc, const Row<T> &row, const Exp64 &exp64, int tile, F put) {
+__device__ __forceinline__ void sum_segments(const Row<T> &row, int n, const Exp64 &exp64, int tile, Tile<T, ROW_WAVES> &now, F put) {
     using L = Tile<T, ROW_WAVES>;
-    const int n = (int)sc.n, live = min(L::live(tile, n), (int)L::U);
-    L now;
-    now.load(row, tile, n);
+    const int live = min(L::live(tile, n), (int)L::U);
     float x[L::U * L::V];
     now.p.scores(row, x);
     const float m = group_max<64>(lane_max(x));
@@ -853,12 +932,18 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
     double before = lane_of(lane == 0 ? 0.0 : upto - s, run), found_before = before;
     int found = run * each;
     if (each > 1)
-        for (int k = 0; k < each; k++) {
-            const Segment g = again(run, k);
-            const double w = exp64(exp64.below(g.m, ref)) * g.s;
-            if (w > NOTHING) { found = run * each + k; found_before = before; }
-            before += w;
-            if (w > NOTHING && before > target) break;
+        for (int k0 = 0; k0 < each; k0 += 64) {
+            const Segment g = k0 + lane < each ? again(run, k0 + lane) : Segment{0, 0, NEG_INF};
+            const double w = exp64(exp64.below(g.m, ref)) * g.s, sum = group_scan<64>(w, lane);
+            past = __ballot(w > NOTHING && before + sum > target);
+            any = __ballot(w > NOTHING);
+            if (any) {
+                const int k = past ? first_lane(past) : last_lane(any);
+                found = run * each + k0 + k;
+                found_before = before + lane_of(lane == 0 ? 0.0 : sum - w, k);
+            }
+            if (past) break;
+            before += lane_of(sum, 63);
         }
     // ... and the action in the segment
     const int64_t j = ((int64_t)found * 64 + lane) * V;
@@ -908,12 +993,16 @@ __global__ __launch_bounds__(BLOCK, 4) void k_sample_wave(Scores<T> sc, const vo
         const Row<T> row(sc, r);
         const double u = uniform_at(uniforms, uniform_bytes, r);
         Segment mine{0, 0, NEG_INF};
-        for (int tile = 0; tile < Tile<T, 1>::count(sc.n); tile++)
-            sum_segments<T, 1>(sc, row, exp64, tile, [&](int g, const Segment &v) {
+        const int n = (int)sc.n;
+        for (int tile = 0; tile < Tile<T, 1>::count(n); tile++) {
+            Tile<T, 1> now;
+            now.load(row, tile, n);
+            sum_segments(row, n, exp64, tile, now, [&](int g, const Segment &v) {
                 mine.s = lane == g ? v.s : mine.s;
                 mine.t = lane == g ? v.t : mine.t;
                 mine.m = lane == g ? v.m : mine.m;
             });
+        }
         draw(sc, row, exp64, r, 1, [&](int) { return mine; }, [&](int, int) { return mine; }, u, out);
     }
 }
@@ -927,8 +1016,11 @@ __global__ __launch_bounds__(BLOCK, 4) void k_sample_parts(Scores<T> sc, int par
     for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
         const Row<T> row(sc, r);
         Segment *to = workspace + r * segments;
-        for (int tile = first; tile < behind; tile++)
-            sum_segments<T, WAVES>(sc, row, exp64, tile, [&](int g, const Segment &v) { if ((threadIdx.x & 63) == 0) to[g] = v; });
+        for (int tile = first; tile < behind; tile++) {
+            L now;
+            now.load(row, tile, (int)sc.n);
+            sum_segments(row, (int)sc.n, exp64, tile, now, [&](int g, const Segment &v) { if ((threadIdx.x & 63) == 0) to[g] = v; });
+        }
     }
 }
 constexpr int LDS_SEGMENTS = 512;          // as many are looked at in LDS
@@ -986,18 +1078,25 @@ Scores<T> scores(const void *logits, int64_t rows, int64_t n, int64_t row_stride
 }
 
 // a grid of at most 2^32 work items; the kernels go on from there in strides of the grid (its last dimension)
-template <typename... P, typename... A> int launch(void (*kernel)(P...), dim3 blocks, int threads, void *stream, A... args) {
+template <typename... P, typename... A> int launch_lds(void (*kernel)(P...), dim3 blocks, int threads, int lds, void *stream, A... args) {
     void *ptrs[] = {(void *)&args...};
     static_assert(sizeof...(P) == sizeof...(A) && (std::is_same_v<P, A> && ...), "argument types are the kernel's");
     const int64_t most = 0xffffffffLL / threads;
     if (blocks.y > most / blocks.x) blocks.y = (unsigned)(most / blocks.x);
-    const hipError_t err = hipLaunchKernel((const void *)kernel, blocks, dim3(threads), ptrs, 0, (hipStream_t)stream);
+    const hipError_t err = hipLaunchKernel((const void *)kernel, blocks, dim3(threads), ptrs, (size_t)lds, (hipStream_t)stream);
     return err == hipSuccess ? (int)MGX_OK : fail(MGX_ERR_HIP, hipGetErrorString(err));
+}
+template <typename... P, typename... A> int launch(void (*kernel)(P...), dim3 blocks, int threads, void *stream, A... args) {
+    return launch_lds(kernel, blocks, threads, 0, stream, args...);
 }
 template <typename... P, typename... A> int launch(void (*kernel)(P...), int64_t blocks, int threads, void *stream, A... args) {
     return launch(kernel, dim3((unsigned)std::min<int64_t>(blocks, 0xffffffffLL / threads)), threads, stream, args...);
 }
 
+// Gradients of this size go past the caches: a quarter of the 256 MB that memory has in front of it would be filled with what is read
+// once, much later, and written back while the next kernels read.  1024 x 104976 bf16 (215 MB): backward 84 -> 72 us, and the forward
+// pass after it 58 -> 44; 983040 x 18 fp32 (71 MB): 29.4 -> 28.2 and 20.9 -> 17.2; 61440 x 324 bf16 (40 MB): no difference.
+constexpr int64_t STREAM_BYTES = 64 << 20;
 constexpr int SHORT_MAX = 2048;
 template <int G_, int E_, int W_> struct Shape { static constexpr int G = G_, E = E_, W = W_; };
 // f(lanes a row, scores a lane, scores a load) for rows of n <= SHORT_MAX: up to 32 scores in one lane (no exchanges at all); beyond, the
@@ -1148,17 +1247,22 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
     DeviceGuard guard(device);
     if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
     const Actions given{actions, action_bytes};
+    const bool stream_out = rows * n * (dtype == MGX_REAL_F32 ? 4 : 2) >= STREAM_BYTES;
     const Upstream up{grad_log_prob, grad_entropy, grad_log_prob_stride, grad_entropy_stride};
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (n <= SHORT_MAX)
-            return by_length_64<T>(n, [&](auto shape) {
+            return by_length<T>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
-                return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad);
+                if constexpr (G == 1) {
+                    const int64_t blocks = std::min<int64_t>((rows + BLOCK - 1) / BLOCK, 0xffffffffLL / BLOCK);
+                    return launch_lds(k_backward_lane<T, G, E, W>, dim3((unsigned)blocks), BLOCK, (int)(BLOCK * n * sizeof(T)), stream, sc, given, entropy,
+                                      up, (T *)grad, stream_out);
+                } else return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad, stream_out);
             });
         return launch(k_backward_long<T>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
-                      stream, sc, given, stats, entropy, up, (T *)grad);
+                      stream, sc, given, stats, entropy, up, (T *)grad, stream_out);
     });
 }
 
