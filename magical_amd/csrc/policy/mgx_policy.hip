@@ -622,13 +622,18 @@ struct Top {
     uint64_t bound = 0;      // what a key has to exceed
     int count = 0, k;
     __device__ Top(uint64_t *lds, int k_) : keys(lds), k(k_) {}
-    // Before the first offers: `x` is one score that each lane is going to offer.  The k-th best of these 64 bounds the k-th best of all from
-    // below; found bit by bit (16 of them: the bound may be lower), it keeps most of the scores out that would not last.
-    __device__ __forceinline__ void expect(float x) {
-        const uint32_t order = x > NEG_INF ? order_of(x) >> 16 : 0;
-        uint32_t at_least = 0;
-        for (uint32_t bit = 0x8000; bit; bit >>= 1)
-            if (__popcll(__ballot(order >= (at_least | bit))) >= k) at_least |= bit;
+    // Before the first offers: x are N scores that each lane is going to offer, the best of some each.  The k-th best of these 64 N bounds the
+    // k-th best of all from below; found bit by bit (16 of them: the bound may be lower), it keeps most of the scores out that would not last.
+    template <int N> __device__ __forceinline__ void expect(const float (&x)[N]) {
+        uint32_t order[N], at_least = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) order[i] = x[i] > NEG_INF ? order_of(x[i]) >> 16 : 0;
+        for (uint32_t bit = 0x8000; bit; bit >>= 1) {
+            int reach = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) reach += __popcll(__ballot(order[i] >= (at_least | bit)));
+            if (reach >= k) at_least |= bit;
+        }
         if (at_least) bound = ((uint64_t)at_least << 48) - 1;
     }
     __device__ __forceinline__ float bound_score() const { return bound ? score_of((uint32_t)(bound >> 32)) : NEG_INF; }          // (none above it: no key beats it)
@@ -720,9 +725,15 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
         for (int tile = first; tile < behind; tile++) {
             L now;
             now.load(row, tile, n);
-            float x[L::U * L::V], m;
+            float x[L::U * L::V], um[L::U];
             now.p.scores(row, x);
-            m = lane_max(x);
+#pragma unroll
+            for (int u = 0; u < L::U; u++) {
+                um[u] = x[u * L::V];
+#pragma unroll
+                for (int k = 1; k < L::V; k++) um[u] = max_of(um[u], x[u * L::V + k]);
+            }
+            const float m = lane_max(um);
             if (m > a.m) a.to(m, sc.inv_t2);
             const float ref = a.m > NEG_INF ? a.m : 0.0f;
             const int live = L::live(tile, n);
@@ -736,7 +747,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                         a.t = fmaf(p, fmaxf(d, -1e30f), a.t);
                     }
             if constexpr (TOP) {
-                if (tile == first) best.expect(m);
+                if (tile == first) best.expect(um);
                 // (the wavefront's places ascend: a later tile's score that only equals the k-th best is behind it)
                 const float bound = best.bound_score();
                 if (__ballot(tile == first ? m >= bound : m > bound)) {
@@ -803,15 +814,20 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
         Top best(lds_keys, top ? top : 1);
         if (top) {
             for (int c0 = 0; c0 < parts * top; c0 += 512) {          // eight keys a lane at a time
-                uint64_t key[8], most = 0;
+                uint64_t key[8];
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const int c = c0 + k * 64 + lane;
                     key[k] = c < parts * top ? keys[c] : 0;
                 }
+                if (c0 == 0) {          // (64 samples bound up to half as many well; eight times as many take eight times as long)
+                    float x[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) most = key[k] > most ? key[k] : most;
-                if (c0 == 0) best.expect(most ? score_of((uint32_t)(most >> 32)) : NEG_INF);
+                    for (int k = 0; k < 8; k++) x[k] = key[k] ? score_of((uint32_t)(key[k] >> 32)) : NEG_INF;
+                    const float most[1] = {lane_max(x)};
+                    if (top <= 32) best.expect(most);
+                    else best.expect(x);
+                }
                 for (int k = 0; k < 8; k++) {
                     uint64_t v = key[0];
 #pragma unroll
@@ -900,14 +916,20 @@ __device__ __forceinline__ void sum_segments(const Row<T> &row, int n, const Exp
     }
 }
 
-// One wavefront: the row's action.  Every lane has a run of `each` neighbouring segments from lane * each on; of(k) is its k-th, and
-// again(run, k) the k-th of another lane's.
-template <typename T, typename F, typename A>
+// One wavefront: the row's action.  Every lane has a run of `each` neighbouring segments from lane * each on; of(k) is its k-th (empty from
+// `each` on), and again(run, k) the k-th of another lane's.  STEP segments are looked at together.
+template <int STEP, typename T, typename F, typename A>
 __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, const Exp64 &exp64, int64_t r, int each, F of, A again, double u, const Drawn &out) {
     constexpr int V = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, n = (int)sc.n;
     float m = NEG_INF;
-    for (int k = 0; k < each; k++) m = max_of(m, of(k).m);
+    for (int k = 0; k < each; k += STEP) {
+        Segment g[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; i++) g[i] = of(k + i);
+#pragma unroll
+        for (int i = 0; i < STEP; i++) m = max_of(m, g[i].m);
+    }
     m = group_max<64>(m);
     const bool some = m > NEG_INF, undefined = m != m || m == -NEG_INF;
     if (undefined || !some) {
@@ -916,11 +938,16 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
     }
     const double ref = m;
     double s = 0, t = 0;
-    for (int k = 0; k < each; k++) {
-        const Segment g = of(k);
-        const double d = exp64.below(g.m, ref), w = exp64(d);
-        s = fma(w, g.s, s);
-        t = fma(w, fma(d, g.s, g.t), t);
+    for (int k = 0; k < each; k += STEP) {
+        Segment g[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; i++) g[i] = of(k + i);
+#pragma unroll
+        for (int i = 0; i < STEP; i++) {
+            const double d = exp64.below(g[i].m, ref), w = exp64(d);
+            s = fma(w, g[i].s, s);
+            t = fma(w, fma(d, g[i].s, g[i].t), t);
+        }
     }
     double upto = group_scan<64>(s, lane);
     const double total = lane_of(upto, 63);
@@ -1003,24 +1030,21 @@ __global__ __launch_bounds__(BLOCK, 4) void k_sample_wave(Scores<T> sc, const vo
                 mine.m = lane == g ? v.m : mine.m;
             });
         }
-        draw(sc, row, exp64, r, 1, [&](int) { return mine; }, [&](int, int) { return mine; }, u, out);
+        draw<1>(sc, row, exp64, r, 1, [&](int) { return mine; }, [&](int, int) { return mine; }, u, out);
     }
 }
 
-// longer rows: workgroups sum parts of part_tiles tiles each, a wavefront draws
+// longer rows: workgroups sum a tile each, a wavefront draws
 template <typename T>
-__global__ __launch_bounds__(BLOCK, 4) void k_sample_parts(Scores<T> sc, int part_tiles, int segments, Segment *workspace) {
+__global__ __launch_bounds__(BLOCK, 4) void k_sample_parts(Scores<T> sc, int segments, Segment *workspace) {
     using L = Tile<T, WAVES>;
     const Exp64 exp64(sc.inv_t2_64);
-    const int first = (int)blockIdx.x * part_tiles, behind = min(first + part_tiles, L::count(sc.n));
     for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
         const Row<T> row(sc, r);
         Segment *to = workspace + r * segments;
-        for (int tile = first; tile < behind; tile++) {
-            L now;
-            now.load(row, tile, (int)sc.n);
-            sum_segments(row, (int)sc.n, exp64, tile, now, [&](int g, const Segment &v) { if ((threadIdx.x & 63) == 0) to[g] = v; });
-        }
+        L now;
+        now.load(row, blockIdx.x, (int)sc.n);
+        sum_segments(row, (int)sc.n, exp64, (int)blockIdx.x, now, [&](int g, const Segment &v) { if ((threadIdx.x & 63) == 0) to[g] = v; });
     }
 }
 constexpr int LDS_SEGMENTS = 512;          // as many are looked at in LDS
@@ -1039,9 +1063,9 @@ __global__ __launch_bounds__(BLOCK) void k_draw(Scores<T> sc, const void *unifor
         const int lane = threadIdx.x, each = (segments + 63) / 64;
         const auto at = [&](int run, int k) {
             const int g = run * each + k;
-            return g < segments ? seg[g] : Segment{0, 0, NEG_INF};
+            return k < each && g < segments ? seg[g] : Segment{0, 0, NEG_INF};
         };
-        if (threadIdx.x < 64) draw(sc, Row<T>(sc, r), exp64, r, each, [&](int k) { return at(lane, k); }, at, u, out);
+        if (threadIdx.x < 64) draw<8>(sc, Row<T>(sc, r), exp64, r, each, [&](int k) { return at(lane, k); }, at, u, out);
         __syncthreads();
     }
 }
@@ -1097,10 +1121,15 @@ template <typename... P, typename... A> int launch(void (*kernel)(P...), int64_t
 // once, much later, and written back while the next kernels read.  1024 x 104976 bf16 (215 MB): backward 84 -> 72 us, and the forward
 // pass after it 58 -> 44; 983040 x 18 fp32 (71 MB): 29.4 -> 28.2 and 20.9 -> 17.2; 61440 x 324 bf16 (40 MB): no difference.
 constexpr int64_t STREAM_BYTES = 64 << 20;
-constexpr int SHORT_MAX = 2048;
+// Rows of up to 2 KB of scores stay in a few lanes' registers.  Measured against a wavefront a row that goes over it in tiles, 65536 rows (log
+// probabilities / with five alternatives / draws, us): 600 bf16 23 / 57 / 84 against 36 / 79 / 116, 1000 bf16 30 / 72 / 105 against 38 / 81 /
+// 116; 1500 bf16 53 / 117 / 170 against 53 / 96 / 151, 1000 fp32 52 / 100 / 151 against 53 / 74 / 118.
+template <typename T> constexpr bool is_short(int64_t n) { return n * (int64_t)sizeof(T) <= 2048; }
+// The backward pass, which needs no second look, keeps rows of up to 2048 scores there, and needs nothing of the forward pass for them.
+constexpr int BACKWARD_SHORT_MAX = 2048;
 template <int G_, int E_, int W_> struct Shape { static constexpr int G = G_, E = E_, W = W_; };
-// f(lanes a row, scores a lane, scores a load) for rows of n <= SHORT_MAX: up to 32 scores in one lane (no exchanges at all); beyond, the
-// fewest lanes that hold the row in four 16-byte pieces each, or all 64.
+// f(lanes a row, scores a lane, scores a load): up to 32 scores in one lane (no exchanges at all); beyond, the fewest lanes that hold the row
+// in four 16-byte pieces each, or 64.
 template <typename T, int G, typename F> int by_pieces(int64_t n, F f) {
     constexpr int W = 16 / sizeof(T);
     const int64_t c = (n + G * W - 1) / (G * W);
@@ -1113,16 +1142,19 @@ template <typename T, int G, typename F> int by_pieces(int64_t n, F f) {
         return f(Shape<G, 8 * W, W>());
     }
 }
-template <typename T, typename F> int by_lanes(int64_t n, F f) {
+template <typename T, bool BACKWARD, typename F> int by_lanes(int64_t n, F f) {
     const int64_t lanes = (n + 64 / sizeof(T) - 1) / (64 / sizeof(T));
     if (lanes <= 4) return by_pieces<T, 4>(n, f);
     if (lanes <= 8) return by_pieces<T, 8>(n, f);
     if (lanes <= 16) return by_pieces<T, 16>(n, f);
-    if (lanes <= 32) return by_pieces<T, 32>(n, f);
-    return by_pieces<T, 64>(n, f);
+    if constexpr (!BACKWARD) return by_pieces<T, 32>(n, f);
+    else {
+        if (lanes <= 32) return by_pieces<T, 32>(n, f);
+        return by_pieces<T, 64>(n, f);
+    }
 }
-template <typename T, typename F> int by_length(int64_t n, F f) {
-    if (n > 32) return by_lanes<T>(n, f);
+template <typename T, bool BACKWARD, typename F> int by_length(int64_t n, F f) {
+    if (n > 32) return by_lanes<T, BACKWARD>(n, f);
     switch ((n + 3) / 4) {
         case 1: return f(Shape<1, 4, 4>());
         case 2: return f(Shape<1, 8, 4>());
@@ -1136,7 +1168,7 @@ template <typename T, typename F> int by_length(int64_t n, F f) {
 }
 // Drawing: up to 32 scores over four lanes (64-bit exponentials take twenty times what an exchange takes)
 template <typename T, typename F> int by_length_64(int64_t n, F f) {
-    if (n > 32) return by_lanes<T>(n, f);
+    if (n > 32) return by_lanes<T, false>(n, f);
     switch ((n + 3) / 4) {
         case 1: return f(Shape<4, 1, 1>());
         case 2: return f(Shape<4, 2, 1>());
@@ -1148,21 +1180,31 @@ template <typename T, typename F> int by_length_64(int64_t n, F f) {
         default: return f(Shape<4, 8, 1>());
     }
 }
-// How a long row is shared out.  4096 rows or more: a wavefront each (four for every SIMD; no exchange between wavefronts).  Fewer: a workgroup
-// each, or several where that leaves CUs without one, no more than the row has tiles.
+// How a long row is shared out: a wavefront a row (no exchange between wavefronts) where these are many or the rows not that long, else a
+// workgroup, or several where that leaves CUs without one (no more than the row has tiles).  Measured (log probabilities / with five
+// alternatives, us; wavefront against workgroup): 512 x 2500 bf16 5.1 / 7.6 against 5.1 / 7.4, 2048 x 2500 5.3 / 8.9 against 6.9 / 14.4;
+// 512 x 5832 5.5 / 10.3 against 5.0 / 7.9, 2048 x 5832 8.2 / 13.4 against 9.9 / 17.4, 4096 x 5832 12.2 / 18.0 against 15.1 / 28.7; 1024 x 20000
+// 14.9 / 29.5 against 12.0 / 18.3, 2048 x 20000 18.8 / 33.7 against 19.4 / 31.0, 4096 x 20000 32.6 / 50.0 against 35.0 / 60.5.
 struct Split {
     int row_waves, parts, part_tiles;
 };
 template <typename T> Split split(int64_t rows, int64_t n) {
-    if (rows >= 4096) return {1, 1, 0};
+    const int64_t wave_tiles = Tile<T, 1>::count(n);
+    if (wave_tiles <= 2 || rows >= 4096 || (rows >= 2048 && wave_tiles <= 8)) return {1, 1, 0};
     const int64_t tiles = Tile<T, WAVES>::count(n), wanted = std::max<int64_t>(1, std::min<int64_t>(tiles, 1024 / std::max<int64_t>(rows, 1)));
     const int64_t each = (tiles + wanted - 1) / wanted;
     return {WAVES, (int)((tiles + each - 1) / each), (int)each};
 }
+// Short rows' alternatives come one after the other, a pass over the registers each; from nine on, of rows of some length, a wavefront a row that
+// collects and ranks them is faster (7 x 1000 fp32, 20 of them: 5.6 us against 14.6 in passes).
+template <typename T> bool in_lanes(int64_t n, int top) { return is_short<T>(n) && !(n > 256 && top > 8); }
 template <typename T> int n_segments(int64_t n) { return (int)((n + 64 * (16 / sizeof(T)) - 1) / (64 * (16 / sizeof(T)))); }
-// Drawing: a wavefront a row up to four tiles, or up to 64 segments if there are rows enough
+// Drawing: a wavefront a row up to 12 tiles where there are rows enough, else a workgroup a tile and a second kernel.  Measured (us; the first against the
+// second): 16 x 2500 bf16 7.7 against 9.9; 16 x 5832 11.4 against 9.9, 1024 x 5832 12.1 against 14.4, 4096 x 5832 28 against 44; 1024 x 20000
+// 33 against 27, 2048 x 20000 45 against 48, 4096 x 20000 80 against 94; fp32, 20 tiles: 2048 x 20000 76 against 57.
 template <typename T> bool sample_by_waves(int64_t rows, int64_t n) {
-    return Tile<T, 1>::count(n) <= 4 || (rows >= 1024 && n_segments<T>(n) <= 64);
+    const int64_t tiles = Tile<T, 1>::count(n);
+    return tiles <= 2 || (tiles <= 4 && rows >= 512) || (tiles <= 12 && rows >= 2048);          // (at most 48 segments: a lane each)
 }
 
 int64_t short_blocks(int64_t rows, int G) { return (rows * G + BLOCK - 1) / BLOCK; }
@@ -1183,9 +1225,10 @@ extern "C" {
 const char *mgx_policy_last_error(void) { return g_err; }
 
 int64_t mgx_policy_workspace_bytes(int op, int dtype, int64_t rows, int64_t n, int top) {
-    if (n <= SHORT_MAX || rows <= 0) return 0;
+    if (n <= 0 || rows <= 0) return 0;
     const auto bytes = [&](auto v) -> int64_t {
         using T = decltype(v);
+        if (op == MGX_POLICY_SAMPLE ? is_short<T>(n) : in_lanes<T>(n, top)) return 0;
         if (op == MGX_POLICY_SAMPLE) return sample_by_waves<T>(rows, n) ? 0 : rows * n_segments<T>(n) * (int64_t)sizeof(Segment);
         const Split sp = split<T>(rows, n);
         return sp.parts == 1 ? 0 : rows * sp.parts * (16 + 8 * (int64_t)top);
@@ -1193,7 +1236,7 @@ int64_t mgx_policy_workspace_bytes(int op, int dtype, int64_t rows, int64_t n, i
     return dtype == MGX_REAL_F32 ? bytes(float()) : bytes(half());
 }
 
-int64_t mgx_policy_stats_bytes(int64_t rows, int64_t n) { return n > SHORT_MAX ? rows * 8 : 0; }
+int64_t mgx_policy_stats_bytes(int64_t rows, int64_t n) { return n > BACKWARD_SHORT_MAX ? rows * 8 : 0; }
 
 int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride, const uint8_t *mask,
                          int64_t mask_row_stride, double temperature, const void *actions, int action_bytes, int top, float *log_prob,
@@ -1212,8 +1255,8 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
-        if (n <= SHORT_MAX)
-            return by_length<T>(n, [&](auto shape) {
+        if (in_lanes<T>(n, top))
+            return by_length<T, false>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
                 return launch(k_log_probs_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, top,
                               log_prob, entropy, top_log_probs, top_actions);
@@ -1252,8 +1295,8 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
-        if (n <= SHORT_MAX)
-            return by_length<T>(n, [&](auto shape) {
+        if (n <= BACKWARD_SHORT_MAX)
+            return by_length<T, true>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
                 if constexpr (G == 1) {
                     const int64_t blocks = std::min<int64_t>((rows + BLOCK - 1) / BLOCK, 0xffffffffLL / BLOCK);
@@ -1281,17 +1324,16 @@ int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, i
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
-        if (n <= SHORT_MAX)
+        if (is_short<T>(n))
             return by_length_64<T>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
                 return launch(k_sample_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, uniforms, uniform_bytes, out);
             });
         if (sample_by_waves<T>(rows, n))
             return launch(k_sample_wave<T>, (rows + WAVES - 1) / WAVES, BLOCK, stream, sc, uniforms, uniform_bytes, out);
-        // (parts of up to four tiles: with many rows a workgroup's start is worth that much)
-        const int tiles = Tile<T, WAVES>::count(n), each = rows >= 256 ? 4 : 1, segments = n_segments<T>(n);
-        if (const int rc = launch(k_sample_parts<T>, dim3((unsigned)((tiles + each - 1) / each), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK, stream,
-                                  sc, each, segments, (Segment *)workspace))
+        const int segments = n_segments<T>(n);
+        if (const int rc = launch(k_sample_parts<T>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK, stream, sc,
+                                  segments, (Segment *)workspace))
             return rc;
         return launch(k_draw<T>, rows, BLOCK, stream, sc, uniforms, uniform_bytes, out, segments, (const Segment *)workspace);
     });

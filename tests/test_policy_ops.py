@@ -440,7 +440,7 @@ def test_strides_offsets_and_orders_change_no_bit(n, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize('rows,n', [((1 << 20) + 3, 18), (300007, 5), (70001, 324), (5003, 2500)])
+@pytest.mark.parametrize('rows,n', [((1 << 20) + 3, 18), (2000003, 31), (300007, 5), (200003, 324), (5003, 2500), (40009, 1700), (1031, 40000)])
 def test_many_rows(rows, n):
     """Every row of a large batch is worked on: the results of row subsets equal those of the whole."""
     import torch
@@ -466,6 +466,40 @@ def test_many_rows(rows, n):
     cut = rows - 1234
     part = m.sample_actions(x[cut:], u[cut:])
     assert torch.equal(part.action, drawn.action[cut:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('n,rows', [(18, 5000), (40, 700), (700, 3000), (3000, 600), (3000, 4200), (9000, 40), (9000, 2100), (9000, 4100), (30011, 700),
+                                    (30011, 2100)])
+def test_every_row_alike_in_every_launch_shape(n, rows, dtype):
+    """The special rows (nothing open, one action, all equal, the lowest value, ties, masks), repeated to many: how rows are shared out over lanes,
+    wavefronts and workgroups goes by their number and length.  One copy against 64 bits, the others the same bits."""
+    import torch
+    import magical_amd as m
+    x, mask, actions, rng = _case(n, dtype, n + rows, rows=13, masked='rows')
+    copies = -(-rows // 13)
+    rep = lambda t: torch.as_tensor(t).repeat((copies,) + (1,) * (torch.as_tensor(t).dim() - 1))[:rows].cuda()      # noqa: E731
+    u = rng.rand(13)
+    g_lp, g_h = rng.randn(13).astype(np.float32), (rng.randn(13) * 0.1).astype(np.float32)
+    leaf = rep(x).requires_grad_(True)
+    for top in (0, 5, 40):
+        top = min(top, n)
+        out = m.action_log_probs(leaf, rep(actions), mask=rep(mask), temperature=1.3, top=top)
+        first = m.policy.ActionLogProbs(*(None if t is None else t[:13] for t in out))
+        is_open, lp, h, bad = _check_forward(first, x.double().numpy(), mask, actions, 1.3, top, (n, rows, dtype, top))
+        for t in out:
+            assert t is None or torch.equal(t, rep(t[:13]))
+    grad, = torch.autograd.grad((out.log_prob, out.entropy), (leaf,), (rep(g_lp), rep(g_h)))
+    want = oracle_grad(is_open, lp, h, actions, g_lp.astype(np.float64), g_h.astype(np.float64), 1.3)
+    bound = err_grad(is_open, lp, h, g_lp.astype(np.float64), g_h.astype(np.float64), want, 1.3, torch.finfo(x.dtype).eps, 0.0)
+    assert np.all(np.abs(grad[:13].double().cpu().numpy() - want) <= bound)
+    assert torch.equal(grad, rep(grad[:13]))
+    drawn = m.sample_actions(leaf.detach(), rep(u), mask=rep(mask), temperature=1.3)
+    want_a, gap = oracle_draw(*oracle(x.double().numpy(), mask, 1.3)[:2], u)
+    assert (gap > 1e-11).all() and np.array_equal(drawn.action[:13].cpu().numpy(), want_a)
+    for t in drawn:
+        assert torch.equal(t, rep(t[:13]))
 
 
 @pytest.mark.gpu
