@@ -10,7 +10,7 @@
  *
  * The scores: `logits` points at element (0, 0) of rows x n values of type `dtype` (mgx_real), value (r, j) at r * row_stride + j
  * (elements; any stride >= 0: rows may overlap or coincide, as an expanded tensor's do; no alignment beyond the element's).  `mask`:
- * NULL, or u8 at r * mask_row_stride + j: 1, or 0 = action j is ruled out in row r.  An action is OPEN if its mask is not 0 and its
+ * NULL, or u8 at r * mask_row_stride + j, 0 = action j is ruled out in row r.  An action is OPEN if its mask is not 0 and its
  * score is not -inf.  With the open scores x, m = max x, T = temperature:
  *     d_j = (x_j - m) / T,  s = sum e^d_j,   log p_j = d_j - log s,   entropy H = -sum p_j log p_j = log s - (sum d_j e^d_j) / s
  *   - an action that is not open has log p = -inf, takes no part in H and gets gradient 0;

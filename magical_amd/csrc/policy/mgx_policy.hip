@@ -68,9 +68,9 @@ template <typename T> constexpr uint32_t neg_inf_bits = sizeof(T) == 4 ? 0xff800
 // N pieces of W neighbouring scores of a row, as they lie in memory (16-bit scores two a word), with their mask bytes.  One load a piece and
 // one for its mask (gfx950 loads any alignment); what is behind the row's end is -inf.  SMALL: n may be less than W.
 template <typename T, int W, int N, bool SMALL = false> struct Pieces {
-    static constexpr int BITS = 8 * sizeof(T), WORDS = W * BITS < 32 ? 1 : W * BITS / 32, MASK_WORDS = (W + 3) / 4;
+    static constexpr int BITS = 8 * sizeof(T), WORDS = W * BITS / 32, MASK_WORDS = W / 4;
     uint32_t w[N][WORDS], open[N][MASK_WORDS];
-    static_assert(W == 1 || W >= 4);
+    static_assert(W % 4 == 0);
     using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
     static constexpr uint32_t CLOSED = sizeof(T) == 4 ? neg_inf_bits<T> : neg_inf_bits<T> << 16 | neg_inf_bits<T>;
     // v shifted down by `bits` (0 ... 64 * words), zeros from above
@@ -93,11 +93,7 @@ template <typename T, int W, int N, bool SMALL = false> struct Pieces {
     }
     // Piece p from place j on.  Where the row ends inside it (or before it), the row's last W scores are loaded instead and shifted down.
     __device__ __forceinline__ void fetch(const Row<T> &row, int p, int j, int n, bool whole) {
-        if (W == 1) {
-            Bits b;
-            __builtin_memcpy(&b, row.x + (j < n ? j : n - 1), sizeof b);
-            w[p][0] = j < n ? b : neg_inf_bits<T>;
-        } else if (whole) __builtin_memcpy(w[p], row.x + j, W * sizeof(T));
+        if (whole) __builtin_memcpy(w[p], row.x + j, W * sizeof(T));
         else if (!SMALL || n >= W) {
             const int from = j < n - W ? j : n - W, bits = (j - from < W ? j - from : W) * BITS;
             __builtin_memcpy(w[p], row.x + from, W * sizeof(T));
@@ -119,8 +115,7 @@ template <typename T, int W, int N, bool SMALL = false> struct Pieces {
         }
     }
     __device__ __forceinline__ void fetch_mask(const Row<T> &row, int p, int j, int n, bool whole) {
-        if (W == 1) open[p][0] = row.mask[j < n ? j : n - 1];
-        else if (whole) __builtin_memcpy(open[p], row.mask + j, W);
+        if (whole) __builtin_memcpy(open[p], row.mask + j, W);
         else if (!SMALL || n >= W) {
             const int from = j < n - W ? j : n - W;
             __builtin_memcpy(open[p], row.mask + from, W);
@@ -153,7 +148,6 @@ template <typename T, int W, int N, bool SMALL = false> struct Pieces {
     // W values of type T to `to` from place j on, as far as the row goes
     static __device__ __forceinline__ void store(T *to, int j, int n, bool whole, const T (&v)[W], bool stream) {
         if (whole || j + W <= n) return store_bytes(to + j, v, stream);
-        if constexpr (W == 1) return;
         uint32_t q[WORDS];
         __builtin_memcpy(q, v, sizeof v);
         int left = n - j;
@@ -174,21 +168,22 @@ template <typename T, int W, int N, bool SMALL = false> struct Pieces {
         else if constexpr (std::is_same_v<T, half>) return (float)__builtin_bit_cast(half, (uint16_t)(w[p][k / 2] >> (k % 2 * 16)));
         else return __builtin_bit_cast(float, k % 2 ? w[p][k / 2] & 0xffff0000u : w[p][k / 2] << 16);
     }
-    // the N * W scores in fp32, -inf where the mask rules them out (its bytes are 0 or 1: spread to all bits, they select)
+    // the N * W scores in fp32, -inf where the mask rules them out (a byte less 1 is negative if it was 0, and only then: spread to all bits,
+    // its sign selects)
     __device__ __forceinline__ void scores(const Row<T> &row, float *x) {
         if (row.mask)
 #pragma unroll
             for (int p = 0; p < N; p++)
 #pragma unroll
                 for (int k = 0; k < WORDS; k++) {
-                    uint32_t all;
-                    if constexpr (sizeof(T) == 4) all = (uint32_t)((int32_t)(open[p][k / 4] << (31 - k % 4 * 8)) >> 31);
+                    uint32_t shut;
+                    if constexpr (sizeof(T) == 4) shut = (uint32_t)(((int32_t)(open[p][k / 4] >> (k % 4 * 8) & 0xff) - 1) >> 31);
                     else {
                         using Two16 = short __attribute__((ext_vector_type(2)));
-                        const Two16 ones = __builtin_bit_cast(Two16, __builtin_amdgcn_perm(0, open[p][k / 2], k % 2 ? 0x0c030c02 : 0x0c010c00));
-                        all = __builtin_bit_cast(uint32_t, -ones);
+                        const Two16 bytes = __builtin_bit_cast(Two16, __builtin_amdgcn_perm(0, open[p][k / 2], k % 2 ? 0x0c030c02 : 0x0c010c00));
+                        shut = __builtin_bit_cast(uint32_t, (Two16)((bytes - (Two16){1, 1}) >> (Two16){15, 15}));
                     }
-                    w[p][k] = (all & w[p][k]) | (~all & CLOSED);
+                    w[p][k] = (shut & CLOSED) | (~shut & w[p][k]);
                 }
 #pragma unroll
         for (int p = 0; p < N; p++)
@@ -305,8 +300,10 @@ struct Exp64 {
 constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
-// A row of up to 2048 scores stays in the registers of G lanes (1 ... 64), E a lane: one read of the scores, all sums by lane exchanges, no
-// LDS, no barrier.  Lane g holds pieces of W neighbouring scores (16 bytes, or 1): x[e] is score place(g, e).
+// A row stays in the registers of G lanes (1 ... 64), E scores a lane: one read of the scores, all sums by lane exchanges, no barrier.  What
+// bounds it: memory (983040 x 18 fp32: 17 us, 5.1 TB/s; backward 28 us, 5.6 TB/s), from some dozen scores a row on also the vector unit,
+// which issues ten to twelve instructions a score, the exponential counted as four (61440 x 324 bf16 with a mask: 14 us where memory would take
+// 8; backward 24 where it would take 16).  Lane g holds pieces of W neighbouring scores (16 bytes, or 4 scores): x[e] is score place(g, e).
 template <int G, int E, int W> struct Spread {
     static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
     template <typename T> static __device__ __forceinline__ void load_row(const Row<T> &row, int g, int n, float (&x)[E]) {
@@ -380,7 +377,6 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
             if constexpr (G > 4) take(dpp<DPP_HALF_MIRROR>(v), dpp<DPP_HALF_MIRROR>(i));
             if constexpr (G > 8) take(dpp<DPP_MIRROR>(v), dpp<DPP_MIRROR>(i));
             if constexpr (G > 16) { const auto ov = swap<16>(v); const auto oi = swap<16>(i); take(ov.a, oi.a); take(ov.b, oi.b); }
-            if constexpr (G > 32) { const auto ov = swap<32>(v); const auto oi = swap<32>(i); take(ov.a, oi.a); take(ov.b, oi.b); }
             if (k + 1 < top)
 #pragma unroll
                 for (int e = 0; e < E; e++) x[e] = S::place(g, e) == i ? NEG_INF : x[e];
@@ -516,8 +512,8 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const double u = uniform_at(uniforms, uniform_bytes, r);
         float x[E];
         {
-            Pieces<T, W, E / W> p;
-            p.load(row, n, n / (G * E) * (E / W), E / W, [&](int k) { return g * E + k * W; });
+            Pieces<T, W, E / W, G == 1> p;
+            p.load(row, n, G == 1 ? n / W : n / (G * E) * (E / W), E / W, [&](int k) { return g * E + k * W; });
             p.scores(row, x);
         }
         const float m = group_max<G>(lane_max(x));
@@ -535,7 +531,7 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const double upto = group_scan<G>(s, g), total = __shfl(upto, G - 1, G);
         t = group_sum<G>(t);
         const int group = (threadIdx.x & 63) - g;
-        const uint64_t in_group = G == 64 ? ~0ull : ((1ull << (G & 63)) - 1) << group;
+        const uint64_t in_group = ((1ull << G) - 1) << group;
         const bool undefined = m != m || m == -NEG_INF, none = undefined || !some;
         const double target = u * total;
         // the first lane that passes the target, or else (rounding; a number of 1) the last one with anything in it
@@ -560,8 +556,11 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 }
 
 // ----------------------------------------------------------------------------------------------------------------- long rows
-// A workgroup goes over a row, or over one part of it where there are few rows, in tiles of U 16-byte vectors a lane: running maximum, sum and
-// weighted sum per lane, joined at the end.
+// A wavefront or workgroup goes over a row, or over one part of it where there are few rows, in tiles of U 16-byte vectors a lane: running
+// maximum, sum and weighted sum per lane, joined at the end; every score is read once.  What bounds it: memory (1024 x 104976 bf16: 44 us,
+// 4.9 TB/s; backward 72 us, 6.0 TB/s), with masks and alternatives the vector unit too (4096 x 5832 bf16, a mask, five alternatives: 21 us
+// where memory would take 14), and with few rows two launches (7 x 50021 fp32, 20 alternatives: 8 and 5 us).  Loading the next tile ahead of
+// the present one's arithmetic made it slower (58 -> 64 and 22 -> 28 us): registers, and other wavefronts hide the loads already.
 
 // ROW_WAVES: wavefronts that go over the tile together (1, or the workgroup's 4)
 template <typename T, int ROW_WAVES> struct Tile {
@@ -842,12 +841,15 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
     }
 }
 
-template <typename T>
+// blockIdx.x: the tile, of a wavefront (ROW_WAVES 1, four rows a workgroup) or a workgroup (4)
+template <typename T, int ROW_WAVES>
 __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions actions, const float *stats, const float *entropy, Upstream up,
                                                          T *grad, bool stream) {
-    using L = Tile<T, WAVES>;
+    using L = Tile<T, ROW_WAVES>;
+    constexpr int ROWS = WAVES / ROW_WAVES;
     const int n = (int)sc.n;
-    for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
+    for (int64_t r = (int64_t)blockIdx.y * ROWS + (ROW_WAVES == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0); r < sc.rows;
+         r += (int64_t)gridDim.y * ROWS) {
         const Row<T> row(sc, r);
         L tile;
         tile.load(row, blockIdx.x, n);
@@ -883,7 +885,10 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
     }
 }
 
-// ---- drawing: the row's segments of 64 vectors (one a lane), each with its own maximum and 64-bit sums, then the one segment the target lies in
+// ---- drawing: the row's segments of 64 vectors (one a lane), each with its own maximum and 64-bit sums, then the one segment the target lies in,
+// read once more.  What bounds it: the 64-bit exponentials, 20 instructions each (4096 x 5832 bf16: 27 us, of which the vector unit issues
+// for 21; memory would take 9); with few rows two launches (16 x 104976 fp32: 6 and 6 us).  32 bits would not do: a border between two actions is off by
+// some 2^-24 there, and with ten thousand actions a random number lies that close to one every thousandth time.
 struct Segment {
     double s, t;        // sums of the exponentials, and of these times their differences to the maximum
     float m;            // its maximum (-inf: nothing open; NaN: there is one)
@@ -1013,7 +1018,7 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
 
 // rows of up to 64 segments: one wavefront each, lane i keeps the i-th segment's sums
 template <typename T>
-__global__ __launch_bounds__(BLOCK, 4) void k_sample_wave(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out) {
+__global__ __launch_bounds__(BLOCK) void k_sample_wave(Scores<T> sc, const void *uniforms, int uniform_bytes, Drawn out) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Exp64 exp64(sc.inv_t2_64);
     for (int64_t r = (int64_t)blockIdx.x * WAVES + wave; r < sc.rows; r += (int64_t)gridDim.x * WAVES) {
@@ -1036,7 +1041,7 @@ __global__ __launch_bounds__(BLOCK, 4) void k_sample_wave(Scores<T> sc, const vo
 
 // longer rows: workgroups sum a tile each, a wavefront draws
 template <typename T>
-__global__ __launch_bounds__(BLOCK, 4) void k_sample_parts(Scores<T> sc, int segments, Segment *workspace) {
+__global__ __launch_bounds__(BLOCK) void k_sample_parts(Scores<T> sc, int segments, Segment *workspace) {
     using L = Tile<T, WAVES>;
     const Exp64 exp64(sc.inv_t2_64);
     for (int64_t r = blockIdx.y; r < sc.rows; r += gridDim.y) {
@@ -1125,11 +1130,12 @@ constexpr int64_t STREAM_BYTES = 64 << 20;
 // probabilities / with five alternatives / draws, us): 600 bf16 23 / 57 / 84 against 36 / 79 / 116, 1000 bf16 30 / 72 / 105 against 38 / 81 /
 // 116; 1500 bf16 53 / 117 / 170 against 53 / 96 / 151, 1000 fp32 52 / 100 / 151 against 53 / 74 / 118.
 template <typename T> constexpr bool is_short(int64_t n) { return n * (int64_t)sizeof(T) <= 2048; }
-// The backward pass, which needs no second look, keeps rows of up to 2048 scores there, and needs nothing of the forward pass for them.
+// The backward pass, which needs no second look, keeps rows of up to 2048 scores there, and needs nothing of the forward pass for them (65536
+// x 1500: bf16 77 us, fp32 149; in tiles, from the forward pass's statistics, 198 and 217).
 constexpr int BACKWARD_SHORT_MAX = 2048;
 template <int G_, int E_, int W_> struct Shape { static constexpr int G = G_, E = E_, W = W_; };
-// f(lanes a row, scores a lane, scores a load): up to 32 scores in one lane (no exchanges at all); beyond, the fewest lanes that hold the row
-// in four 16-byte pieces each, or 64.
+// f(lanes a row, scores a lane, scores a load): up to 32 scores in one lane (no exchanges at all: 983040 x 18 fp32 20 us, over four lanes 24;
+// 61 rows 3.4, over four lanes 3.0; drawing 983040 x 18 bf16 38 us, over four lanes 49); beyond, the fewest lanes that hold the row in four 16-byte pieces each, or 64.
 template <typename T, int G, typename F> int by_pieces(int64_t n, F f) {
     constexpr int W = 16 / sizeof(T);
     const int64_t c = (n + G * W - 1) / (G * W);
@@ -1166,20 +1172,6 @@ template <typename T, bool BACKWARD, typename F> int by_length(int64_t n, F f) {
         default: return f(Shape<1, 32, 4>());
     }
 }
-// Drawing: up to 32 scores over four lanes (64-bit exponentials take twenty times what an exchange takes)
-template <typename T, typename F> int by_length_64(int64_t n, F f) {
-    if (n > 32) return by_lanes<T, false>(n, f);
-    switch ((n + 3) / 4) {
-        case 1: return f(Shape<4, 1, 1>());
-        case 2: return f(Shape<4, 2, 1>());
-        case 3: return f(Shape<4, 3, 1>());
-        case 4: return f(Shape<4, 4, 1>());
-        case 5: return f(Shape<4, 5, 1>());
-        case 6: return f(Shape<4, 6, 1>());
-        case 7: return f(Shape<4, 7, 1>());
-        default: return f(Shape<4, 8, 1>());
-    }
-}
 // How a long row is shared out: a wavefront a row (no exchange between wavefronts) where these are many or the rows not that long, else a
 // workgroup, or several where that leaves CUs without one (no more than the row has tiles).  Measured (log probabilities / with five
 // alternatives, us; wavefront against workgroup): 512 x 2500 bf16 5.1 / 7.6 against 5.1 / 7.4, 2048 x 2500 5.3 / 8.9 against 6.9 / 14.4;
@@ -1195,6 +1187,10 @@ template <typename T> Split split(int64_t rows, int64_t n) {
     const int64_t each = (tiles + wanted - 1) / wanted;
     return {WAVES, (int)((tiles + each - 1) / each), (int)each};
 }
+// The backward pass of a longer row has a tile of a wavefront's or of a workgroup's size for each wavefront or workgroup; smaller tiles leave less of the last one empty.
+// Measured (us): 32768 x 2500 bf16 93 against 132, 16384 x 5832 76 against 86, 8192 x 20000 124 against 126, 3000 x 40001 99 against 96, 1024 x
+// 104976 86 against 81.
+template <typename T> bool backward_by_waves(int64_t n) { return Tile<T, 1>::count(n) <= 12; }
 // Short rows' alternatives come one after the other, a pass over the registers each; from nine on, of rows of some length, a wavefront a row that
 // collects and ranks them is faster (7 x 1000 fp32, 20 of them: 5.6 us against 14.6 in passes).
 template <typename T> bool in_lanes(int64_t n, int top) { return is_short<T>(n) && !(n > 256 && top > 8); }
@@ -1304,7 +1300,10 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
                                       up, (T *)grad, stream_out);
                 } else return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad, stream_out);
             });
-        return launch(k_backward_long<T>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
+        if (backward_by_waves<T>(n))
+            return launch(k_backward_long<T, 1>, dim3((unsigned)Tile<T, 1>::count(n), (unsigned)std::min<int64_t>((rows + WAVES - 1) / WAVES, 65535)), BLOCK,
+                          stream, sc, given, stats, entropy, up, (T *)grad, stream_out);
+        return launch(k_backward_long<T, WAVES>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
                       stream, sc, given, stats, entropy, up, (T *)grad, stream_out);
     });
 }
@@ -1325,7 +1324,7 @@ int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, i
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (is_short<T>(n))
-            return by_length_64<T>(n, [&](auto shape) {
+            return by_length<T, false>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
                 return launch(k_sample_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, uniforms, uniform_bytes, out);
             });

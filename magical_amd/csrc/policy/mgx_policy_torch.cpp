@@ -59,7 +59,7 @@ struct Scores {
             default: TORCH_CHECK_TYPE(false, "logits: float32, float16 or bfloat16, got ", logits.scalar_type());
         }
         TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits: [..., n] with n >= 1, got ", logits.sizes());
-        TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(temperature), "temperature: positive and finite, got ", temperature);
+        TORCH_CHECK_VALUE(temperature >= 1e-37 && temperature <= 1e37, "temperature: 1e-37 ... 1e37, got ", temperature);
         n = logits.size(-1);
         x = dense_rows(logits);
         rows = x.size(0);

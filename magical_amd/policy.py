@@ -11,7 +11,7 @@
 A row holds the logits of one choice among n: 18 for one env-step, 18 ** c for a policy that answers with c env-steps at once, a
 vocabulary for one that answers in tokens.  Logits are float32, float16 or bfloat16 tensors [..., n] on the GPU, of any strides (a last
 dimension that is not dense is copied first); `mask` is a bool tensor that broadcasts to them, False = ruled out; the distribution is
-softmax(logits / temperature) over the actions that are open (not ruled out, logit above -inf).  Results are float32 whatever the
+softmax(logits / temperature), temperature in 1e-37 ... 1e37, over the actions that are open (not ruled out, logit above -inf).  Results are float32 whatever the
 logits' type.  Rows with nothing open give log probability -inf, entropy 0 and action -1 with gradient 0; rows with NaN or +inf among
 the open logits give NaN and action -1.  Calls run on torch's current stream of the logits' device; they can be captured into a HIP graph.
 """

@@ -186,7 +186,7 @@ def test_the_python_entries_refuse_bad_arguments():
     for bad in (torch.ones(17, dtype=torch.bool), torch.ones(2, 18, dtype=torch.bool), torch.ones(1, 3, 18, dtype=torch.bool)):
         with pytest.raises(ValueError):
             m.action_log_probs(x, a, mask=bad)
-    for bad in (0.0, -1.0, float('nan'), float('inf')):
+    for bad in (0.0, -1.0, float('nan'), float('inf'), 1e-38, 1e38):
         with pytest.raises(ValueError):
             m.action_log_probs(x, a, temperature=bad)
         with pytest.raises(ValueError):
@@ -360,6 +360,72 @@ def test_rows_that_nothing_or_nonsense_is_left_in(n):
     out = m.action_log_probs(leaf.detach(), torch.tensor([-1, -7, n, n + 5, -1, -1, -1, n]).cuda(), mask=mask.cuda())
     got = out.log_prob.cpu().numpy()
     assert np.all(got[[0, 1, 4, 5, 6]] == 0) and np.all(np.isnan(got[[2, 3, 7]]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [140001, 300000, 1200007])
+def test_very_long_rows(n):
+    """Rows of more segments than a workgroup keeps together (512), and of more than 64 a lane."""
+    import torch
+    import magical_amd as m
+    rng = np.random.RandomState(n)
+    x = (rng.randn(2, n) * 2).astype(np.float32)
+    x[1] = 0.5
+    u = rng.rand(2)
+    is_open, lp, h, bad = oracle(x)
+    actions = rng.randint(0, n, 2)
+    out = m.action_log_probs(torch.tensor(x).cuda(), torch.tensor(actions).cuda(), top=33)
+    _check_forward(out, x.astype(np.float64), None, actions, 1.0, 33, n)
+    want, gap = oracle_draw(is_open, lp, u)
+    assert (gap > 1e-11).all()
+    drawn = m.sample_actions(torch.tensor(x).cuda(), torch.tensor(u).cuda())
+    assert np.array_equal(drawn.action.cpu().numpy(), want)
+    assert np.all(np.abs(drawn.entropy.double().cpu().numpy() - h) <= U * h + 1e-10)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('n', [18, 500, 5000])
+def test_any_byte_but_zero_in_a_mask_is_open(n, dtype):
+    import torch
+    import magical_amd as m
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(9, n, generator=g).to(_torch_type(dtype)).cuda()
+    a = torch.randint(0, n, (9,), generator=g).cuda()
+    u = torch.rand(9, generator=g).cuda()
+    raw = (torch.randint(0, 256, (9, n), generator=g) * (torch.rand(9, n, generator=g) < 0.7)).to(torch.uint8).cuda()
+    leaf = x.clone().requires_grad_(True)
+    got = [*m.action_log_probs(leaf, a, mask=raw.view(torch.bool), top=4), *m.sample_actions(x, u, mask=raw.view(torch.bool))]
+    got.append(torch.autograd.grad(got[0].sum(), leaf)[0])
+    want = [*m.action_log_probs(leaf, a, mask=raw != 0, top=4), *m.sample_actions(x, u, mask=raw != 0)]
+    want.append(torch.autograd.grad(want[0].sum(), leaf)[0])
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('temperature', [1e-37, 1e-20, 1e20, 1e37])
+@pytest.mark.parametrize('n', [18, 600, 5000])
+def test_temperatures_at_the_ends(n, temperature):
+    """Towards 0 only the best action is left (all of them, if several are equal), towards infinity all are alike."""
+    import torch
+    import magical_amd as m
+    x = torch.randn(5, n, generator=torch.Generator().manual_seed(n))
+    x[1, 3] = x[1, 9] = 8.0
+    x[2, 4] = float('-inf')
+    best = x.argmax(1)
+    out = m.action_log_probs(x.cuda().requires_grad_(True), best.cuda(), temperature=temperature, top=2)
+    drawn = m.sample_actions(x.cuda(), torch.full((5,), 0.25).cuda(), temperature=temperature)
+    is_open, lp, h, _ = oracle(x.double().numpy(), None, temperature)
+    want = lp[np.arange(5), best.numpy()]
+    assert np.all(np.abs(out.log_prob.detach().cpu().numpy() - want) <= err_log_prob(0, n))
+    assert np.all(np.abs(out.entropy.detach().cpu().numpy() - h) <= err_entropy(n))
+    # (5000 equal probabilities have a border at exactly 0.25 = 1250 / 5000, where sums of 1250 terms, each rounded by up to 2^-53, lie on either
+    # side: within that, 1250 x 2^-53 < 1e-11, the action on either side of the border is the formula's)
+    got_a, (want_a, gap) = drawn.action.cpu().numpy(), oracle_draw(is_open, lp, np.full(5, 0.25))
+    assert np.all((got_a == want_a) | ((gap < 1e-11) & (np.abs(got_a - want_a) == 1)))
+    if temperature < 1:
+        assert np.array_equal(drawn.action.cpu().numpy(), [int(b) for b in x.argmax(1)])
 
 
 @pytest.mark.gpu
