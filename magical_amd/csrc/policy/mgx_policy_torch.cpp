@@ -9,8 +9,11 @@
 #include <ATen/ops/empty.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -20,7 +23,7 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
@@ -138,29 +141,26 @@ struct Upstream {
     }
 };
 
-struct LogProbs : torch::autograd::Function<LogProbs> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &actions, const OptTensor &mask, double temperature,
-                                 int64_t top) {
-        Forward f = ::forward(logits, actions, mask, temperature, top, true);
-        ctx->save_for_backward({logits, f.actions, mask ? *mask : Tensor(), f.stats, f.entropy});
-        ctx->saved_data["temperature"] = temperature;
-        ctx->set_materialize_grads(false);
-        if (!top) return {f.log_prob, f.entropy};
-        ctx->mark_non_differentiable({f.top_log_probs, f.top_actions});
-        return {f.log_prob, f.entropy, f.top_log_probs, f.top_actions};
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        variable_list out(5);
+// The backward pass's node.  (A custom Function keeps the same, with a dictionary and checks that cost 2 us a call.)
+struct LogProbsBackward : torch::autograd::Node {
+    SavedVariable logits, actions, mask, stats, entropy;
+    double temperature = 1;
+
+    variable_list apply(variable_list &&grads) override {
+        variable_list out(1);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        const variable_list saved = ctx->get_saved_variables();
-        const Tensor &logits = saved[0], &actions = saved[1], &stats = saved[3], &entropy = saved[4];
-        const Scores s(logits, saved[2].defined() ? OptTensor(saved[2]) : OptTensor(), ctx->saved_data["temperature"].toDouble());
-        const Upstream lp(grads[0]), h(grads[1]);
-        Tensor grad = at::empty(logits.sizes(), logits.options());
-        check(C.log_probs_backward(logits.device().index(), SCORES(s), actions.data_ptr(), (int)actions.element_size(),
-                                   stats.defined() ? stats.const_data_ptr<float>() : nullptr, entropy.const_data_ptr<float>(), lp.ptr,
-                                   lp.stride, h.ptr, h.stride, grad.data_ptr(), stream_of(logits)));
-        if (at::GradMode::is_enabled()) {      // create_graph: the gradient has none of its own, and says so when it is asked for
+        std::lock_guard<std::mutex> lock(mutex_);
+        const Tensor x = logits.unpack(), a = actions.unpack(), m = mask.unpack(), st = stats.unpack(), h = entropy.unpack(shared_from_this());
+        const bool differentiated = at::GradMode::is_enabled();
+        at::NoGradGuard no_grad;
+        const Scores s(x, m.defined() ? OptTensor(m) : OptTensor(), temperature);
+        const Upstream g_lp(grads[0]), g_h(grads[1]);
+        Tensor grad = at::empty(x.sizes(), x.options());
+        check(C.log_probs_backward(x.device().index(), SCORES(s), a.data_ptr(), (int)a.element_size(),
+                                   st.defined() ? st.const_data_ptr<float>() : nullptr, h.const_data_ptr<float>(), g_lp.ptr, g_lp.stride, g_h.ptr,
+                                   g_h.stride, grad.data_ptr(), stream_of(x)));
+        if (differentiated) {      // create_graph: the gradient has none of its own, and says so when it is asked for
+            at::AutoGradMode with_grad(true);
             Tensor fake = grad.detach();
             fake.set_requires_grad(true);
             auto refuse = std::make_shared<torch::autograd::DelayedError>("action_log_probs is differentiable once", 1);
@@ -169,16 +169,37 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
         out[0] = grad;
         return out;
     }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&logits, &actions, &mask, &stats, &entropy}) v->reset_data();
+    }
+    std::string name() const override { return "ActionLogProbsBackward"; }
 };
+
+Forward forward_with_graph(const Tensor &logits, const Tensor &actions, const OptTensor &mask, double temperature, int64_t top) {
+    Forward f;
+    {
+        at::NoGradGuard no_grad;
+        f = forward(logits, actions, mask, temperature, top, true);
+    }
+    std::shared_ptr<LogProbsBackward> node(new LogProbsBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->temperature = temperature;
+    node->logits = SavedVariable(logits, false);
+    node->actions = SavedVariable(f.actions, false);
+    if (mask) node->mask = SavedVariable(*mask, false);
+    if (f.stats.defined()) node->stats = SavedVariable(f.stats, false);
+    torch::autograd::set_history(f.log_prob, node);
+    torch::autograd::set_history(f.entropy, node);
+    node->entropy = SavedVariable(f.entropy, true);
+    return f;
+}
 
 py::object or_none(const Tensor &t) { return t.defined() ? py::cast(t) : py::none(); }
 
 py::tuple log_probs(const Tensor &logits, const Tensor &actions, const OptTensor &mask, double temperature, int64_t top) {
-    if (at::GradMode::is_enabled() && logits.requires_grad()) {
-        const variable_list v = LogProbs::apply(logits, actions, mask, temperature, top);
-        return py::make_tuple(v[0], v[1], top ? py::cast(v[2]) : py::none(), top ? py::cast(v[3]) : py::none());
-    }
-    const Forward f = forward(logits, actions, mask, temperature, top, false);
+    const Forward f = at::GradMode::is_enabled() && logits.requires_grad() ? forward_with_graph(logits, actions, mask, temperature, top)
+                                                                           : forward(logits, actions, mask, temperature, top, false);
     return py::make_tuple(f.log_prob, f.entropy, or_none(f.top_log_probs), or_none(f.top_actions));
 }
 

@@ -718,6 +718,30 @@ def test_refusals_on_the_gpu():
     g, = torch.autograd.grad(m.action_log_probs(leaf, a).entropy.sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match='differentiable once'):
         g.sum().backward()
+    # a graph is there for one backward pass unless it is kept, and holds no memory afterwards
+    out = m.action_log_probs(leaf, a)
+    first, = torch.autograd.grad(out.log_prob.sum(), leaf, retain_graph=True)
+    assert torch.equal(first, torch.autograd.grad(out.log_prob.sum(), leaf)[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out.entropy.sum(), leaf)
+    del out, first
+    big = torch.randn(64, 100000, device='cuda').requires_grad_(True)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    for _ in range(3):
+        out = m.action_log_probs(big, torch.zeros(64, dtype=torch.int64, device='cuda'), top=3)
+        (out.log_prob.sum() + out.entropy.sum()).backward()
+        big.grad = None
+        unused = m.action_log_probs(big, torch.zeros(64, dtype=torch.int64, device='cuda'))
+    del out, unused
+    assert torch.cuda.memory_allocated() == held
+    # one of the two upstream gradients, or neither
+    out = m.action_log_probs(leaf, a)
+    g_lp, = torch.autograd.grad(out.log_prob.sum(), leaf, retain_graph=True)
+    g_h, = torch.autograd.grad(out.entropy.sum(), leaf, retain_graph=True)
+    both, = torch.autograd.grad(out.log_prob.sum() + out.entropy.sum(), leaf)
+    assert torch.allclose(g_lp + g_h, both, rtol=0, atol=2.0 ** -20)
+    assert torch.autograd.grad((leaf * 0).sum() + m.action_log_probs(leaf, a, top=1).top_log_probs.sum(), leaf)[0].abs().max() == 0
     # inputs changed in between are noticed
     y = (leaf * 1.0)
     out = m.action_log_probs(y, a)
