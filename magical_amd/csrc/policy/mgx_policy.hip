@@ -326,11 +326,29 @@ struct Given {          // a row's action and its score
         : a(actions.at(r)), x(a >= 0 && a < n ? row.at(a) : NEG_INF) {}
 };
 
+// A wavefront's run of `bytes` bytes from LDS (at a multiple of 16) to memory, in 16-byte vectors and a rest of `unit` bytes each, by its first `lanes` lanes.
+template <int UNIT> __device__ __forceinline__ void store_run(void *out, const unsigned char *run, int bytes, int lane, int lanes, bool stream) {
+    unsigned char *const to = (unsigned char *)out;
+    for (int at = lane * 16; at + 16 <= bytes; at += lanes * 16) {
+        uint32_t v[4];
+        __builtin_memcpy(v, __builtin_assume_aligned(run + at, 16), 16);
+        store_bytes((uint32_t *)(to + at), v, stream);
+    }
+    for (int at = (bytes & ~15) + lane * UNIT; at < bytes; at += lanes * UNIT) __builtin_memcpy(to + at, run + at, UNIT);
+}
+
+// Rows in one lane put their alternatives together in LDS, as k_backward_lane does with the gradients (288296 x 18 fp16, a lane storing its own: 5
+// alternatives 12.4 us, 8 19.6, 18 56; by way of LDS 12.2, 15.9, 27).
 template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy,
                                                            float *top_log_probs, int32_t *top_actions) {
     using S = Spread<G, E, W>;
+    extern __shared__ __align__(16) unsigned char lds_bytes[];          // (staged: [wavefronts][2][64][top])
     const int g = threadIdx.x % G, n = (int)sc.n;
+    constexpr bool staged = G == 1;
+    const int lane = threadIdx.x & 63;
+    float *const run_log_probs = (float *)lds_bytes + (threadIdx.x >> 6) * 128 * top;
+    int32_t *const run_actions = (int32_t *)(run_log_probs + 64 * top);
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
         const Given given(actions, row, r, n);
@@ -382,10 +400,26 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
                 for (int e = 0; e < E; e++) x[e] = S::place(g, e) == i ? NEG_INF : x[e];
             if (g == 0) {
                 const bool there = v > NEG_INF && !undefined;
-                top_actions[r * top + k] = there ? i : -1;
-                top_log_probs[r * top + k] = there ? (v - ref) * sc.inv_t - log_s : NEG_INF;
+                const int action = there ? i : -1;
+                const float lp = there ? (v - ref) * sc.inv_t - log_s : NEG_INF;
+                if constexpr (staged) {
+                    run_actions[lane * top + k] = action;
+                    run_log_probs[lane * top + k] = lp;
+                } else {
+                    top_actions[r * top + k] = action;
+                    top_log_probs[r * top + k] = lp;
+                }
             }
         }
+        if constexpr (staged)
+            if (top) {          // (the lanes with a row are the wavefront's first)
+                wave_sync();
+                const int64_t r0 = r - lane;
+                const int lanes = (int)(sc.rows - r0 < 64 ? sc.rows - r0 : 64), bytes = lanes * top * 4;
+                store_run<4>(top_actions + r0 * top, (const unsigned char *)run_actions, bytes, lane, lanes, false);
+                store_run<4>(top_log_probs + r0 * top, (const unsigned char *)run_log_probs, bytes, lane, lanes, false);
+                wave_sync();
+            }
     }
 }
 
@@ -476,14 +510,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions a
         }
         wave_sync();
         const int bytes = (int)(sc.rows - r0 < 64 ? sc.rows - r0 : 64) * n * (int)sizeof(T);
-        unsigned char *const to = (unsigned char *)(grad + r0 * n);
-        for (int at = lane * 16; at + 16 <= bytes; at += 1024) {
-            uint32_t v[4];
-            __builtin_memcpy(v, __builtin_assume_aligned(run + at, 16), 16);
-            store_bytes((uint32_t *)(to + at), v, stream);
-        }
-        const int at = (bytes & ~15) + lane * (int)sizeof(T);
-        if (at < bytes) __builtin_memcpy(to + at, run + at, sizeof(T));
+        store_run<(int)sizeof(T)>(grad + r0 * n, run, bytes, lane, 64, stream);
         wave_sync();
     }
 }
@@ -531,7 +558,7 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const double upto = group_scan<G>(s, g), total = __shfl(upto, G - 1, G);
         t = group_sum<G>(t);
         const int group = (threadIdx.x & 63) - g;
-        const uint64_t in_group = ((1ull << G) - 1) << group;
+        const uint64_t in_group = G == 64 ? ~0ull : ((1ull << (G & 63)) - 1) << group;
         const bool undefined = m != m || m == -NEG_INF, none = undefined || !some;
         const double target = u * total;
         // the first lane that passes the target, or else (rounding; a number of 1) the last one with anything in it
@@ -1135,32 +1162,31 @@ template <typename T> constexpr bool is_short(int64_t n) { return n * (int64_t)s
 constexpr int BACKWARD_SHORT_MAX = 2048;
 template <int G_, int E_, int W_> struct Shape { static constexpr int G = G_, E = E_, W = W_; };
 // f(lanes a row, scores a lane, scores a load): up to 32 scores in one lane (no exchanges at all: 983040 x 18 fp32 20 us, over four lanes 24;
-// 61 rows 3.4, over four lanes 3.0; drawing 983040 x 18 bf16 38 us, over four lanes 49); beyond, the fewest lanes that hold the row in four 16-byte pieces each, or 64.
-template <typename T, int G, typename F> int by_pieces(int64_t n, F f) {
-    constexpr int W = 16 / sizeof(T);
+// 61 rows 3.4, over four lanes 3.0; drawing 983040 x 18 bf16 38 us, over four lanes 49); beyond, the fewest lanes that hold the row in four
+// pieces of W scores each, or 64 lanes with up to MOST pieces.
+template <int W, int G, int MOST, typename F> int by_pieces(int64_t n, F f) {
     const int64_t c = (n + G * W - 1) / (G * W);
     if constexpr (G == 4) if (c <= 2) return f(Shape<G, 2 * W, W>());
     if (c <= 3) return f(Shape<G, 3 * W, W>());
-    if constexpr (G < 64 || sizeof(T) == 2) return f(Shape<G, 4 * W, W>());
+    if constexpr (G < 64 || MOST == 4) return f(Shape<G, 4 * W, W>());
     else {
         if (c <= 4) return f(Shape<G, 4 * W, W>());
         if (c <= 6) return f(Shape<G, 6 * W, W>());
         return f(Shape<G, 8 * W, W>());
     }
 }
-template <typename T, bool BACKWARD, typename F> int by_lanes(int64_t n, F f) {
-    const int64_t lanes = (n + 64 / sizeof(T) - 1) / (64 / sizeof(T));
-    if (lanes <= 4) return by_pieces<T, 4>(n, f);
-    if (lanes <= 8) return by_pieces<T, 8>(n, f);
-    if (lanes <= 16) return by_pieces<T, 16>(n, f);
-    if constexpr (!BACKWARD) return by_pieces<T, 32>(n, f);
+template <int W, int LONGEST, typename F> int by_lanes(int64_t n, F f) {
+    const int64_t lanes = (n + 4 * W - 1) / (4 * W);
+    if (lanes <= 4) return by_pieces<W, 4, 4>(n, f);
+    if (lanes <= 8) return by_pieces<W, 8, 4>(n, f);
+    if (lanes <= 16) return by_pieces<W, 16, 4>(n, f);
+    if constexpr (LONGEST <= 32 * 4 * W) return by_pieces<W, 32, 4>(n, f);
     else {
-        if (lanes <= 32) return by_pieces<T, 32>(n, f);
-        return by_pieces<T, 64>(n, f);
+        if (lanes <= 32) return by_pieces<W, 32, 4>(n, f);
+        return by_pieces<W, 64, LONGEST / (64 * W)>(n, f);
     }
 }
-template <typename T, bool BACKWARD, typename F> int by_length(int64_t n, F f) {
-    if (n > 32) return by_lanes<T, BACKWARD>(n, f);
+template <typename F> int by_length_32(int64_t n, F f) {
     switch ((n + 3) / 4) {
         case 1: return f(Shape<1, 4, 4>());
         case 2: return f(Shape<1, 8, 4>());
@@ -1172,10 +1198,16 @@ template <typename T, bool BACKWARD, typename F> int by_length(int64_t n, F f) {
         default: return f(Shape<1, 32, 4>());
     }
 }
+template <typename T, int LONGEST, typename F> int by_length(int64_t n, F f) {
+    return n <= 32 ? by_length_32(n, f) : by_lanes<16 / sizeof(T), LONGEST>(n, f);
+}
 // Drawing for up to 16384 rows, which do not fill the GPU: short rows over four lanes.  (64-bit exponentials one after the other: 4096 x 18 fp32 4.4 us, in
 // one lane 5.2; 65536 x 18 7.2, in one lane 5.6.)
+// Beyond 32 scores, 16 a lane at most, whatever their type: more leave too few registers for two wavefronts' exponentials to overlap (51738 x 616 fp16, 20
+// a lane 72 us, 10 a lane 65; 46394 x 242, 16 a lane 23.3, 8 a lane 21.7).
 template <typename T, typename F> int by_length_to_draw(int64_t rows, int64_t n, F f) {
-    if (rows > 16384 || n < 8 || n > 32) return by_length<T, false>(n, f);
+    if (n > 32) return by_lanes<4, 2048 / sizeof(T)>(n, f);
+    if (rows > 16384 || n < 8) return by_length_32(n, f);
     return n <= 16 ? f(Shape<4, 4, 4>()) : f(Shape<4, 8, 4>());
 }
 // How a long row is shared out: a wavefront a row (no exchange between wavefronts) where these are many or the rows not that long, else a
@@ -1209,7 +1241,7 @@ template <typename T> bool sample_by_waves(int64_t rows, int64_t n) {
     return tiles <= 2 || (tiles <= 4 && rows >= 512) || (tiles <= 12 && rows >= 2048);          // (at most 48 segments: a lane each)
 }
 
-int64_t short_blocks(int64_t rows, int G) { return (rows * G + BLOCK - 1) / BLOCK; }
+dim3 short_blocks(int64_t rows, int G) { return dim3((unsigned)std::min<int64_t>((rows * G + BLOCK - 1) / BLOCK, 0xffffffffLL / BLOCK)); }
 
 // f(a value of the scores' element type)
 template <typename F> int by_dtype(int dtype, F f) {
@@ -1258,10 +1290,10 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (in_lanes<T>(n, top))
-            return by_length<T, false>(n, [&](auto shape) {
+            return by_length<T, 2048 / sizeof(T)>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
-                return launch(k_log_probs_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, top,
-                              log_prob, entropy, top_log_probs, top_actions);
+                return launch_lds(k_log_probs_short<T, G, E, W>, short_blocks(rows, G), BLOCK, G == 1 ? BLOCK * top * 8 : 0, stream, sc,
+                                  given, top, log_prob, entropy, top_log_probs, top_actions);
             });
         const Split sp = split<T>(rows, n);
         const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_actions, top};
@@ -1298,13 +1330,12 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
         using T = decltype(v);
         const Scores<T> sc = scores<T>(logits, rows, n, row_stride, mask, mask_row_stride, temperature);
         if (n <= BACKWARD_SHORT_MAX)
-            return by_length<T, true>(n, [&](auto shape) {
+            return by_length<T, BACKWARD_SHORT_MAX>(n, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, E = decltype(shape)::E, W = decltype(shape)::W;
-                if constexpr (G == 1) {
-                    const int64_t blocks = std::min<int64_t>((rows + BLOCK - 1) / BLOCK, 0xffffffffLL / BLOCK);
-                    return launch_lds(k_backward_lane<T, G, E, W>, dim3((unsigned)blocks), BLOCK, (int)(BLOCK * n * sizeof(T)), stream, sc, given, entropy,
+                if constexpr (G == 1)
+                    return launch_lds(k_backward_lane<T, G, E, W>, short_blocks(rows, 1), BLOCK, (int)(BLOCK * n * sizeof(T)), stream, sc, given, entropy,
                                       up, (T *)grad, stream_out);
-                } else return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad, stream_out);
+                else return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad, stream_out);
             });
         if (backward_by_waves<T>(n))
             return launch(k_backward_long<T, 1>, dim3((unsigned)Tile<T, 1>::count(n), (unsigned)std::min<int64_t>((rows + WAVES - 1) / WAVES, 65535)), BLOCK,

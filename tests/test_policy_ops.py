@@ -569,6 +569,33 @@ def test_every_row_alike_in_every_launch_shape(n, rows, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows', [1, 2, 63, 64, 65, 190, 257])
+def test_alternatives_of_a_few_rows_more_or_less_than_a_wavefront_holds(rows):
+    import torch
+    import magical_amd as m
+    for n, dtype in ((2, 'f32'), (7, 'bf16'), (18, 'f16'), (32, 'f32')):
+        x, mask, actions, _ = _case(n, dtype, rows * n, rows=rows, masked='rows')
+        for top in sorted({1, 2, 3, n}):
+            if top <= n:
+                out = m.action_log_probs(x.cuda(), torch.tensor(actions).cuda(), mask=torch.tensor(mask).cuda(), top=top)
+                _check_forward(out, x.double().numpy(), mask, actions, 1.0, top, (rows, n, top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [70, 190, 385, 511, 513, 616, 768, 769, 1023])
+def test_draws_of_rows_in_a_few_lanes(n):
+    import torch
+    import magical_amd as m
+    for dtype in DTYPES:
+        x, mask, _, rng = _case(n, dtype, n, rows=37, masked='rows')
+        u = rng.rand(37)
+        want_a, gap = oracle_draw(*oracle(x.double().numpy(), mask, 0.8)[:2], u)
+        assert (gap > 1e-11).all()
+        got = m.sample_actions(x.cuda(), torch.tensor(u).cuda(), mask=torch.tensor(mask).cuda(), temperature=0.8)
+        assert np.array_equal(got.action.cpu().numpy(), want_a), dtype
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """Rows that lie further than 2^32 bytes and 2^31 elements from the first one."""
     import torch
