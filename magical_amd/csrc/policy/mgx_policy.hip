@@ -272,6 +272,7 @@ __device__ __forceinline__ double fma_64(double a, double b, double c) {
 // For drawing: scores as differences to a maximum, in 64 bits, and 2^(d * inv_t2) of them.  A difference below 2^-1000's counts as that, -inf
 // and NaN too (the callers look for NaN themselves), and what is below NOTHING as no probability at all.
 constexpr double NOTHING = 0x1p-990;
+__device__ __forceinline__ double or_nothing(double p) { return p > NOTHING ? p : 0.0; }
 struct Exp64 {
     double inv_t2, least;
     __device__ __forceinline__ explicit Exp64(double inv_t2_) : inv_t2(inv_t2_), least(-1000.0 / inv_t2_) {}
@@ -342,6 +343,7 @@ template <int UNIT> __device__ __forceinline__ void store_run(void *out, const u
 template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy,
                                                            float *top_log_probs, int32_t *top_actions) {
+    static_assert(G <= 32, "the best of a group: exchanges over 32 lanes");
     using S = Spread<G, E, W>;
     extern __shared__ __align__(16) unsigned char lds_bytes[];          // (staged: [wavefronts][2][64][top])
     const int g = threadIdx.x % G, n = (int)sc.n;
@@ -529,6 +531,22 @@ struct Drawn {
     }
 };
 
+// The place, among the E of the lane that a draw falls into, that passes the target (else the last one with anything in it), and its score.
+template <int E> __device__ __forceinline__ int in_lane(const float (&x)[E], const double (&p)[E], double c, double target, float &xa) {
+    int a = -1;
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        c += p[e];
+        if (p[e] > NOTHING && !found) { a = e; xa = x[e]; found = c > target; }
+    }
+    if (a < 0)          // (each below NOTHING, their sum above it: the first one that is open)
+#pragma unroll
+        for (int e = E - 1; e >= 0; e--)
+            if (x[e] > NEG_INF) { a = e; xa = x[e]; }
+    return a;
+}
+
 // Lane g holds the E consecutive scores from g * E on: a running sum in index order is a lane's sum, a scan over the lanes, and a second
 // look at the one lane in which the target lies.
 template <typename T, int G, int E, int W>
@@ -565,15 +583,9 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
         const uint64_t past = __ballot(s > NOTHING && upto > target) & in_group, any = __ballot(s > NOTHING) & in_group;
         const int owner = none ? group : past ? first_lane(past) : last_lane(any);
         if ((threadIdx.x & 63) == owner) {
-            double c = g == 0 ? 0.0 : upto - s;
-            int a = -1;
+            const double c = g == 0 ? 0.0 : upto - s;
             float xa = 0;
-            bool found = false;
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                c += p[e];
-                if (p[e] > NOTHING && !found) { a = g * E + e; xa = x[e]; found = c > target; }
-            }
+            const int a = g * E + in_lane(x, p, c, target, xa);
             const double log_s = log(total);
             const float nil = undefined ? __builtin_nanf("") : NEG_INF;
             out.put(r, none ? -1 : a, none ? nil : (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s),
@@ -977,7 +989,7 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
 #pragma unroll
         for (int i = 0; i < STEP; i++) {
             const double d = exp64.below(g[i].m, ref), w = exp64(d);
-            s = fma(w, g[i].s, s);
+            s += or_nothing(w * g[i].s);          // (a run of segments in which nothing is open is to have a sum of 0)
             t = fma(w, fma(d, g[i].s, g[i].t), t);
         }
     }
@@ -986,16 +998,16 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
     t = group_sum<64>(t);
     const double target = u * total;
     // the first run that passes the target, or else (rounding; a number of 1) the last one with anything in it; then the segment in it
-    uint64_t past = __ballot(s > NOTHING && upto > target), any = __ballot(s > NOTHING);
+    uint64_t past = __ballot(s > 0 && upto > target), any = __ballot(s > 0);
     const int run = past ? first_lane(past) : last_lane(any);
     double before = lane_of(lane == 0 ? 0.0 : upto - s, run), found_before = before;
     int found = run * each;
     if (each > 1)
         for (int k0 = 0; k0 < each; k0 += 64) {
             const Segment g = k0 + lane < each ? again(run, k0 + lane) : Segment{0, 0, NEG_INF};
-            const double w = exp64(exp64.below(g.m, ref)) * g.s, sum = group_scan<64>(w, lane);
-            past = __ballot(w > NOTHING && before + sum > target);
-            any = __ballot(w > NOTHING);
+            const double w = or_nothing(exp64(exp64.below(g.m, ref)) * g.s), sum = group_scan<64>(w, lane);
+            past = __ballot(w > 0 && before + sum > target);
+            any = __ballot(w > 0);
             if (any) {
                 const int k = past ? first_lane(past) : last_lane(any);
                 found = run * each + k0 + k;
@@ -1020,8 +1032,7 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
     upto = group_scan<64>(s, lane);
     past = __ballot(s > NOTHING && found_before + upto > target);
     any = __ballot(s > NOTHING);
-    const bool tiny = !any;          // (the segment's sum is above NOTHING and none of its terms: the first one that is open)
-    if (tiny) {
+    if (!any) {          // (the segment's sum is above NOTHING and none of its lanes': the first one with something open)
         bool open = false;
 #pragma unroll
         for (int k = 0; k < V; k++) open |= x[k] > NEG_INF;
@@ -1029,17 +1040,10 @@ __device__ __forceinline__ void draw(const Scores<T> &sc, const Row<T> &row, con
     }
     const int owner = past ? first_lane(past) : last_lane(any);
     if (lane == owner) {
-        double c = found_before + (lane == 0 ? 0.0 : upto - s);
-        int a = -1;
         float xa = 0;
-        bool done = false;
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            c += p[k];
-            if ((tiny ? x[k] > NEG_INF : p[k] > NOTHING) && !done) { a = (int)j + k; xa = x[k]; done = tiny || c > target; }
-        }
+        const int k = in_lane(x, p, found_before + (lane == 0 ? 0.0 : upto - s), target, xa);
         const double log_s = log(total);
-        out.put(r, a, (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s), (float)(log_s - t / total * sc.inv_t2_64 * LN_2));
+        out.put(r, (int)j + k, (float)(((double)xa - ref) * sc.inv_t2_64 * LN_2 - log_s), (float)(log_s - t / total * sc.inv_t2_64 * LN_2));
     }
 }
 

@@ -46,6 +46,9 @@ void check(int rc) {
     if (rc < 0) throw MgxError("mgx error " + std::to_string(rc) + ": " + C.last_error());
 }
 
+// what lies in memory behind a tensor is its values (no negation put off, no zeros without memory)
+Tensor plain(const Tensor &t) { return t._is_zerotensor() ? t.clone() : t.is_neg() ? t.resolve_neg() : t; }
+
 // rows x n scores as the C calls take them, and the tensors behind the pointers
 struct Scores {
     int dtype;
@@ -77,7 +80,7 @@ struct Scores {
     }
     // [rows][n] with neighbouring columns: a view where there is one
     Tensor dense_rows(const Tensor &t) const {
-        Tensor v = t.dim() == 2 ? t : t.reshape({t.numel() / n, n});
+        const Tensor p = plain(t), v = p.dim() == 2 ? p : p.reshape({p.numel() / n, n});
         return n > 1 && v.stride(1) != 1 ? v.contiguous() : v;
     }
 };
@@ -109,7 +112,7 @@ Forward forward(const Tensor &logits, const Tensor &actions, const OptTensor &ma
     void *stream = stream_of(logits);
     const at::TensorOptions f32 = logits.options().dtype(at::kFloat);
     Forward f;
-    f.actions = actions.contiguous();
+    f.actions = plain(actions).contiguous();
     f.log_prob = at::empty(lead, f32);
     f.entropy = at::empty(lead, f32);
     if (for_backward)
@@ -135,7 +138,8 @@ struct Upstream {
     int64_t stride = 0;
     explicit Upstream(const Tensor &t) {
         if (!t.defined()) return;
-        g = t.dim() == 1 ? t : t.reshape({-1});
+        g = plain(t);
+        if (g.dim() != 1) g = g.reshape({-1});
         ptr = g.const_data_ptr<float>();
         stride = g.stride(0);
     }
@@ -212,7 +216,7 @@ py::tuple sample(const Tensor &logits, const Tensor &uniforms, const OptTensor &
     TORCH_CHECK_VALUE(uniforms.sizes() == lead, "uniforms: one for each row of logits, ", lead, ", got ", uniforms.sizes());
     void *stream = stream_of(logits);
     const at::TensorOptions f32 = logits.options().dtype(at::kFloat);
-    const Tensor u = uniforms.contiguous(), action = at::empty(lead, f32.dtype(at::kInt)), log_prob = at::empty(lead, f32),
+    const Tensor u = plain(uniforms).contiguous(), action = at::empty(lead, f32.dtype(at::kInt)), log_prob = at::empty(lead, f32),
                  entropy = at::empty(lead, f32), ws = workspace(MGX_POLICY_SAMPLE, s, 0, logits);
     check(C.sample(logits.device().index(), SCORES(s), u.data_ptr(), (int)u.element_size(), action.data_ptr<int32_t>(),
                    log_prob.data_ptr<float>(), entropy.data_ptr<float>(), ws.defined() ? ws.data_ptr() : nullptr,

@@ -596,6 +596,49 @@ def test_draws_of_rows_in_a_few_lanes(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows', [16, 4096])
+@pytest.mark.parametrize('n', [18, 900, 2500, 5832, 20000, 104976])
+def test_draws_next_to_long_closed_stretches(n, rows):
+    """The first and the last that is open, with everything before and behind it ruled out: numbers of 0 and 1 have to reach them."""
+    import torch
+    import magical_amd as m
+    if rows * n > 1 << 27:
+        rows = 1100
+    x = torch.zeros(rows, n, dtype=torch.bfloat16, device='cuda')
+    u = (torch.arange(rows, device='cuda') % 2).float()
+    for first in sorted({0, 1, n // 9, min(2048, n // 2), n // 2}):
+        mask = torch.zeros(n, dtype=torch.bool, device='cuda')
+        last = n - 1 - first // 2
+        mask[first:last + 1] = True
+        old = torch.full((rows,), -7, dtype=torch.int32, device='cuda')          # (what the result's memory holds before, most likely)
+        del old
+        got = m.sample_actions(x, u, mask=mask)
+        assert torch.equal(got.action, torch.where(u == 0, first, last).int()), (first, last)
+        want = -np.log(last + 1 - first)
+        assert (got.log_prob.double() - want).abs().max() <= U * abs(want) + 1e-12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [18, 200, 900, 5832, 104976])
+def test_draws_among_probabilities_that_are_next_to_nothing(n):
+    """Each below 2^-990, their sum above it: still an action that is open."""
+    import torch
+    import magical_amd as m
+    for rows in (3, 4096):
+        for bits in (985, 991, 994, 998, 1200):
+            x = torch.full((1, n), -bits * float(np.log(2)), device='cuda')
+            x[0, n // 3 * 2:] = 0
+            x[0, :n // 9] = -float('inf')
+            x = x.expand(rows, n)
+            got = m.sample_actions(x, torch.zeros(rows, device='cuda'))
+            assert (got.action >= n // 9).all() and (got.action <= n // 3 * 2).all(), (rows, bits)
+            if bits < 990:
+                assert (got.action == n // 9).all()
+            if bits > 1100:
+                assert (got.action == n // 3 * 2).all()
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """Rows that lie further than 2^32 bytes and 2^31 elements from the first one."""
     import torch
@@ -727,6 +770,18 @@ def test_calls_on_other_streams_and_interleaved():
     for k, (p, q) in enumerate(got):
         for t, w in zip(list(p) + list(q), list(want[k % 4][0]) + list(want[k % 4][1])):
             assert torch.equal(t, w)
+
+
+@pytest.mark.gpu
+def test_negations_that_torch_has_put_off_are_taken():
+    import torch
+    import magical_amd as m
+    z = torch.complex(torch.zeros(9, 18), torch.randn(9, 18)).cuda()
+    x, a, u = z.conj().imag, torch.arange(9, device='cuda'), torch.rand(9, device='cuda')
+    assert x.is_neg()
+    for got, want in zip(m.action_log_probs(x, a, top=3) + m.sample_actions(x, u),
+                         m.action_log_probs(x.resolve_neg().clone(), a, top=3) + m.sample_actions(x.resolve_neg().clone(), u)):
+        assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
