@@ -302,9 +302,10 @@ constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
 // A row stays in the registers of G lanes (1 ... 64), E scores a lane: one read of the scores, all sums by lane exchanges, no barrier.  What
-// bounds it: memory (983040 x 18 fp32: 17 us, 5.1 TB/s; backward 28 us, 5.6 TB/s), from some dozen scores a row on also the vector unit,
-// which issues ten to twelve instructions a score, the exponential counted as four (61440 x 324 bf16 with a mask: 14 us where memory would take
-// 8; backward 24 where it would take 16).  Lane g holds pieces of W neighbouring scores (16 bytes, or 4 scores): x[e] is score place(g, e).
+// bounds it: memory (983040 x 18 fp32: 17.5 us where its 83 MB take 16 at a copy's rate; backward 28, 16 of them the reads and 14 the writes), from some
+// dozen scores a row on the vector unit, which issues some 15 instructions a score, 20 with a mask (61440 x 324 bf16 with a mask: 16 us, 12 of
+// them issued, where memory would take 8; backward 25, 16 issued, 16 of memory).  Lane g holds pieces of W neighbouring scores (16 bytes, or 4
+// scores): x[e] is score place(g, e).
 template <int G, int E, int W> struct Spread {
     static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
     template <typename T> static __device__ __forceinline__ void load_row(const Row<T> &row, int g, int n, float (&x)[E]) {
@@ -597,8 +598,8 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 // ----------------------------------------------------------------------------------------------------------------- long rows
 // A wavefront or workgroup goes over a row, or over one part of it where there are few rows, in tiles of U 16-byte vectors a lane: running
 // maximum, sum and weighted sum per lane, joined at the end; every score is read once.  What bounds it: memory (1024 x 104976 bf16: 44 us,
-// 4.9 TB/s; backward 72 us, 6.0 TB/s), with masks and alternatives the vector unit too (4096 x 5832 bf16, a mask, five alternatives: 21 us
-// where memory would take 14), and with few rows two launches (7 x 50021 fp32, 20 alternatives: 8 and 5 us).  Loading the next tile ahead of
+// 4.9 TB/s; backward 72 us, 6.0 TB/s), with masks and alternatives the vector unit too (4096 x 5832 bf16, a mask, five alternatives: 23 us,
+// 14 of them issued, where memory would take 14), and with few rows two launches (7 x 50021 fp32, 20 alternatives: 8 and 5 us).  Loading the next tile ahead of
 // the present one's arithmetic made it slower (58 -> 64 and 22 -> 28 us): registers, and other wavefronts hide the loads already.
 
 // ROW_WAVES: wavefronts that go over the tile together (1, or the workgroup's 4)
@@ -925,7 +926,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
 }
 
 // ---- drawing: the row's segments of 64 vectors (one a lane), each with its own maximum and 64-bit sums, then the one segment the target lies in,
-// read once more.  What bounds it: the 64-bit exponentials, 20 instructions each (4096 x 5832 bf16: 27 us, of which the vector unit issues
+// read once more.  What bounds it: the 64-bit exponentials, 20 instructions each (4096 x 5832 bf16: 28 us, of which the vector unit issues
 // for 21; memory would take 9); with few rows two launches (16 x 104976 fp32: 6 and 6 us).  32 bits would not do: a border between two actions is off by
 // some 2^-24 there, and with ten thousand actions a random number lies that close to one every thousandth time.
 struct Segment {

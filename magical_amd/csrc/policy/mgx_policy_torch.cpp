@@ -7,6 +7,7 @@
 #include <ATen/ExpandUtils.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -180,8 +181,22 @@ struct LogProbsBackward : torch::autograd::Node {
     std::string name() const override { return "ActionLogProbsBackward"; }
 };
 
+// A leaf's gradient arrives on the stream on which an earlier call first asked for it, as long as results of such calls are alive.  A captured
+// backward pass would have to wait for that stream, and the default stream cannot take part in a capture: torch ends the process.
+void refuse_capture_beside_eager_graph(const Tensor &logits) {
+    if (!logits.is_leaf()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(logits);
+    if (!accumulator || !logits.is_cuda()) return;
+    const auto earlier = accumulator->stream();
+    if (!earlier || *earlier != c10::hip::getDefaultHIPStream(logits.device().index()).unwrap()) return;
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+        throw MgxError("logits that need a gradient still belong to results of earlier calls on the default stream: free these results before this "
+                       "call is captured, or give logits.detach()");
+}
+
 Forward forward_with_graph(const Tensor &logits, const Tensor &actions, const OptTensor &mask, double temperature, int64_t top) {
     Forward f;
+    refuse_capture_beside_eager_graph(logits);
     {
         at::NoGradGuard no_grad;
         f = forward(logits, actions, mask, temperature, top, true);

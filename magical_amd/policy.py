@@ -11,9 +11,14 @@
 A row holds the logits of one choice among n: 18 for one env-step, 18 ** c for a policy that answers with c env-steps at once, a
 vocabulary for one that answers in tokens.  Logits are float32, float16 or bfloat16 tensors [..., n] on the GPU, of any strides (a last
 dimension that is not dense is copied first); `mask` is a bool tensor that broadcasts to them, False = ruled out; the distribution is
-softmax(logits / temperature), temperature in 1e-37 ... 1e37, over the actions that are open (not ruled out, logit above -inf).  Results are float32 whatever the
-logits' type.  Rows with nothing open give log probability -inf, entropy 0 and action -1 with gradient 0; rows with NaN or +inf among
-the open logits give NaN and action -1.  Calls run on torch's current stream of the logits' device; they can be captured into a HIP graph.
+softmax(logits / temperature), temperature in 1e-37 ... 1e37, over the actions that are open (not ruled out, logit above -inf).  Results are
+float32 whatever the logits' type.  Rows with nothing open give log probability -inf, entropy 0 and action -1 with gradient 0; rows with NaN
+or +inf among the open logits give NaN and action -1.  Calls run on torch's current stream of the logits' device.
+
+Calls, and the backward pass, can be captured into a HIP graph and replayed.  While a backward pass is captured, no results of earlier calls
+on the same leaves (a logits tensor, a network's weights) and the default stream may be alive: torch would make that stream part of the
+capture, which it cannot be, and end the process.  Where the logits are such a leaf themselves the call is refused (MgxError); a network's
+weights are for the caller to see to.
 """
 from typing import NamedTuple, Optional
 

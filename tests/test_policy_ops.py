@@ -773,6 +773,31 @@ def test_calls_on_other_streams_and_interleaved():
 
 
 @pytest.mark.gpu
+def test_a_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
+    import torch
+    import magical_amd as m
+    x, a = torch.randn(9, 18, device='cuda', requires_grad=True), torch.arange(9, device='cuda')
+    alive = m.action_log_probs(x, a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(m._native.MgxError, match='earlier calls'):
+            m.action_log_probs(x, a)
+        detached = m.action_log_probs(x.detach(), a)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(detached.log_prob, alive.log_prob.detach())
+    want, = torch.autograd.grad(alive.log_prob.sum(), x)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(m.action_log_probs(x, a).log_prob.sum(), x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_negations_that_torch_has_put_off_are_taken():
     import torch
     import magical_amd as m
