@@ -188,7 +188,7 @@ void refuse_capture_beside_eager_graph(const Tensor &logits) {
     const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(logits);
     if (!accumulator || !logits.is_cuda()) return;
     const auto earlier = accumulator->stream();
-    if (!earlier || *earlier != c10::hip::getDefaultHIPStream(logits.device().index()).unwrap()) return;
+    if (!earlier || earlier->id() != c10::hip::getDefaultHIPStream(logits.device().index()).id()) return;
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
         throw MgxError("logits that need a gradient still belong to results of earlier calls on the default stream: free these results before this "
                        "call is captured, or give logits.detach()");

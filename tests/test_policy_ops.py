@@ -798,6 +798,34 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
 
 
 @pytest.mark.gpu
+def test_a_capture_beside_a_warm_up_on_a_side_stream():
+    """The usual way to a captured training step: warmed up on a side stream, its results freed."""
+    import torch
+    import magical_amd as m
+    x, a = torch.randn(9, 18, device='cuda', requires_grad=True), torch.arange(9, device='cuda')
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            x.grad = None
+            loss = m.action_log_probs(x, a).log_prob.sum()
+            loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    want = x.grad.clone()
+    del loss
+    x.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        m.action_log_probs(x, a).log_prob.sum().backward()
+    for _ in range(3):
+        x.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, want)
+
+
+@pytest.mark.gpu
 def test_negations_that_torch_has_put_off_are_taken():
     import torch
     import magical_amd as m
