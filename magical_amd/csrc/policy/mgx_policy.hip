@@ -675,7 +675,9 @@ struct Top {
         }
         if (at_least) bound = ((uint64_t)at_least << 48) - 1;
     }
-    __device__ __forceinline__ float bound_score() const { return bound ? score_of((uint32_t)(bound >> 32)) : NEG_INF; }          // (none above it: no key beats it)
+    // the least score that can still get in, offered from further on in the row (an equal one with a lower index could too: there are none);
+    // one up from the bound's, and never -inf, which is not open
+    __device__ __forceinline__ float least_score() const { return fmaxf(score_of((uint32_t)(bound >> 32) + 1), -FLT_MAX); }          // (no bound: a NaN's bits)
     // every lane offers one key (0: none)
     __device__ __forceinline__ void offer(uint64_t key) {
         uint64_t who = __ballot(key > bound);
@@ -752,6 +754,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
     __shared__ float lds[WAVES][3];
     __shared__ uint64_t lds_keys[TOP ? WAVES : 1][TOP ? Top::CAPACITY : 1];
     __shared__ int lds_count[WAVES];
+    __shared__ uint4 lds_scores[TOP ? BLOCK : 1][TOP ? L::U : 1];
     const int n = (int)sc.n, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), top = TOP ? out.top : 0;
     const int first = SPLIT ? (int)blockIdx.x * part_tiles : 0, behind = SPLIT ? min(first + part_tiles, L::count(n)) : L::count(n);
     constexpr int ROWS = WAVES / ROW_WAVES;          // of a workgroup
@@ -787,15 +790,19 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                     }
             if constexpr (TOP) {
                 if (tile == first) best.expect(um);
-                // (the wavefront's places ascend: a later tile's score that only equals the k-th best is behind it)
-                const float bound = best.bound_score();
-                if (__ballot(tile == first ? m >= bound : m > bound)) {
-                    uint32_t mine = 0;          // which of the lane's scores are in question; read again one by one, few as they are
+                const float least = best.least_score();          // (the wavefront's places ascend with the tiles; expect()'s bound lies between two scores)
+                if (__ballot(m >= least)) {
+                    uint32_t mine = 0;          // which of the lane's scores are in question; taken one by one, by way of LDS (its own place: no waits)
 #pragma unroll
-                    for (int k = 0; k < L::U * L::V; k++) mine |= x[k] >= bound && x[k] > NEG_INF ? 1u << k : 0;          // (what is behind the end is -inf)
+                    for (int k = L::U * L::V - 1; k >= 0; k--) mine = mine + mine + (x[k] >= least);
+                    if (mine)
+#pragma unroll
+                        for (int u = 0; u < L::U; u++) __builtin_memcpy(&lds_scores[threadIdx.x][u], now.p.w[u], 16);
                     while (__ballot(mine != 0)) {
                         const int k = __ffs((int)mine) - 1, j = (int)L::place(tile, k / L::V) + k % L::V;
-                        best.offer(mine ? key_of(row.at(j), j) : 0);
+                        T score;
+                        __builtin_memcpy(&score, (const unsigned char *)lds_scores[threadIdx.x] + (mine ? k : 0) * sizeof(T), sizeof(T));
+                        best.offer(mine ? key_of(to_f32(score), j) : 0);
                         mine &= mine - 1;
                     }
                 }

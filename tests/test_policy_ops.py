@@ -639,6 +639,36 @@ def test_draws_among_probabilities_that_are_next_to_nothing(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('n', [257, 1025, 5832, 20011, 104976])
+def test_alternatives_among_equal_extreme_and_few_scores(n):
+    """Rows of the lowest value, of zeros of both signs, of the smallest numbers around zero, with less open than asked for, with the best far back."""
+    import torch
+    import magical_amd as m
+    for dtype in DTYPES:
+        t = _torch_type(dtype)
+        low, tiny = float(torch.finfo(t).min), float(torch.finfo(t).smallest_normal)
+        x = torch.full((9, n), -float('inf'), dtype=torch.float64)
+        x[0] = low
+        x[1, n // 2:] = low
+        x[2, ::97] = low
+        x[3] = torch.where(torch.arange(n) % 3 == 0, -0.0, 0.0)
+        x[4] = torch.where(torch.arange(n) % 5 == 0, -tiny, 0.0)
+        x[4, n - 2] = tiny
+        x[5, n - 3:] = low
+        x[6] = low
+        x[6, n - 1] = 0.0
+        x[7] = torch.linspace(-3, 3, n, dtype=torch.float64)
+        x[8] = torch.linspace(3, -3, n, dtype=torch.float64)
+        x = x.to(t)
+        actions = np.full(9, n - 1)
+        for top in (1, 5, 9, 64):
+            out = m.action_log_probs(x.cuda(), torch.tensor(actions).cuda(), top=top)
+            is_open, _, _, bad = oracle(x.double().numpy())
+            want = oracle_top(x.double().numpy(), is_open, bad, top)
+            assert np.array_equal(out.top_actions.cpu().numpy(), want), (dtype, top)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """Rows that lie further than 2^32 bytes and 2^31 elements from the first one."""
     import torch
