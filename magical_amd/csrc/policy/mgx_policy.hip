@@ -603,8 +603,8 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 // the present one's arithmetic made it slower (58 -> 64 and 22 -> 28 us): registers, and other wavefronts hide the loads already.
 
 // ROW_WAVES: wavefronts that go over the tile together (1, or the workgroup's 4)
-template <typename T, int ROW_WAVES> struct Tile {
-    static constexpr int V = 16 / sizeof(T), U = 4, LANES = 64 * ROW_WAVES, SIZE = LANES * U * V;
+template <typename T, int ROW_WAVES, int VECTORS = 4> struct Tile {
+    static constexpr int V = 16 / sizeof(T), U = VECTORS, LANES = 64 * ROW_WAVES, SIZE = LANES * U * V;
     static __device__ __forceinline__ int lane() { return (int)threadIdx.x % LANES; }
     static __device__ __forceinline__ int wave() { return ROW_WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
     // vector u of a tile in this lane: a wavefront's 64 vectors are neighbours, and its places ascend with the tile and u
@@ -889,10 +889,10 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
 }
 
 // blockIdx.x: the tile, of a wavefront (ROW_WAVES 1, four rows a workgroup) or a workgroup (4)
-template <typename T, int ROW_WAVES>
+template <typename T, int ROW_WAVES, int U>
 __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions actions, const float *stats, const float *entropy, Upstream up,
                                                          T *grad, bool stream) {
-    using L = Tile<T, ROW_WAVES>;
+    using L = Tile<T, ROW_WAVES, U>;
     constexpr int ROWS = WAVES / ROW_WAVES;
     const int n = (int)sc.n;
     for (int64_t r = (int64_t)blockIdx.y * ROWS + (ROW_WAVES == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0); r < sc.rows;
@@ -1240,6 +1240,8 @@ template <typename T> Split split(int64_t rows, int64_t n) {
 // The backward pass of a longer row has a tile of a wavefront's or of a workgroup's size for each wavefront or workgroup; smaller tiles leave less of the last one empty.
 // Measured (us): 32768 x 2500 bf16 93 against 132, 16384 x 5832 76 against 86, 8192 x 20000 124 against 126, 3000 x 40001 99 against 96, 1024 x
 // 104976 86 against 81.
+// Up to two wavefront's tiles, halves of them (16-bit scores alone are that short here): 32768 x 2100 bf16 88 -> 67, x 2500 89 -> 70, x 4000 112 -> 110; longer rows 75.6 -> 76.9
+// (16384 x 5832), 60 -> 62 (750 x 50021 by workgroups), and quarters 83, 89, 149.
 template <typename T> bool backward_by_waves(int64_t n) { return Tile<T, 1>::count(n) <= 12; }
 // Short rows' alternatives come one after the other, a pass over the registers each; from nine on, of rows of some length, a wavefront a row that
 // collects and ranks them is faster (7 x 1000 fp32, 20 of them: 5.6 us against 14.6 in passes).
@@ -1349,10 +1351,16 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
                                       up, (T *)grad, stream_out);
                 else return launch(k_backward_short<T, G, E, W>, short_blocks(rows, G), BLOCK, stream, sc, given, entropy, up, (T *)grad, stream_out);
             });
-        if (backward_by_waves<T>(n))
-            return launch(k_backward_long<T, 1>, dim3((unsigned)Tile<T, 1>::count(n), (unsigned)std::min<int64_t>((rows + WAVES - 1) / WAVES, 65535)), BLOCK,
-                          stream, sc, given, stats, entropy, up, (T *)grad, stream_out);
-        return launch(k_backward_long<T, WAVES>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
+        if (backward_by_waves<T>(n)) {
+            const unsigned by_fours = (unsigned)std::min<int64_t>((rows + WAVES - 1) / WAVES, 65535);
+            if constexpr (sizeof(T) == 2)
+                if (Tile<T, 1>::count(n) <= 2)
+                    return launch(k_backward_long<T, 1, 2>, dim3((unsigned)Tile<T, 1, 2>::count(n), by_fours), BLOCK, stream, sc, given, stats, entropy, up,
+                                  (T *)grad, stream_out);
+            return launch(k_backward_long<T, 1, 4>, dim3((unsigned)Tile<T, 1>::count(n), by_fours), BLOCK, stream, sc, given, stats, entropy, up,
+                          (T *)grad, stream_out);
+        }
+        return launch(k_backward_long<T, WAVES, 4>, dim3((unsigned)Tile<T, WAVES>::count(n), (unsigned)std::min<int64_t>(rows, 65535)), BLOCK,
                       stream, sc, given, stats, entropy, up, (T *)grad, stream_out);
     });
 }
