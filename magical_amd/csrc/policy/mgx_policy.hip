@@ -663,7 +663,13 @@ struct Top {
     __device__ Top(uint64_t *lds, int k_) : keys(lds), k(k_) {}
     // Before the first offers: x are N scores that each lane is going to offer, the best of some each.  The k-th best of these 64 N bounds the
     // k-th best of all from below; found bit by bit (16 of them: the bound may be lower), it keeps most of the scores out that would not last.
+    // For one alternative it is the best of them.  (32768 x 2500 bf16: 52 us, bit by bit 59.)
     template <int N> __device__ __forceinline__ void expect(const float (&x)[N]) {
+        if (k == 1) {
+            const float most = group_max<64>(lane_max(x));
+            if (most > NEG_INF) bound = ((uint64_t)order_of(most) << 32) - 1;
+            return;
+        }
         uint32_t order[N], at_least = 0;
 #pragma unroll
         for (int i = 0; i < N; i++) order[i] = x[i] > NEG_INF ? order_of(x[i]) >> 16 : 0;
