@@ -302,8 +302,8 @@ constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
 // A row stays in the registers of G lanes (1 ... 64), E scores a lane: one read of the scores, all sums by lane exchanges, no barrier.  What
-// bounds it: memory (983040 x 18 fp32: 17.5 us where its 83 MB take 16 at a copy's rate; backward 28, 16 of them the reads and 14 the writes), from some
-// dozen scores a row on the vector unit, which issues some 15 instructions a score, 20 with a mask (61440 x 324 bf16 with a mask: 16 us, 12 of
+// bounds it: memory (983040 x 18 fp32: 16 us where its 86 MB take 17 at a copy's rate; backward 28 where its 161 MB take 31: part of them lies in the cache), from some
+// dozen scores a row on the vector unit, which issues some 15 instructions a score, 20 with a mask (61440 x 324 bf16 with a mask: 15 us, 12 of
 // them issued, where memory would take 8; backward 25, 16 issued, 16 of memory).  Lane g holds pieces of W neighbouring scores (16 bytes, or 4
 // scores): x[e] is score place(g, e).
 template <int G, int E, int W> struct Spread {
@@ -598,8 +598,8 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 // ----------------------------------------------------------------------------------------------------------------- long rows
 // A wavefront or workgroup goes over a row, or over one part of it where there are few rows, in tiles of U 16-byte vectors a lane: running
 // maximum, sum and weighted sum per lane, joined at the end; every score is read once.  What bounds it: memory (1024 x 104976 bf16: 44 us,
-// 4.9 TB/s; backward 72 us, 6.0 TB/s), with masks and alternatives the vector unit too (4096 x 5832 bf16, a mask, five alternatives: 23 us,
-// 14 of them issued, where memory would take 14), and with few rows two launches (7 x 50021 fp32, 20 alternatives: 8 and 5 us).  Loading the next tile ahead of
+// 4.9 TB/s; backward 72 us, 6.0 TB/s), with masks and alternatives the vector unit too (4096 x 5832 bf16, a mask, five alternatives: 22 us,
+// 13 of them issued, where memory would take 14), and with few rows two launches (7 x 50021 fp32, 20 alternatives: 8 and 5 us).  Loading the next tile ahead of
 // the present one's arithmetic made it slower (58 -> 64 and 22 -> 28 us): registers, and other wavefronts hide the loads already.
 
 // ROW_WAVES: wavefronts that go over the tile together (1, or the workgroup's 4)
