@@ -302,10 +302,10 @@ constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
 // A row stays in the registers of G lanes (1 ... 64), E scores a lane: one read of the scores, all sums by lane exchanges, no barrier.  What
-// bounds it: memory (983040 x 18 fp32: 16 us where its 86 MB take 17 at a copy's rate; backward 28 where its 161 MB take 31: part of them lies in the cache), from some
-// dozen scores a row on the vector unit, which issues some 15 instructions a score, 20 with a mask (61440 x 324 bf16 with a mask: 15 us, 12 of
-// them issued, where memory would take 8; backward 25, 16 issued, 16 of memory).  Lane g holds pieces of W neighbouring scores (16 bytes, or 4
-// scores): x[e] is score place(g, e).
+// bounds it: memory (983040 x 18 fp32: 16 us where its 86 MB take 17 at a copy's rate; backward 28 where its 161 MB take 31: part of them lies
+// in the cache), from some dozen scores a row on the vector unit, which issues some 15 instructions a score, 20 with a mask (61440 x 324 bf16
+// with a mask: 15 us, 12 of them issued, where memory would take 8; backward 25, 16 issued, 16 of memory).  Lane g holds pieces of W
+// neighbouring scores (16 bytes, or 4 scores): x[e] is score place(g, e).
 template <int G, int E, int W> struct Spread {
     static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
     template <typename T> static __device__ __forceinline__ void load_row(const Row<T> &row, int g, int n, float (&x)[E]) {

@@ -133,7 +133,7 @@ def replay_demos(demo_dicts, device='cuda:0', preproc=None, policy=None, **env_k
     """Replay the action tapes of demos of ONE env name through the engine, all demos in lockstep (one env per demo;
     shorter demos idle on action 0 after their end and are scored at their own last step).  Returns
     {'scores': f64[n], 'recorded_scores': f64[n], 'final_obs': [...]}: with the reference's data the two score columns are
-    the end-to-end parity check of SURVEY.md section 8f-4 (demonstrations solve their task, so both should be ~1).
+    the end-to-end parity check (demonstrations solve their task, so both should be ~1).
 
     policy: also score a policy on the demonstrations.  A callable from the env's observation (before the step) to logits
     [n, 18] on the GPU; the result then has, per demo, 'log_probs' and 'entropies' (f32[T]: log p of the recorded action, the policy's
