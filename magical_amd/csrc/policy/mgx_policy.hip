@@ -13,6 +13,7 @@
 namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
+constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // The rows of scores a call works on; an action that is not open reads as -inf.
 template <typename T> struct Scores {
@@ -298,7 +299,6 @@ struct Exp64 {
         return __builtin_bit_cast(double, w);
     }
 };
-constexpr double LOG2_E = 1.4426950408889634, LN_2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
 // A row stays in the registers of G lanes (1 ... 64), E scores a lane: one read of the scores, all sums by lane exchanges, no barrier.  What
@@ -426,11 +426,34 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
     }
 }
 
-__device__ __forceinline__ bool finite(float a, float b) { return fabsf(a) < __builtin_inff() && fabsf(b) < __builtin_inff(); }
-
 struct Upstream {          // gradients to the log probabilities and entropies, one value a row (stride 0: one for all), or NULL
     const float *lp, *h;
     int64_t lp_stride, h_stride;
+    __device__ __forceinline__ float to_log_prob(int64_t r, int64_t a) const { return lp && a >= 0 ? lp[r * lp_stride] : 0.0f; }
+    __device__ __forceinline__ float to_entropy(int64_t r) const { return h ? h[r * h_stride] : 0.0f; }
+};
+
+// The gradient is p (c0 + c1 log2 p), with log2 p no lower than LEAST_LOG2: p is 0 there in fp32, so is the product, and -inf stays out of it.  That takes
+// moderate c0 and c1: of larger ones (a gradient to the entropy over a tiny temperature) the product with log2 p overflows, and 0 x inf is NaN, or what
+// fp32 has no exponential for is no longer nothing; and NaN has to stay out of the places that are not open.  Rows with such factors are worked out
+// place by place in 64 bits.
+constexpr float LEAST_LOG2 = -256.0f, MODERATE = 0x1p40f;
+__device__ __forceinline__ bool moderate(float c0, float c1) { return fabsf(c0) <= MODERATE && fabsf(c1) <= MODERATE; }
+// (All that the row's factors were made of is read again, so that nothing stays in registers for it.)
+template <typename T> struct RowGradient64 {
+    const Scores<T> &sc;
+    const Row<T> row;
+    const int64_t a;
+    const float ref, log2_s, gl, gh, h;
+    __device__ __forceinline__ RowGradient64(const Scores<T> &sc_, int64_t r, const Actions &actions, const float *entropy, const Upstream &up, float ref_, float log2_s_)
+        : sc(sc_), row(sc_, r), a(actions.at(r)), ref(ref_), log2_s(log2_s_), gl(up.to_log_prob(r, a)), gh(up.to_entropy(r)), h(entropy[r]) {}
+    __device__ __forceinline__ T at(int64_t j) const {
+        const float x = row.at(j);
+        if (x == NEG_INF) return from_f32<T>(0.0f);
+        // (nothing overflows: the factors are fp32 numbers.  Below 2^-1000 a p makes 0 of them; where it is NaN, so is h)
+        const double l2 = ((double)x - ref) * sc.inv_t2_64 - log2_s, factor = (double)gl + (double)gh * (h + l2 * LN_2);
+        return from_f32<T>((float)(((j == a ? (double)gl : 0.0) - Exp64(1.0)(fmax(l2, -1000.0)) * factor) * (sc.inv_t2_64 * LN_2)));
+    }
 };
 
 template <typename T, int G, int E, int W>
@@ -440,7 +463,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
         const int64_t a = actions.at(r);
-        const float h = entropy[r], gl = up.lp && a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
+        const float h = entropy[r], gl = up.to_log_prob(r, a), gh = up.to_entropy(r);
         float x[E];
         S::load_row(row, g, n, x);
         // maximum and sum again (cheaper than 8 bytes a row written and read)
@@ -452,23 +475,25 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
             s += p[e];
         }
         s = group_sum<G>(s);
-        // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a
-        const float inv_s = 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
+        // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a (nothing open: s = 0, and with it both factors)
+        const float inv_s = s == 0 ? 0.0f : 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
         T *to = grad + r * sc.n;
+        if (moderate(c0, c1)) {
 #pragma unroll
-        for (int e = 0; e < E; e += W) {
-            T out[W];
+            for (int e = 0; e < E; e += W) {
+                T out[W];
 #pragma unroll
-            for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf((x[e + k] - ref) * sc.inv_t2 - log2_s, -1e30f), c0));
-            Pieces<T, W, 1>::store(to, S::place(g, e), n, e / W < n / (G * W), out, stream);
-        }
-        if (!finite(c0, c1))          // NaN, but for the places that are not open
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                if (S::place(g, e) < n && x[e] == NEG_INF) to[S::place(g, e)] = from_f32<T>(0.0f);
-        if (a >= 0 && a < n && (int)(a / W) % G == g) {          // (the lane that has just written this place)
-            const float xa = row.at(a), d = (xa - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
-            to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, -1e30f), c0), gl * sc.inv_t));
+                for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf((x[e + k] - ref) * sc.inv_t2 - log2_s, LEAST_LOG2), c0));
+                Pieces<T, W, 1>::store(to, S::place(g, e), n, e / W < n / (G * W), out, stream);
+            }
+            if (a >= 0 && a < n && (int)(a / W) % G == g) {          // (the lane that has just written this place)
+                const float xa = row.at(a), d = (xa - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
+                to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, LEAST_LOG2), c0), gl * sc.inv_t));
+            }
+        } else {
+            const RowGradient64<T> exact(sc, r, actions, entropy, up, ref, log2_s);
+#pragma unroll 1
+            for (int j = g; j < n; j += G) to[j] = exact.at(j);
         }
     }
 }
@@ -488,7 +513,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions a
         if (r < sc.rows) {
             const Row<T> row(sc, r);
             const Given given(actions, row, r, n);
-            const float h = entropy[r], gl = up.lp && given.a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
+            const float h = entropy[r], gl = up.to_log_prob(r, given.a), gh = up.to_entropy(r);
             float x[E];
             Spread<1, E, W>::load_row(row, 0, n, x);
             const float m = lane_max(x), ref = m > NEG_INF ? m : 0.0f;
@@ -498,17 +523,18 @@ __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions a
                 p[e] = __builtin_amdgcn_exp2f((x[e] - ref) * sc.inv_t2);
                 s += p[e];
             }
-            const float inv_s = 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
-            const bool nan = !finite(c0, c1);          // NaN, but for the places that are not open
+            const float inv_s = s == 0 ? 0.0f : 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (e < n) {
-                    const float v = p[e] * fmaf(c1, fmaxf((x[e] - ref) * sc.inv_t2 - log2_s, -1e30f), c0);
-                    mine[e] = from_f32<T>(nan && x[e] == NEG_INF ? 0.0f : v);
-                }
+                if (e < n) mine[e] = from_f32<T>(p[e] * fmaf(c1, fmaxf((x[e] - ref) * sc.inv_t2 - log2_s, LEAST_LOG2), c0));
             if (given.a >= 0 && given.a < n) {
                 const float d = (given.x - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
-                mine[given.a] = from_f32<T>(given.x == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, -1e30f), c0), gl * sc.inv_t));
+                mine[given.a] = from_f32<T>(given.x == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, LEAST_LOG2), c0), gl * sc.inv_t));
+            }
+            if (!moderate(c0, c1)) {
+                const RowGradient64<T> exact(sc, r, actions, entropy, up, ref, log2_s);
+#pragma unroll 1
+                for (int j = 0; j < n; j++) mine[j] = exact.at(j);
             }
         }
         wave_sync();
@@ -904,13 +930,14 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
     for (int64_t r = (int64_t)blockIdx.y * ROWS + (ROW_WAVES == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0); r < sc.rows;
          r += (int64_t)gridDim.y * ROWS) {
         const Row<T> row(sc, r);
-        L tile;
-        tile.load(row, blockIdx.x, n);
+        // (the row's own values are asked for before its scores: they come in that order, and 1024 x 104976 bf16 takes 66 us, the other way round 76)
         const int64_t a = actions.at(r);
         const float ref = stats[2 * r], log2_s = stats[2 * r + 1], h = entropy[r];
-        const float gl = up.lp && a >= 0 ? up.lp[r * up.lp_stride] : 0.0f, gh = up.h ? up.h[r * up.h_stride] : 0.0f;
+        const float gl = up.to_log_prob(r, a), gh = up.to_entropy(r);
         // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a
         const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t;
+        L tile;
+        tile.load(row, blockIdx.x, n);
         float x[L::U * L::V];
         tile.p.scores(row, x);
         T *to = grad + r * sc.n;
@@ -923,16 +950,20 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
 #pragma unroll
             for (int k = 0; k < L::V; k++) {
                 const float l2 = fmaf(x[u * L::V + k] - ref, sc.inv_t2, -log2_s);
-                v[k] = from_f32<T>(__builtin_amdgcn_exp2f(l2) * fmaf(c1, fmaxf(l2, -1e30f), c0));
+                v[k] = from_f32<T>(__builtin_amdgcn_exp2f(l2) * fmaf(c1, fmaxf(l2, LEAST_LOG2), c0));
             }
             if (j < n) Pieces<T, L::V, 1>::store(to, (int)j, n, false, v, stream);
-            if (!finite(c0, c1))          // NaN, but for the places that are not open
-#pragma unroll
-                for (int k = 0; k < L::V; k++)
-                    if (j + k < n && x[u * L::V + k] == NEG_INF) to[j + k] = from_f32<T>(0.0f);
             if (a >= j && a < j + L::V && a < n) {          // (the lane that has just written this place)
                 const float xa = row.at(a), l2 = fmaf(xa - ref, sc.inv_t2, -log2_s);
-                to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(__builtin_amdgcn_exp2f(l2), fmaf(c1, fmaxf(l2, -1e30f), c0), gl * sc.inv_t));
+                to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(__builtin_amdgcn_exp2f(l2), fmaf(c1, fmaxf(l2, LEAST_LOG2), c0), gl * sc.inv_t));
+            }
+        }
+        if (__ballot(!moderate(c0, c1))) {          // (one row a wavefront: a scalar branch.  Over what has just been written, each lane its own)
+            const RowGradient64<T> exact(sc, r, actions, entropy, up, stats[2 * r], stats[2 * r + 1]);
+#pragma unroll 1
+            for (int i = 0; i < L::U * L::V; i++) {
+                const int64_t j = L::place(blockIdx.x, i / L::V) + i % L::V;
+                if (j < n) to[j] = exact.at(j);
             }
         }
     }

@@ -1,0 +1,76 @@
+"""The operators on a policy's action scores at the ends of what is documented, and beside torch's own machinery: each test fails for a fault that
+was there once.  The oracle and the counting of roundings are test_policy_ops.py's; where a bound differs, it is derived beside the test."""
+import math
+
+import numpy as np
+import pytest
+
+from tests.test_policy_ops import U, _torch_type, err_entropy, err_log_prob, oracle, oracle_grad
+
+
+def grad_bound(is_open, lp, h, g_lp, g_h, want, temperature, eps, tiny):
+    """dx = p (g_lp' + g_H (log p + H)) / T: p is off by err(log p) + 4 u relative, the factor by the roundings of its terms; one rounding to the
+    logits' type.  As in test_policy_ops.py but for two things.  An exponential below 2^-126 may be taken as none: times a factor of at most
+    2^40 (1 + 160 ln 2), beyond which the kernels work in 64 bits, that is below 2^-79.  And nothing is added for the least number the result's type
+    holds where the type is fp32: results here go down to 1e-37, and what is below the normal numbers, 2^-126, counts as nothing."""
+    n = lp.shape[1]
+    lpz = np.where(is_open & ~np.isneginf(lp), lp, 0.0)
+    p = np.where(is_open, np.exp(lp), 0.0)
+    rel = err_log_prob(np.abs(lpz) + math.log(n), n) + 4 * U
+    size = np.abs(g_lp)[:, None] + np.abs(g_h)[:, None] * (np.abs(lpz) + h[:, None])
+    e = p * (rel * size + np.abs(g_h)[:, None] * (rel + err_entropy(n)) + 4 * U * size) / temperature + 4 * U * np.abs(want)
+    scale = (np.abs(g_lp) + np.abs(g_h) * (h + 1))[:, None] / temperature
+    return e + np.maximum(np.abs(want) * (1 + 1e-3) * eps / 2, tiny) + 2.0 ** -126 * (1 + 160 * np.minimum(scale, 2.0 ** 40))
+
+
+# (n, rows): a lane a row, 4 ... 64 lanes, a wavefront a row by halves of tiles (16-bit) and by whole ones, a workgroup a row
+GRADIENT_SHAPES = [(18, 13), (40, 13), (324, 13), (1500, 13), (2500, 13), (6000, 13), (60000, 7)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('n,rows', GRADIENT_SHAPES)
+def test_gradients_at_every_temperature_and_scale(n, rows, dtype):
+    """Places that are not open, and open ones of no probability, have gradient 0 whatever the temperature and the upstream gradients: in products
+    with what overflows they would be NaN."""
+    import torch
+    import magical_amd as m
+    t = _torch_type(dtype)
+    rng = np.random.RandomState(n)
+    x = rng.randn(rows, n) * 3
+    x[rng.rand(rows, n) < 0.1] = -np.inf
+    x[rng.rand(rows, n) < 0.1] = float(torch.finfo(t).min)
+    x[0] = -np.inf
+    x[1] = 0.75
+    x[2] = float(torch.finfo(t).min)
+    x[3, : n // 2] = 2.0
+    x[4] = rng.randn(n) * 1e-3
+    x = torch.tensor(x).to(t)
+    x64 = x.double().numpy()
+    mask = rng.rand(rows, n) < 0.8
+    mask[5] = False
+    actions = rng.randint(0, n, rows)
+    actions[6] = -1
+    base_lp, base_h = rng.randn(rows), rng.randn(rows)
+    for temperature, scale in [(1e-37, 1.0), (1e-37, 1e-30), (1e-30, 1.0), (1e-20, 1.0), (1e-20, 1e-18), (1e-10, 1.0), (1e-9, 1.0), (1e-4, 65536.0),
+                               (1e-4, 1.0), (1.0, 1e9), (1.0, 1e30), (1.0, 2.0 ** 24), (1.0, 1e-30), (1e4, 1.0), (1e10, 1e10), (1e20, 1e30), (1e37, 1e37)]:
+        for use_mask in (None, mask):
+            g_lp, g_h = (base_lp * scale).astype(np.float32), (base_h * scale).astype(np.float32)
+            if scale == 2.0 ** 24:
+                g_lp[:] = 0
+            leaf = x.cuda().requires_grad_(True)
+            out = m.action_log_probs(leaf, torch.tensor(actions).cuda(), mask=None if use_mask is None else torch.tensor(mask).cuda(), temperature=temperature)
+            torch.autograd.backward((out.log_prob, out.entropy), (torch.tensor(g_lp).cuda(), torch.tensor(g_h).cuda()))
+            got = leaf.grad.double().cpu().numpy()
+            is_open, lp, h, bad = oracle(x64, use_mask, temperature)
+            gl64, gh64 = g_lp.astype(np.float64), g_h.astype(np.float64)
+            want = oracle_grad(is_open, lp, h, actions, gl64, gh64, temperature)
+            bound = grad_bound(is_open, lp, h, gl64, gh64, want, temperature, torch.finfo(t).eps, 2.0 ** -25 if dtype == 'f16' else 0.0)
+            what = (n, dtype, temperature, scale, use_mask is not None)
+            assert not np.isnan(got).any(), what
+            assert np.all(got[~is_open] == 0), what
+            big = float(torch.finfo(t).max)
+            huge = np.isinf(got)          # (beyond the type's range)
+            assert np.all(np.sign(got[huge]) == np.sign(want[huge])) and np.all(np.abs(want[huge]) + bound[huge] >= big), what
+            err = np.abs(got - want)[~huge]
+            assert np.all(err <= bound[~huge]), (what, np.max(err / bound[~huge]))
