@@ -46,7 +46,7 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
                          int64_t workspace_bytes, void *stream);
 /* gradient of sum_r grad_log_prob[r] * log_prob[r] + grad_entropy[r] * entropy[r] to the scores, in their type: grad [rows][n], dense.
  * grad_log_prob / grad_entropy: f32, row r at r * stride (0: one value for all), NULL = zero; the other arguments are the forward
- * call's, stats and entropy its outputs. */
+ * call's, stats and entropy its outputs.  A row whose given action is >= n has NaN at its open places, unless its grad_log_prob is 0. */
 int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride,
                                   const uint8_t *mask, int64_t mask_row_stride, double temperature, const void *actions,
                                   int action_bytes, const float *stats, const float *entropy, const float *grad_log_prob,

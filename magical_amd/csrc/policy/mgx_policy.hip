@@ -429,7 +429,11 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
 struct Upstream {          // gradients to the log probabilities and entropies, one value a row (stride 0: one for all), or NULL
     const float *lp, *h;
     int64_t lp_stride, h_stride;
-    __device__ __forceinline__ float to_log_prob(int64_t r, int64_t a) const { return lp && a >= 0 ? lp[r * lp_stride] : 0.0f; }
+    // (behind the last action the log probability is NaN: whatever flows back through it is, too)
+    __device__ __forceinline__ float to_log_prob(int64_t r, int64_t a, int64_t n) const {
+        const float g = lp && a >= 0 ? lp[r * lp_stride] : 0.0f;
+        return a < n || g == 0 ? g : __builtin_nanf("");
+    }
     __device__ __forceinline__ float to_entropy(int64_t r) const { return h ? h[r * h_stride] : 0.0f; }
 };
 
@@ -446,7 +450,7 @@ template <typename T> struct RowGradient64 {
     const int64_t a;
     const float ref, log2_s, gl, gh, h;
     __device__ __forceinline__ RowGradient64(const Scores<T> &sc_, int64_t r, const Actions &actions, const float *entropy, const Upstream &up, float ref_, float log2_s_)
-        : sc(sc_), row(sc_, r), a(actions.at(r)), ref(ref_), log2_s(log2_s_), gl(up.to_log_prob(r, a)), gh(up.to_entropy(r)), h(entropy[r]) {}
+        : sc(sc_), row(sc_, r), a(actions.at(r)), ref(ref_), log2_s(log2_s_), gl(up.to_log_prob(r, a, sc_.n)), gh(up.to_entropy(r)), h(entropy[r]) {}
     __device__ __forceinline__ T at(int64_t j) const {
         const float x = row.at(j);
         if (x == NEG_INF) return from_f32<T>(0.0f);
@@ -463,7 +467,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
         const int64_t a = actions.at(r);
-        const float h = entropy[r], gl = up.to_log_prob(r, a), gh = up.to_entropy(r);
+        const float h = entropy[r], gl = up.to_log_prob(r, a, n), gh = up.to_entropy(r);
         float x[E];
         S::load_row(row, g, n, x);
         // maximum and sum again (cheaper than 8 bytes a row written and read)
@@ -513,7 +517,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions a
         if (r < sc.rows) {
             const Row<T> row(sc, r);
             const Given given(actions, row, r, n);
-            const float h = entropy[r], gl = up.to_log_prob(r, given.a), gh = up.to_entropy(r);
+            const float h = entropy[r], gl = up.to_log_prob(r, given.a, n), gh = up.to_entropy(r);
             float x[E];
             Spread<1, E, W>::load_row(row, 0, n, x);
             const float m = lane_max(x), ref = m > NEG_INF ? m : 0.0f;
@@ -933,7 +937,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
         // (the row's own values are asked for before its scores: they come in that order, and 1024 x 104976 bf16 takes 66 us, the other way round 76)
         const int64_t a = actions.at(r);
         const float ref = stats[2 * r], log2_s = stats[2 * r + 1], h = entropy[r];
-        const float gl = up.to_log_prob(r, a), gh = up.to_entropy(r);
+        const float gl = up.to_log_prob(r, a, n), gh = up.to_entropy(r);
         // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a
         const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t;
         L tile;

@@ -50,7 +50,8 @@ def action_log_probs(logits, actions, *, mask=None, temperature=1.0, top=0):
     alternatives of each row (best first, equal logits by the lower index).
 
     logits [..., n]; actions int32 / int64 [...]: a negative one marks a row in which none is given (a padded step: log probability 0,
-    no gradient through it; entropy and alternatives are still there), one >= n gives NaN.  top: 0 ... min(n, 64).
+    no gradient through it; entropy and alternatives are still there), one >= n gives NaN, and NaN as gradient unless nothing flows
+    back through its log probability.  top: 0 ... min(n, 64).
     Differentiable to the logits through log_prob and entropy (once); the gradient has the logits' type and is 0 wherever an action is
     not open.  Returns ActionLogProbs.  Refuses wrong types (TypeError), shapes, devices and ranges (ValueError)."""
     return ActionLogProbs(*_ops.log_probs(logits, actions, mask, temperature, top))

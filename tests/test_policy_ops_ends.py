@@ -74,3 +74,46 @@ def test_gradients_at_every_temperature_and_scale(n, rows, dtype):
             assert np.all(np.sign(got[huge]) == np.sign(want[huge])) and np.all(np.abs(want[huge]) + bound[huge] >= big), what
             err = np.abs(got - want)[~huge]
             assert np.all(err <= bound[~huge]), (what, np.max(err / bound[~huge]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('n,rows', [(18, 13), (40, 13), (324, 13), (1500, 13), (2500, 13), (6000, 13), (60000, 7)])
+def test_an_action_behind_the_last_one_has_no_finite_gradient(n, rows, dtype):
+    """Its log probability is NaN, and so is what flows back through it -- unless nothing does.  The entropy's gradient and other rows are not
+    touched."""
+    import torch
+    import magical_amd as m
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(rows, n, generator=g).to(_torch_type(dtype))
+    x[:, 1] = float('-inf')
+    mask = torch.rand(rows, n, generator=g) < 0.8
+    mask[:, 0] = True
+    mask[4] = False
+    is_open = (mask & (x > float('-inf'))).numpy()
+    actions = torch.randint(0, n, (rows,), generator=g)
+    bad = actions.clone()
+    bad[0], bad[2], bad[3], bad[4] = n, n + 7, n, n
+    g_lp, g_h = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    g_lp[3] = 0.0
+    leaf = x.cuda().requires_grad_(True)
+
+    def grads(acts, gl, gh):
+        out = m.action_log_probs(leaf, acts.cuda(), mask=mask.cuda())
+        outs, ups = zip(*[(o, u.cuda()) for o, u in ((out.log_prob, gl), (out.entropy, gh)) if u is not None])
+        return torch.autograd.grad(outs, leaf, ups)[0].float().cpu().numpy()
+
+    for kind in (torch.int64, torch.int32):
+        for gh in (g_h, None):
+            got, fine = grads(bad.to(kind), g_lp, gh), grads(actions.to(kind), g_lp, gh)
+            for r in range(rows):
+                if r in (0, 2):
+                    assert np.all(np.isnan(got[r][is_open[r]])) and np.all(got[r][~is_open[r]] == 0), r
+                elif r == 4:
+                    assert np.all(got[r] == 0)
+                elif r != 3:
+                    assert np.array_equal(got[r], fine[r]), r
+            assert np.array_equal(got[3], grads(torch.full_like(actions, -1).to(kind), g_lp, gh)[3])
+    # (against rows without an action: the place of a given one is worked out with a rounding less than its neighbours)
+    entropy_only, none = grads(bad, None, g_h), grads(torch.where(bad >= n, -1, bad), None, g_h)
+    assert np.array_equal(entropy_only, none) and np.all(np.isfinite(none))
