@@ -815,15 +815,18 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
             if (m > a.m) a.to(m, sc.inv_t2);
             const float ref = a.m > NEG_INF ? a.m : 0.0f;
             const int live = L::live(tile, n);
+            float s = 0, t = 0;          // (the tile's own: scores next to nothing each are added up before they meet a large sum)
 #pragma unroll
             for (int u = 0; u < L::U; u++)
                 if (u < live)
 #pragma unroll
                     for (int k = u * L::V; k < (u + 1) * L::V; k++) {
                         const float d = (x[k] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
-                        a.s += p;
-                        a.t = fmaf(p, fmaxf(d, -1e30f), a.t);
+                        s += p;
+                        t = fmaf(p, fmaxf(d, -1e30f), t);
                     }
+            a.s += s;
+            a.t += t;
             if constexpr (TOP) {
                 if (tile == first) best.expect(um);
                 const float least = best.least_score();          // (the wavefront's places ascend with the tiles; expect()'s bound lies between two scores)

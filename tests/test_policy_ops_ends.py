@@ -117,3 +117,43 @@ def test_an_action_behind_the_last_one_has_no_finite_gradient(n, rows, dtype):
     # (against rows without an action: the place of a given one is worked out with a rounding less than its neighbours)
     entropy_only, none = grads(bad, None, g_h), grads(torch.where(bad >= n, -1, bad), None, g_h)
     assert np.array_equal(entropy_only, none) and np.all(np.isfinite(none))
+
+
+def additions(n, rows, dtype):
+    """The longest chain of additions behind a row's sums: a tile's scores of a lane, its tiles, the 6 steps over a wavefront's lanes, 3 over a
+    workgroup's wavefronts, 16 parts of a lane and 6 steps over the lanes that join them.  Tiles are 4 vectors of 16 bytes a lane."""
+    in_tile = 16 if dtype == 'f32' else 32
+    tiles = -(-n // (64 * in_tile)) if rows >= 2048 else -(-n // (256 * in_tile))          # (fewer where a row is shared out further)
+    return in_tile + tiles + 6 + 3 + 16 + 6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('n,rows', [(2500, 5), (5832, 4096), (20000, 1), (20000, 4096), (104976, 3), (104976, 1100), (104976, 4096), (1200007, 2), (1200007, 4096)])
+def test_sums_of_long_rows_are_as_close_as_their_additions(n, rows, dtype):
+    """One score ahead of all others, so far that each of these is next to nothing beside it and all together are not: a sum that takes them one
+    by one loses them.  log p = d - log s: 3 roundings of d, a relative error of A u of the sum of A additions in a row, 4 u d of the others'
+    exponentials, 8 u for the exponential, the logarithm and the difference, 2 u |log s|; H = log s - t / s with t / s, d times the others' share,
+    off by twice as much relative (t and s)."""
+    import torch
+    import magical_amd as m
+    L = math.log(n)
+    for ahead in (17.5, 15.0, 12.0, L):
+        row = torch.zeros(n, dtype=_torch_type(dtype))
+        row[n // 3] = ahead
+        x64 = row.double().numpy()[None]
+        _, lp, h, _ = oracle(x64)
+        d = float(x64.max())
+        A = additions(n, rows, dtype)
+        share = float(np.exp(lp[0, 0]) * (n - 1))          # of the sum, the others'
+        tol_lp = lambda dist: U * (4 * dist + A + 8 + 4 * d * share + 2 * abs(lp[0, n // 3]))      # noqa: E731
+        tol_h = tol_lp(0.0) + U * (2 * A + 16 + 8 * d) * d * share
+        actions = torch.full((rows,), n // 3, device='cuda')
+        actions[1::2] = n - 1
+        for top in (0, 3):
+            out = m.action_log_probs(row.cuda().expand(rows, n), actions, top=top)
+            got_lp, got_h = out.log_prob.double().cpu().numpy(), out.entropy.double().cpu().numpy()
+            assert np.abs(got_lp[::2] - lp[0, n // 3]).max() <= tol_lp(0.0), (ahead, np.abs(got_lp[::2] - lp[0, n // 3]).max() / U, A)
+            if rows > 1:
+                assert np.abs(got_lp[1::2] - lp[0, n - 1]).max() <= tol_lp(d), (ahead, np.abs(got_lp[1::2] - lp[0, n - 1]).max() / U, A)
+            assert np.abs(got_h - h[0]).max() <= tol_h, (ahead, np.abs(got_h - h[0]).max(), tol_h)
