@@ -22,12 +22,31 @@ template <typename T> struct Scores {
     int64_t rows, n, stride, mask_stride;
     float inv_t, inv_t2;        // 1 / temperature, log2(e) / temperature: exponentials are taken to the base 2, as the hardware does
     double inv_t2_64;
+    // Two scores may be further apart than the largest fp32 number (3e38 and -3e38).  Over a T of up to 1e36 their quotient is one whose exponential is 0
+    // all the same; over a larger one the difference is taken of their halves (unit 1 / 2, else 1), in one operation.  (From what is there: two more
+    // arguments cost 983040 x 18 fp32 0.7 us of 17.)
+    __host__ __device__ __forceinline__ bool by_halves() const { return __builtin_bit_cast(uint32_t, inv_t2) < __builtin_bit_cast(uint32_t, 1.44e-36f); }
+    // one score's (v - ref) / T as a result, which is to be finite over smaller T too: always by halves
+    __device__ __forceinline__ float over_t(float v, float ref) const { return 2.0f * (fmaf(v, 0.5f, -0.5f * ref) * inv_t); }
 };
 
 using half = _Float16;
 using bf16 = __bf16;
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }          // to nearest, ties to even
+
+// Differences of scores, in a loop's scalar registers (worked out on their bits: there is no scalar unit for floats; the long rows' kernel is given it,
+// 65536 x 1500 bf16 44.7 us, itself 45.7, without halves 42.9).
+struct Difference {
+    float unit, per_t2;         // per_t2: log2(e) / (T unit)
+    template <typename T> __host__ __device__ __forceinline__ explicit Difference(const Scores<T> &sc) {
+        const uint32_t one_exponent = sc.by_halves() ? 1u << 23 : 0;
+        unit = __builtin_bit_cast(float, 0x3f800000u - one_exponent);
+        per_t2 = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, sc.inv_t2) + one_exponent);
+    }
+    __device__ __forceinline__ float operator()(float v, float unit_ref) const { return fmaf(v, unit, -unit_ref); }
+    __device__ __forceinline__ float over_t2(float v, float unit_ref) const { return (*this)(v, unit_ref) * per_t2; }
+};
 
 template <typename T> struct Row {
     const T *x;
@@ -361,12 +380,17 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
         const bool some = m > NEG_INF;
         const float ref = some ? m : 0.0f;
         float s = 0, t = 0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const float d = (x[e] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
+        const auto add = [&](float d) {
+            const float p = __builtin_amdgcn_exp2f(d);
             s += p;
             t = fmaf(p, fmaxf(d, -1e30f), t);          // (not open: 0 x a finite number)
-        }
+        };
+        if (!sc.by_halves())
+#pragma unroll
+            for (int e = 0; e < E; e++) add((x[e] - ref) * sc.inv_t2);
+        else
+#pragma unroll
+            for (int e = 0; e < E; e++) add(fmaf(x[e], 0.5f, -0.5f * ref) * (2.0f * sc.inv_t2));
         s = group_sum<G>(s);
         t = group_sum<G>(t);
         const bool undefined = !(s == s);
@@ -374,7 +398,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
         if (g == 0) {
             float lp = 0.0f;
             if (given.a >= n || (given.a >= 0 && undefined)) lp = nan;
-            else if (given.a >= 0) lp = some ? (given.x - ref) * sc.inv_t - log_s : NEG_INF;
+            else if (given.a >= 0) lp = some ? sc.over_t(given.x, ref) - log_s : NEG_INF;
             log_prob[r] = lp;
             entropy[r] = undefined ? nan : some ? log_s - t / s * (float)LN_2 : 0.0f;
         }
@@ -404,7 +428,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions
             if (g == 0) {
                 const bool there = v > NEG_INF && !undefined;
                 const int action = there ? i : -1;
-                const float lp = there ? (v - ref) * sc.inv_t - log_s : NEG_INF;
+                const float lp = there ? sc.over_t(v, ref) - log_s : NEG_INF;
                 if constexpr (staged) {
                     run_actions[lane * top + k] = action;
                     run_log_probs[lane * top + k] = lp;
@@ -464,6 +488,7 @@ template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions actions, const float *entropy, Upstream up, T *grad, bool stream) {
     using S = Spread<G, E, W>;
     const int g = threadIdx.x % G, n = (int)sc.n;
+    const Difference diff(sc);
     for (int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G; r < sc.rows; r += (int64_t)gridDim.x * (BLOCK / G)) {
         const Row<T> row(sc, r);
         const int64_t a = actions.at(r);
@@ -471,11 +496,11 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
         float x[E];
         S::load_row(row, g, n, x);
         // maximum and sum again (cheaper than 8 bytes a row written and read)
-        const float m = group_max<G>(lane_max(x)), ref = m > NEG_INF ? m : 0.0f;
+        const float m = group_max<G>(lane_max(x)), ref = m > NEG_INF ? m : 0.0f, unit_ref = diff.unit * ref;
         float s = 0, p[E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            p[e] = __builtin_amdgcn_exp2f((x[e] - ref) * sc.inv_t2);
+            p[e] = __builtin_amdgcn_exp2f(diff.over_t2(x[e], unit_ref));
             s += p[e];
         }
         s = group_sum<G>(s);
@@ -487,11 +512,11 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
             for (int e = 0; e < E; e += W) {
                 T out[W];
 #pragma unroll
-                for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf((x[e + k] - ref) * sc.inv_t2 - log2_s, LEAST_LOG2), c0));
+                for (int k = 0; k < W; k++) out[k] = from_f32<T>(p[e + k] * fmaf(c1, fmaxf(diff.over_t2(x[e + k], unit_ref) - log2_s, LEAST_LOG2), c0));
                 Pieces<T, W, 1>::store(to, S::place(g, e), n, e / W < n / (G * W), out, stream);
             }
             if (a >= 0 && a < n && (int)(a / W) % G == g) {          // (the lane that has just written this place)
-                const float xa = row.at(a), d = (xa - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
+                const float xa = row.at(a), d = diff.over_t2(xa, unit_ref), pa = __builtin_amdgcn_exp2f(d);
                 to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, LEAST_LOG2), c0), gl * sc.inv_t));
             }
         } else {
@@ -510,6 +535,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions a
     static_assert(G == 1);
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (int)sc.n;
+    const Difference diff(sc);
     T *const mine = (T *)lds_bytes + (wave * 64 + lane) * n;
     const unsigned char *const run = lds_bytes + wave * 64 * n * sizeof(T);
     for (int64_t r0 = ((int64_t)blockIdx.x * WAVES + wave) * 64; r0 < sc.rows; r0 += (int64_t)gridDim.x * BLOCK) {
@@ -520,19 +546,19 @@ __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions a
             const float h = entropy[r], gl = up.to_log_prob(r, given.a, n), gh = up.to_entropy(r);
             float x[E];
             Spread<1, E, W>::load_row(row, 0, n, x);
-            const float m = lane_max(x), ref = m > NEG_INF ? m : 0.0f;
+            const float m = lane_max(x), ref = m > NEG_INF ? m : 0.0f, unit_ref = diff.unit * ref;
             float s = 0, p[E];
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                p[e] = __builtin_amdgcn_exp2f((x[e] - ref) * sc.inv_t2);
+                p[e] = __builtin_amdgcn_exp2f(diff.over_t2(x[e], unit_ref));
                 s += p[e];
             }
             const float inv_s = s == 0 ? 0.0f : 1.0f / s, log2_s = log2f(s), c0 = -(gl + gh * h) * sc.inv_t * inv_s, c1 = -gh * (float)LN_2 * sc.inv_t * inv_s;
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (e < n) mine[e] = from_f32<T>(p[e] * fmaf(c1, fmaxf((x[e] - ref) * sc.inv_t2 - log2_s, LEAST_LOG2), c0));
+                if (e < n) mine[e] = from_f32<T>(p[e] * fmaf(c1, fmaxf(diff.over_t2(x[e], unit_ref) - log2_s, LEAST_LOG2), c0));
             if (given.a >= 0 && given.a < n) {
-                const float d = (given.x - ref) * sc.inv_t2, pa = __builtin_amdgcn_exp2f(d);
+                const float d = diff.over_t2(given.x, unit_ref), pa = __builtin_amdgcn_exp2f(d);
                 mine[given.a] = from_f32<T>(given.x == NEG_INF ? 0.0f : fmaf(pa, fmaf(c1, fmaxf(d - log2_s, LEAST_LOG2), c0), gl * sc.inv_t));
             }
             if (!moderate(c0, c1)) {
@@ -648,25 +674,25 @@ template <typename T, int ROW_WAVES, int VECTORS = 4> struct Tile {
     static __host__ __device__ __forceinline__ int count(int64_t n) { return (int)((n + SIZE - 1) / SIZE); }
 };
 
-// Maximum m, s = sum 2^d, t = sum d 2^d with d = (x - m) inv_t2, of scores seen so far (none: m = -inf, s = t = 0).  A NaN or +inf among
+// Maximum m, s = sum 2^d, t = sum d 2^d with d = (x - m) log2(e) / T, of scores seen so far (none: m = -inf, s = t = 0).  A NaN or +inf among
 // them makes s NaN.
 struct Softmax {
     float m = NEG_INF, s = 0, t = 0;
-    __device__ __forceinline__ void to(float new_m, float inv_t2) {          // the same scores against a larger maximum
-        const float d = (m - new_m) * inv_t2, c = __builtin_amdgcn_exp2f(d);
+    __device__ __forceinline__ void to(float new_m, const Difference &diff) {          // the same scores against a larger maximum
+        const float d = diff.over_t2(m, diff.unit * new_m), c = __builtin_amdgcn_exp2f(d);
         t = s == 0 ? 0 : c * fmaf(fmaxf(d, -1e30f), s, t);
         s = s == 0 ? 0 : c * s;
         m = new_m;
     }
-    __device__ __forceinline__ void join(Softmax o, float inv_t2) {
+    __device__ __forceinline__ void join(Softmax o, const Difference &diff) {
         const float top = fmaxf(m, o.m);
-        if (top > NEG_INF) { to(top, inv_t2); o.to(top, inv_t2); }
+        if (top > NEG_INF) { to(top, diff); o.to(top, diff); }
         s += o.s;
         t += o.t;
     }
-    __device__ __forceinline__ void join_wave(float inv_t2) {
+    __device__ __forceinline__ void join_wave(const Difference &diff) {
         const float top = group_max<64>(m);
-        if (top > NEG_INF) to(top, inv_t2);
+        if (top > NEG_INF) to(top, diff);
         s = group_sum<64>(s);
         t = group_sum<64>(t);
     }
@@ -764,7 +790,7 @@ template <typename T> __device__ __forceinline__ void finish_row(const Scores<T>
     if (lane == 0) {
         float lp = 0.0f;
         if (given.a >= n || (given.a >= 0 && undefined)) lp = nan;
-        else if (given.a >= 0) lp = some ? (given.x - ref) * sc.inv_t - log_s : NEG_INF;
+        else if (given.a >= 0) lp = some ? sc.over_t(given.x, ref) - log_s : NEG_INF;
         out.log_prob[r] = lp;
         out.entropy[r] = undefined ? nan : some ? log_s - all.t / all.s * (float)LN_2 : 0.0f;
         if (out.stats) { out.stats[2 * r] = ref; out.stats[2 * r + 1] = all.s == 0 ? 0.0f : log2f(all.s); }
@@ -773,7 +799,7 @@ template <typename T> __device__ __forceinline__ void finish_row(const Scores<T>
         const bool there = lane < best.count && !undefined;
         const uint64_t key = there ? best.keys[lane] : 0;
         out.top_actions[r * out.top + lane] = there ? index_of(key) : -1;
-        out.top_log_probs[r * out.top + lane] = there ? (score_of((uint32_t)(key >> 32)) - ref) * sc.inv_t - log_s : NEG_INF;
+        out.top_log_probs[r * out.top + lane] = there ? sc.over_t(score_of((uint32_t)(key >> 32)), ref) - log_s : NEG_INF;
     }
 }
 
@@ -785,7 +811,7 @@ struct Partials {
 
 // One wavefront (ROW_WAVES 1) or workgroup (4) goes over a row; SPLIT: a workgroup over blockIdx.x-th part of part_tiles tiles of it.
 template <typename T, bool TOP, int ROW_WAVES, bool SPLIT>
-__global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions actions, LogProbOut out, int part_tiles, Partials to) {
+__global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions actions, LogProbOut out, int part_tiles, Partials to, Difference diff) {
     using L = Tile<T, ROW_WAVES>;
     __shared__ float lds[WAVES][3];
     __shared__ uint64_t lds_keys[TOP ? WAVES : 1][TOP ? Top::CAPACITY : 1];
@@ -812,8 +838,8 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                 for (int k = 1; k < L::V; k++) um[u] = max_of(um[u], x[u * L::V + k]);
             }
             const float m = lane_max(um);
-            if (m > a.m) a.to(m, sc.inv_t2);
-            const float ref = a.m > NEG_INF ? a.m : 0.0f;
+            if (m > a.m) a.to(m, diff);
+            const float ref = a.m > NEG_INF ? diff.unit * a.m : 0.0f;
             const int live = L::live(tile, n);
             float s = 0, t = 0;          // (the tile's own: scores next to nothing each are added up before they meet a large sum)
 #pragma unroll
@@ -821,7 +847,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                 if (u < live)
 #pragma unroll
                     for (int k = u * L::V; k < (u + 1) * L::V; k++) {
-                        const float d = (x[k] - ref) * sc.inv_t2, p = __builtin_amdgcn_exp2f(d);
+                        const float d = diff.over_t2(x[k], ref), p = __builtin_amdgcn_exp2f(d);
                         s += p;
                         t = fmaf(p, fmaxf(d, -1e30f), t);
                     }
@@ -847,7 +873,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                 }
             }
         }
-        a.join_wave(sc.inv_t2);
+        a.join_wave(diff);
         if constexpr (ROW_WAVES == 1) {
             if constexpr (TOP) best.sort();
             finish_row(sc, r, given, a, best, out);
@@ -862,7 +888,7 @@ __global__ __launch_bounds__(BLOCK) void k_log_probs_long(Scores<T> sc, Actions 
                     o.m = lds[w][0];
                     o.s = lds[w][1];
                     o.t = lds[w][2];
-                    a.join(o, sc.inv_t2);
+                    a.join(o, diff);
                     if constexpr (TOP)
                         for (int c = 0; c < lds_count[w]; c += 64) best.offer(c + lane < lds_count[w] ? lds_keys[w][c + lane] : 0);
                 }
@@ -883,6 +909,7 @@ template <typename T>
 __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions actions, LogProbOut out, int parts, Partials from) {
     __shared__ uint64_t lds_keys[Top::CAPACITY];
     const int lane = threadIdx.x, top = out.top;
+    const Difference diff(sc);
     for (int64_t r = blockIdx.x; r < sc.rows; r += gridDim.x) {
         const uint64_t *keys = from.keys + r * parts * top;
         const float *sums = from.sums + r * parts * 4;
@@ -893,9 +920,9 @@ __global__ __launch_bounds__(64) void k_log_probs_join(Scores<T> sc, Actions act
             o.m = sums[p * 4];
             o.s = sums[p * 4 + 1];
             o.t = sums[p * 4 + 2];
-            a.join(o, sc.inv_t2);
+            a.join(o, diff);
         }
-        a.join_wave(sc.inv_t2);
+        a.join_wave(diff);
         Top best(lds_keys, top ? top : 1);
         if (top) {
             for (int c0 = 0; c0 < parts * top; c0 += 512) {          // eight keys a lane at a time
@@ -934,12 +961,13 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
     using L = Tile<T, ROW_WAVES, U>;
     constexpr int ROWS = WAVES / ROW_WAVES;
     const int n = (int)sc.n;
+    const Difference diff(sc);
     for (int64_t r = (int64_t)blockIdx.y * ROWS + (ROW_WAVES == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0); r < sc.rows;
          r += (int64_t)gridDim.y * ROWS) {
         const Row<T> row(sc, r);
         // (the row's own values are asked for before its scores: they come in that order, and 1024 x 104976 bf16 takes 66 us, the other way round 76)
         const int64_t a = actions.at(r);
-        const float ref = stats[2 * r], log2_s = stats[2 * r + 1], h = entropy[r];
+        const float unit_ref = diff.unit * stats[2 * r], log2_s = stats[2 * r + 1], h = entropy[r];
         const float gl = up.to_log_prob(r, a, n), gh = up.to_entropy(r);
         // dx = p (c0 + c1 log2 p), and g_lp / T more at j = a
         const float c0 = -(gl + gh * h) * sc.inv_t, c1 = -gh * (float)LN_2 * sc.inv_t;
@@ -956,12 +984,12 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
             T v[L::V];
 #pragma unroll
             for (int k = 0; k < L::V; k++) {
-                const float l2 = fmaf(x[u * L::V + k] - ref, sc.inv_t2, -log2_s);
+                const float l2 = fmaf(diff(x[u * L::V + k], unit_ref), diff.per_t2, -log2_s);
                 v[k] = from_f32<T>(__builtin_amdgcn_exp2f(l2) * fmaf(c1, fmaxf(l2, LEAST_LOG2), c0));
             }
             if (j < n) Pieces<T, L::V, 1>::store(to, (int)j, n, false, v, stream);
             if (a >= j && a < j + L::V && a < n) {          // (the lane that has just written this place)
-                const float xa = row.at(a), l2 = fmaf(xa - ref, sc.inv_t2, -log2_s);
+                const float xa = row.at(a), l2 = fmaf(diff(xa, unit_ref), diff.per_t2, -log2_s);
                 to[a] = from_f32<T>(xa == NEG_INF ? 0.0f : fmaf(__builtin_amdgcn_exp2f(l2), fmaf(c1, fmaxf(l2, LEAST_LOG2), c0), gl * sc.inv_t));
             }
         }
@@ -1185,8 +1213,7 @@ int check_scores(int dtype, const void *logits, int64_t rows, int64_t n, int64_t
 
 template <typename T>
 Scores<T> scores(const void *logits, int64_t rows, int64_t n, int64_t row_stride, const uint8_t *mask, int64_t mask_row_stride, double temperature) {
-    return {(const T *)logits, mask, rows, n, row_stride, mask_row_stride, (float)(1.0 / temperature),
-            (float)(LOG2_E / temperature), LOG2_E / temperature};
+    return {(const T *)logits, mask, rows, n, row_stride, mask_row_stride, (float)(1.0 / temperature), (float)(LOG2_E / temperature), LOG2_E / temperature};
 }
 
 // a grid of at most 2^32 work items; the kernels go on from there in strides of the grid (its last dimension)
@@ -1358,12 +1385,12 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
         const Partials partials{(uint64_t *)workspace, workspace ? (float *)((uint64_t *)workspace + rows * sp.parts * top) : nullptr};
         if (sp.row_waves == 1)
             return launch(top ? k_log_probs_long<T, true, 1, false> : k_log_probs_long<T, false, 1, false>, (rows + WAVES - 1) / WAVES, BLOCK, stream,
-                          sc, given, out, 0, partials);
+                          sc, given, out, 0, partials, Difference(sc));
         if (sp.parts == 1)
             return launch(top ? k_log_probs_long<T, true, WAVES, false> : k_log_probs_long<T, false, WAVES, false>, rows, BLOCK, stream, sc, given,
-                          out, 0, partials);
+                          out, 0, partials, Difference(sc));
         if (const int rc = launch(top ? k_log_probs_long<T, true, WAVES, true> : k_log_probs_long<T, false, WAVES, true>,
-                                  dim3((unsigned)sp.parts, (unsigned)rows), BLOCK, stream, sc, given, out, sp.part_tiles, partials))
+                                  dim3((unsigned)sp.parts, (unsigned)rows), BLOCK, stream, sc, given, out, sp.part_tiles, partials, Difference(sc)))
             return rc;
         return launch(k_log_probs_join<T>, rows, 64, stream, sc, given, out, sp.parts, partials);
     });

@@ -157,3 +157,49 @@ def test_sums_of_long_rows_are_as_close_as_their_additions(n, rows, dtype):
             if rows > 1:
                 assert np.abs(got_lp[1::2] - lp[0, n - 1]).max() <= tol_lp(d), (ahead, np.abs(got_lp[1::2] - lp[0, n - 1]).max() / U, A)
             assert np.abs(got_h - h[0]).max() <= tol_h, (ahead, np.abs(got_h - h[0]).max(), tol_h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('n,rows', [(18, 13), (324, 13), (1500, 13), (2500, 13), (6000, 13), (9000, 2100), (60000, 7), (20000, 4096)])
+def test_scores_further_apart_than_the_largest_number(n, rows, dtype):
+    """3e38 and -3e38 are 6e38 apart, which fp32 does not hold; over a temperature of 1e37 they are 60 apart, and both are open."""
+    import torch
+    import magical_amd as m
+    temperature = 1e37
+    rng = np.random.RandomState(n)
+    base = (rng.rand(13, n) * 2 - 1) * 3.3e38
+    base[0, : n // 2], base[0, n // 2:] = -3.3e38, 3.3e38
+    base[1] = -3.3e38
+    base[1, n // 3] = 3.3e38
+    x = torch.tensor(base).to(_torch_type(dtype))
+    x64 = x.double().numpy()
+    is_open, lp, h, _ = oracle(x64, None, temperature)
+    actions = rng.randint(0, n, 13)
+    actions[:2] = 0
+    g_lp, g_h = (rng.randn(13) * 1e37).astype(np.float32), (rng.randn(13) * 1e36).astype(np.float32)
+    rep = lambda v: torch.as_tensor(v)[torch.arange(rows) % 13].cuda()      # noqa: E731
+    k = min(rows, 13)
+    leaf = rep(x).requires_grad_(True)
+    top = min(n, 9)
+    out = m.action_log_probs(leaf, rep(actions), temperature=temperature, top=top)
+    d = (x64.max(1, keepdims=True) - x64) / temperature
+    got = out.log_prob.detach().double().cpu().numpy()[:k]
+    at = np.arange(k)
+    assert np.all(np.abs(got - lp[at, actions[:k]]) <= err_log_prob(d[at, actions[:k]], n))
+    assert np.all(np.abs(out.entropy.detach().double().cpu().numpy()[:k] - h[:k]) <= err_entropy(n))
+    best = np.argsort(-x64, axis=1, kind='stable')[:k, :top]
+    assert np.array_equal(out.top_actions.cpu().numpy()[:k], best)
+    want = np.take_along_axis(lp[:k], best, 1)
+    assert np.all(np.abs(out.top_log_probs.double().cpu().numpy()[:k] - want) <= err_log_prob(np.take_along_axis(d[:k], best, 1), n))
+    grad, = torch.autograd.grad((out.log_prob, out.entropy), leaf, (rep(g_lp), rep(g_h)))
+    gl64, gh64 = g_lp.astype(np.float64), g_h.astype(np.float64)
+    want = oracle_grad(is_open, lp, h, actions, gl64, gh64, temperature)
+    bound = grad_bound(is_open, lp, h, gl64, gh64, want, temperature, torch.finfo(x.dtype).eps, 0.0)
+    assert np.all(np.abs(grad.double().cpu().numpy()[:k] - want[:k]) <= bound[:k])
+    drawn = m.sample_actions(leaf.detach(), torch.full((rows,), 0.5, device='cuda'), temperature=temperature)
+    a = drawn.action.cpu().numpy()[:k]
+    assert np.all(np.abs(drawn.log_prob.double().cpu().numpy()[:k] - lp[at, a]) <= U * np.abs(lp[at, a]) + 1e-6 * U)
+    if rows > 13:
+        for t in list(out) + [grad, drawn.action]:
+            assert torch.equal(t, t[:13][torch.arange(rows, device='cuda') % 13])
