@@ -1381,7 +1381,8 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
                                   given, top, log_prob, entropy, top_log_probs, top_actions);
             });
         const Split sp = split<T>(rows, n);
-        const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_actions, top};
+        // (shorter rows whose alternatives take this way: the backward call has no use for statistics, and their memory need not be there)
+        const LogProbOut out{log_prob, entropy, mgx_policy_stats_bytes(rows, n) ? stats : nullptr, top_log_probs, top_actions, top};
         const Partials partials{(uint64_t *)workspace, workspace ? (float *)((uint64_t *)workspace + rows * sp.parts * top) : nullptr};
         if (sp.row_waves == 1)
             return launch(top ? k_log_probs_long<T, true, 1, false> : k_log_probs_long<T, false, 1, false>, (rows + WAVES - 1) / WAVES, BLOCK, stream,

@@ -203,3 +203,28 @@ def test_scores_further_apart_than_the_largest_number(n, rows, dtype):
     if rows > 13:
         for t in list(out) + [grad, drawn.action]:
             assert torch.equal(t, t[:13][torch.arange(rows, device='cuda') % 13])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype,n,top', [(0, 1000, 0), (0, 2048, 3), (2, 400, 20), (1, 1500, 0)])
+def test_statistics_that_the_backward_call_does_not_need_are_not_written(dtype, n, top):
+    """mgx_policy_stats_bytes() is 0 for these rows: whatever pointer is given, nothing belongs to the call behind it."""
+    import ctypes
+    import torch
+    from magical_amd import _native
+    L = _native.lib()
+    rows = 6
+    assert L.mgx_policy_stats_bytes(rows, n) == 0
+    x = torch.randn(rows, n, device='cuda').to([torch.float32, torch.float16, torch.bfloat16][dtype])
+    a = torch.zeros(rows, dtype=torch.int32, device='cuda')
+    lp, h = torch.empty(rows, device='cuda'), torch.empty(rows, device='cuda')
+    t_lp, t_a = torch.empty(rows * max(top, 1), device='cuda'), torch.empty(rows * max(top, 1), dtype=torch.int32, device='cuda')
+    ws = torch.empty(max(16, L.mgx_policy_workspace_bytes(0, dtype, rows, n, top)), dtype=torch.uint8, device='cuda')
+    guard = torch.full((2 * rows,), 7.0, device='cuda')          # (another's memory)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())      # noqa: E731
+    rc = L.mgx_policy_log_probs(0, dtype, p(x), rows, n, n, None, 0, 1.0, p(a), 4, top, p(lp), p(h), p(guard), p(t_lp), p(t_a), p(ws), ws.numel(),
+                                ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert torch.isfinite(lp).all() and torch.isfinite(h).all()
+    assert (guard == 7).all()
