@@ -168,10 +168,10 @@ def replay_demos(demo_dicts, device='cuda:0', preproc=None, policy=None, **env_k
                 scores[idx] = env.score_on_end_of_traj(env.get_poses(idx))
         out = {'scores': scores, 'recorded_scores': np.array([float(d.get('score', np.nan)) for d in demo_dicts]), 'final_obs': obs}
         if policy is not None:
-            columns = {'log_probs': [j.log_prob for j in judged], 'entropies': [j.entropy for j in judged],
-                       'best_actions': [j.top_actions[:, 0] for j in judged]}
-            for key, steps in columns.items():
-                whole = torch.stack(steps).cpu().numpy()
+            columns = {'log_probs': ([j.log_prob for j in judged], np.float32), 'entropies': ([j.entropy for j in judged], np.float32),
+                       'best_actions': ([j.top_actions[:, 0] for j in judged], np.int32)}
+            for key, (steps, kind) in columns.items():
+                whole = torch.stack(steps).cpu().numpy() if steps else np.zeros((0, n), kind)
                 out[key] = [whole[:len(tape), k].copy() for k, tape in enumerate(tapes)]
         return out
     finally:

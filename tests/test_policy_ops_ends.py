@@ -228,3 +228,16 @@ def test_statistics_that_the_backward_call_does_not_need_are_not_written(dtype, 
     torch.cuda.synchronize()
     assert torch.isfinite(lp).all() and torch.isfinite(h).all()
     assert (guard == 7).all()
+
+
+@pytest.mark.gpu
+def test_a_policy_scored_on_demonstrations_without_actions():
+    import torch
+    from magical_amd import saved_trajectories as st
+    demos = [{'env_name': 'MoveToCorner-Demo-v0', 'score': 0.0,
+              'trajectory': st.MAGICALTrajectory(acts=np.zeros(0, dtype=np.int64), obs={}, rews=np.zeros(0), infos=None)} for _ in range(2)]
+    plain = st.replay_demos(demos, preproc='LoRes4E')
+    out = st.replay_demos(demos, preproc='LoRes4E', policy=lambda obs: torch.zeros(2, 18, device='cuda'))
+    assert np.array_equal(out['scores'], plain['scores'])
+    for key, kind in (('log_probs', np.float32), ('entropies', np.float32), ('best_actions', np.int32)):
+        assert [v.shape for v in out[key]] == [(0,), (0,)] and all(v.dtype == kind for v in out[key])
