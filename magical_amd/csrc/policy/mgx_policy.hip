@@ -1188,6 +1188,8 @@ __global__ __launch_bounds__(BLOCK) void k_draw(Scores<T> sc, const void *unifor
 
 thread_local char g_err[256] = "";          // (no allocation: nothing may throw across the C boundary)
 int fail(int code, const char *msg) { snprintf(g_err, sizeof g_err, "%s", msg); return code; }
+// an error of HIP's: reported here, and not again by the next call, another library's, that asks for the last one
+int fail_hip(const char *msg) { (void)hipGetLastError(); return fail(MGX_ERR_HIP, msg); }
 
 // the caller's current device is left as it was
 struct DeviceGuard {
@@ -1223,7 +1225,7 @@ template <typename... P, typename... A> int launch_lds(void (*kernel)(P...), dim
     const int64_t most = 0xffffffffLL / threads;
     if (blocks.y > most / blocks.x) blocks.y = (unsigned)(most / blocks.x);
     const hipError_t err = hipLaunchKernel((const void *)kernel, blocks, dim3(threads), ptrs, (size_t)lds, (hipStream_t)stream);
-    return err == hipSuccess ? (int)MGX_OK : fail(MGX_ERR_HIP, hipGetErrorString(err));
+    return err == hipSuccess ? (int)MGX_OK : fail_hip(hipGetErrorString(err));
 }
 template <typename... P, typename... A> int launch(void (*kernel)(P...), dim3 blocks, int threads, void *stream, A... args) {
     return launch_lds(kernel, blocks, threads, 0, stream, args...);
@@ -1369,7 +1371,7 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
         if (!workspace || workspace_bytes < need) return fail(MGX_ERR_ARG, "workspace: smaller than mgx_policy_workspace_bytes()");
     if (!actions || !log_prob || !entropy || (top && (!top_log_probs || !top_actions))) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
-    if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
+    if (!guard.ok) return fail_hip("hipSetDevice failed");
     const Actions given{actions, action_bytes};
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
@@ -1408,7 +1410,7 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
     if (rows == 0) return MGX_OK;
     if (!actions || (!stats && mgx_policy_stats_bytes(rows, n)) || !entropy || !grad) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
-    if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
+    if (!guard.ok) return fail_hip("hipSetDevice failed");
     const Actions given{actions, action_bytes};
     const bool stream_out = rows * n * (dtype == MGX_REAL_F32 ? 4 : 2) >= STREAM_BYTES;
     const Upstream up{grad_log_prob, grad_entropy, grad_log_prob_stride, grad_entropy_stride};
@@ -1447,7 +1449,7 @@ int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, i
         if (!workspace || workspace_bytes < need) return fail(MGX_ERR_ARG, "workspace: smaller than mgx_policy_workspace_bytes()");
     if (!uniforms || !action) return fail(MGX_ERR_ARG, "NULL argument");
     DeviceGuard guard(device);
-    if (!guard.ok) return fail(MGX_ERR_HIP, "hipSetDevice failed");
+    if (!guard.ok) return fail_hip("hipSetDevice failed");
     const Drawn out{action, log_prob, entropy};
     return by_dtype(dtype, [&](auto v) {
         using T = decltype(v);

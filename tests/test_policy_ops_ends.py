@@ -241,3 +241,26 @@ def test_a_policy_scored_on_demonstrations_without_actions():
     assert np.array_equal(out['scores'], plain['scores'])
     for key, kind in (('log_probs', np.float32), ('entropies', np.float32), ('best_actions', np.int32)):
         assert [v.shape for v in out[key]] == [(0,), (0,)] and all(v.dtype == kind for v in out[key])
+
+
+@pytest.mark.gpu
+def test_a_refused_device_is_no_error_of_the_next_call():
+    """The C call says what it could not do; nothing of it is left for somebody else's call to report."""
+    import ctypes
+    import torch
+    from magical_amd import _native
+    L = _native.lib()
+    x, a = torch.randn(6, 18, device='cuda'), torch.zeros(6, dtype=torch.int32, device='cuda')
+    lp, h = torch.empty(6, device='cuda'), torch.empty(6, device='cuda')
+    torch.cuda.synchronize()
+    p = lambda t: ctypes.c_void_p(t.data_ptr())      # noqa: E731
+    scores = [99, 0, p(x), 6, 18, 18, None, 0, 1.0]          # (there is no device 99)
+    for call in (lambda: L.mgx_policy_log_probs(*scores, p(a), 4, 0, p(lp), p(h), None, None, None, None, 0, None),
+                 lambda: L.mgx_policy_log_probs_backward(*scores, p(a), 4, None, p(h), None, 0, None, 0, p(x), None),
+                 lambda: L.mgx_policy_sample(*scores, p(lp), 4, p(a), None, None, None, 0, None)):
+        assert call() == -4          # MGX_ERR_HIP
+        assert L.mgx_policy_last_error() == b'hipSetDevice failed'
+        before = x.sum()
+        y = x + 1
+        torch.cuda.synchronize()
+        assert torch.equal((y - x).round(), torch.ones_like(x)) and torch.equal(x.sum(), before) and torch.cuda.current_device() == 0
