@@ -7,6 +7,7 @@
 #include <ATen/ExpandUtils.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -15,6 +16,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -46,6 +48,14 @@ struct MgxError : torch::PyTorchError {       // raised as magical_amd._native.M
 void check(int rc) {
     if (rc < 0) throw MgxError("mgx error " + std::to_string(rc) + ": " + C.last_error());
 }
+
+// A tangent would not come out at the other end, and nobody would know: refused.  (Without tangents in the process: one look at a pointer.)
+void refuse_tangent(const Tensor &t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t.defined() || !t._fw_grad(0).defined(),
+                                "action_log_probs has no forward-mode derivative");
+}
+// In torch.jit.trace the results would become constants.
+void refuse_tracing() { TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "the operators on action scores cannot be traced"); }
 
 // what lies in memory behind a tensor is its values (no negation put off, no zeros without memory)
 Tensor plain(const Tensor &t) { return t._is_zerotensor() ? t.clone() : t.is_neg() ? t.resolve_neg() : t; }
@@ -154,6 +164,8 @@ struct LogProbsBackward : torch::autograd::Node {
     variable_list apply(variable_list &&grads) override {
         variable_list out(1);
         if (!grads[0].defined() && !grads[1].defined()) return out;
+        refuse_tangent(grads[0]);
+        refuse_tangent(grads[1]);
         std::lock_guard<std::mutex> lock(mutex_);
         const Tensor x = logits.unpack(), a = actions.unpack(), m = mask.unpack(), st = stats.unpack(), h = entropy.unpack(shared_from_this());
         const bool differentiated = at::GradMode::is_enabled();
@@ -217,12 +229,15 @@ Forward forward_with_graph(const Tensor &logits, const Tensor &actions, const Op
 py::object or_none(const Tensor &t) { return t.defined() ? py::cast(t) : py::none(); }
 
 py::tuple log_probs(const Tensor &logits, const Tensor &actions, const OptTensor &mask, double temperature, int64_t top) {
+    refuse_tangent(logits);
+    refuse_tracing();
     const Forward f = at::GradMode::is_enabled() && logits.requires_grad() ? forward_with_graph(logits, actions, mask, temperature, top)
                                                                            : forward(logits, actions, mask, temperature, top, false);
     return py::make_tuple(f.log_prob, f.entropy, or_none(f.top_log_probs), or_none(f.top_actions));
 }
 
 py::tuple sample(const Tensor &logits, const Tensor &uniforms, const OptTensor &mask, double temperature) {
+    refuse_tracing();
     const Scores s(logits, mask, temperature);
     const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
     TORCH_CHECK_TYPE(uniforms.scalar_type() == at::kFloat || uniforms.scalar_type() == at::kDouble,

@@ -52,14 +52,15 @@ def action_log_probs(logits, actions, *, mask=None, temperature=1.0, top=0):
     logits [..., n]; actions int32 / int64 [...]: a negative one marks a row in which none is given (a padded step: log probability 0,
     no gradient through it; entropy and alternatives are still there), one >= n gives NaN, and NaN as gradient unless nothing flows
     back through its log probability.  top: 0 ... min(n, 64).
-    Differentiable to the logits through log_prob and entropy (once); the gradient has the logits' type and is 0 wherever an action is
-    not open.  Returns ActionLogProbs.  Refuses wrong types (TypeError), shapes, devices and ranges (ValueError)."""
+    Differentiable to the logits through log_prob and entropy (once, backwards; logits or upstream gradients with a forward-mode tangent
+    are refused, NotImplementedError); the gradient has the logits' type and is 0 wherever an action is not open.  Returns ActionLogProbs.
+    Refuses wrong types (TypeError), shapes, devices and ranges (ValueError), and to be traced (torch.jit.trace: NotImplementedError)."""
     return ActionLogProbs(*_ops.log_probs(logits, actions, mask, temperature, top))
 
 
 def sample_actions(logits, uniforms, *, mask=None, temperature=1.0):
     """One action per row, drawn from softmax(logits / temperature) by the given random numbers: the first action j with
     p_0 + ... + p_j > u, the sums in 64 bits, so that it does not depend on how they are split.  uniforms: float32 / float64 [...] in
-    [0, 1), one a row (`torch.rand`); numbers outside are taken as the nearest end.  Returns SampledActions (no gradient: for that,
-    give the drawn actions to `action_log_probs`).  Refusals are those of `action_log_probs`."""
+    [0, 1), one a row (`torch.rand`); numbers outside are taken as the nearest end.  Returns SampledActions (no gradient, of any mode: for
+    that, give the drawn actions to `action_log_probs`).  Other refusals are those of `action_log_probs`."""
     return SampledActions(*_ops.sample(logits, uniforms, mask, temperature))

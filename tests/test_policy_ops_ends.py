@@ -264,3 +264,43 @@ def test_a_refused_device_is_no_error_of_the_next_call():
         y = x + 1
         torch.cuda.synchronize()
         assert torch.equal((y - x).round(), torch.ones_like(x)) and torch.equal(x.sum(), before) and torch.cuda.current_device() == 0
+
+
+def test_what_would_drop_a_derivative_or_bake_a_result_in_is_refused():
+    """Forward-mode tangents do not come out at the other end; traced, the results would be constants."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+    import magical_amd as m
+    x, a, u = torch.zeros(3, 18), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match='forward'):
+            m.action_log_probs(dual, a)
+        with pytest.raises(NotImplementedError, match='forward'):
+            m.action_log_probs(dual.requires_grad_(True), a)
+    for call in (lambda x: m.action_log_probs(x, a).log_prob, lambda x: m.sample_actions(x, u).log_prob):
+        with pytest.raises(NotImplementedError, match='trac'):
+            torch.jit.trace(call, (x,))
+
+
+@pytest.mark.gpu
+def test_forward_mode_on_the_gpu():
+    import torch
+    import torch.autograd.forward_ad as fwd
+    import magical_amd as m
+    x, a = torch.randn(3, 18, device='cuda'), torch.zeros(3, dtype=torch.int64, device='cuda')
+    want = m.action_log_probs(x, a).log_prob
+    leaf = x.clone().requires_grad_(True)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match='forward'):
+            m.action_log_probs(dual, a)
+        # tangents of the upstream gradients would be lost just so
+        out = m.action_log_probs(leaf, a).log_prob
+        with pytest.raises(NotImplementedError, match='forward'):
+            torch.autograd.grad(out, leaf, fwd.make_dual(torch.ones(3, device='cuda'), torch.ones(3, device='cuda')))
+        # a draw has no derivative, of any mode; where tangents are switched off there is none to lose
+        assert (m.sample_actions(dual, torch.zeros(3, device='cuda')).action >= 0).all()
+        with fwd._set_fwd_grad_enabled(False):
+            assert torch.equal(m.action_log_probs(dual, a).log_prob, want)
+    assert torch.equal(m.action_log_probs(x, a).log_prob, want)
