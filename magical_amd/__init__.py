@@ -19,6 +19,7 @@ from magical_amd.benchmarks import (ALL_REGISTERED_ENVS, AVAILABLE_PREPROCESSORS
 from magical_amd.reference_demos import try_download_demos  # noqa: F401
 from magical_amd.saved_trajectories import (load_demos, preprocess_demos_with_wrapper,  # noqa: F401
                                             splice_in_preproc_name)
+from magical_amd.policy import ActionLogProbs, SampledActions, action_log_probs, sample_actions  # noqa: F401
 from magical_amd.version import __version__  # noqa: F401
 
 # (magical/__init__.py:2-8 exports exactly: ALL_REGISTERED_ENVS, AVAILABLE_PREPROCESSORS, DEMO_ENVS_TO_TEST_ENVS_MAP, register_envs,
@@ -27,12 +28,3 @@ __all__ = ['DEMO_ENVS_TO_TEST_ENVS_MAP', 'register_envs', 'make', 'EnvName', 'AL
            'AVAILABLE_PREPROCESSORS', 'update_magical_env_name', 'try_download_demos', 'load_demos',
            'preprocess_demos_with_wrapper', 'splice_in_preproc_name', '__version__',
            'ActionLogProbs', 'SampledActions', 'action_log_probs', 'sample_actions']
-
-
-def __getattr__(name):
-    """The operators on a policy's action scores (magical_amd/policy.py), looked up when asked for: that module needs torch, which the
-    rest of the package imports with the first env."""
-    if name in ('ActionLogProbs', 'SampledActions', 'action_log_probs', 'sample_actions'):
-        from magical_amd import policy
-        return getattr(policy, name)
-    raise AttributeError(f'module {__name__!r} has no attribute {name!r}')

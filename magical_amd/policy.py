@@ -20,29 +20,37 @@ on the same leaves (a logits tensor, a network's weights) and the default stream
 capture, which it cannot be, and end the process.  Where the logits are such a leaf themselves the call is refused (MgxError); a network's
 weights are for the caller to see to.
 """
-from typing import NamedTuple, Optional
-
-import torch
+from typing import TYPE_CHECKING, NamedTuple, Optional
 
 from . import _native as nat
+
+if TYPE_CHECKING:                # (the package is imported without torch, which comes with the first env or call)
+    import torch
 
 __all__ = ['ActionLogProbs', 'SampledActions', 'action_log_probs', 'sample_actions', 'MAX_TOP']
 
 MAX_TOP = 64                     # MGX_POLICY_MAX_TOP
-_ops = nat.policy_ops()          # csrc/policy/mgx_policy_torch.cpp: argument checks, outputs, autograd, the C calls
+_ops = None                      # csrc/policy/mgx_policy_torch.cpp: argument checks, outputs, autograd, the C calls; loaded by the first call
+
+
+def _load():
+    global _ops
+    import torch  # noqa: F401  (the module's types are torch's)
+    _ops = nat.policy_ops()
+    return _ops
 
 
 class ActionLogProbs(NamedTuple):
-    log_prob: torch.Tensor                    # f32 [...]: log p of the given action
-    entropy: torch.Tensor                     # f32 [...]
-    top_log_probs: Optional[torch.Tensor]     # f32 [..., top], best first (None if top == 0); no gradient
-    top_actions: Optional[torch.Tensor]       # i32 [..., top]; -1 where a row has no more open actions
+    log_prob: 'torch.Tensor'                    # f32 [...]: log p of the given action
+    entropy: 'torch.Tensor'                     # f32 [...]
+    top_log_probs: Optional['torch.Tensor']     # f32 [..., top], best first (None if top == 0); no gradient
+    top_actions: Optional['torch.Tensor']       # i32 [..., top]; -1 where a row has no more open actions
 
 
 class SampledActions(NamedTuple):
-    action: torch.Tensor       # i32 [...]; -1 where nothing is open
-    log_prob: torch.Tensor     # f32 [...]
-    entropy: torch.Tensor      # f32 [...]
+    action: 'torch.Tensor'       # i32 [...]; -1 where nothing is open
+    log_prob: 'torch.Tensor'     # f32 [...]
+    entropy: 'torch.Tensor'      # f32 [...]
 
 
 def action_log_probs(logits, actions, *, mask=None, temperature=1.0, top=0):
@@ -55,7 +63,7 @@ def action_log_probs(logits, actions, *, mask=None, temperature=1.0, top=0):
     Differentiable to the logits through log_prob and entropy (once, backwards; logits or upstream gradients with a forward-mode tangent
     are refused, NotImplementedError); the gradient has the logits' type and is 0 wherever an action is not open.  Returns ActionLogProbs.
     Refuses wrong types (TypeError), shapes, devices and ranges (ValueError), and to be traced (torch.jit.trace: NotImplementedError)."""
-    return ActionLogProbs(*_ops.log_probs(logits, actions, mask, temperature, top))
+    return ActionLogProbs(*(_ops or _load()).log_probs(logits, actions, mask, temperature, top))
 
 
 def sample_actions(logits, uniforms, *, mask=None, temperature=1.0):
@@ -63,4 +71,4 @@ def sample_actions(logits, uniforms, *, mask=None, temperature=1.0):
     p_0 + ... + p_j > u, the sums in 64 bits, so that it does not depend on how they are split.  uniforms: float32 / float64 [...] in
     [0, 1), one a row (`torch.rand`); numbers outside are taken as the nearest end.  Returns SampledActions (no gradient, of any mode: for
     that, give the drawn actions to `action_log_probs`).  Other refusals are those of `action_log_probs`."""
-    return SampledActions(*_ops.sample(logits, uniforms, mask, temperature))
+    return SampledActions(*(_ops or _load()).sample(logits, uniforms, mask, temperature))

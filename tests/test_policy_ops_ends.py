@@ -304,3 +304,19 @@ def test_forward_mode_on_the_gpu():
         with fwd._set_fwd_grad_enabled(False):
             assert torch.equal(m.action_log_probs(dual, a).log_prob, want)
     assert torch.equal(m.action_log_probs(x, a).log_prob, want)
+
+
+def test_a_star_import_needs_neither_torch_nor_the_library():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ('from magical_amd import *\nimport sys, magical_amd\nassert "torch" not in sys.modules\nmake, register_envs\n'
+            'assert action_log_probs is magical_amd.action_log_probs is magical_amd.policy.action_log_probs and SampledActions and sample_actions\n'
+            'import torch\n'
+            'try:\n    action_log_probs(torch.zeros(2, 18), torch.zeros(2, dtype=torch.int64))\n'
+            'except magical_amd._native.MgxError as e:\n    assert "not built" in str(e) or "not found" in str(e), e\n'
+            'else:\n    raise AssertionError\n')
+    env = dict(os.environ, MGX_LIB_PATH='/nonexistent/libmagical_hip.so')
+    run = subprocess.run([sys.executable, '-c', code], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
