@@ -81,7 +81,7 @@ def build(force=False, verbose=False, defines=(), out=None, extra=()):
         failed = [cmd for cmd, job in jobs if job.wait() != 0]
         if failed:
             raise subprocess.CalledProcessError(1, failed[0])
-        link = ['hipcc', '--offload-arch=gfx950', '-shared', '-fPIC', '-pthread', '-o', out or LIB_PATH] + objects
+        link = ['hipcc', '--offload-arch=gfx950', '-shared', '-fPIC', '-pthread', '-o', out or LIB_PATH] + list(extra) + objects
         if verbose:
             print(' '.join(link), flush=True)
         subprocess.check_call(link, cwd=_CSRC)

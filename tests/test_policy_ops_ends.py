@@ -320,3 +320,21 @@ def test_a_star_import_needs_neither_torch_nor_the_library():
     env = dict(os.environ, MGX_LIB_PATH='/nonexistent/libmagical_hip.so')
     run = subprocess.run([sys.executable, '-c', code], cwd=root, env=env, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
+
+
+def test_a_development_builds_flags_reach_the_compiler_and_the_linker(monkeypatch, tmp_path):
+    from magical_amd import _native
+    commands = []
+
+    class Done:
+        def __init__(self, cmd, **kw):
+            commands.append(cmd)
+
+        def wait(self):
+            return 0
+    monkeypatch.setattr(_native.subprocess, 'Popen', Done)
+    monkeypatch.setattr(_native.subprocess, 'check_call', lambda cmd, **kw: commands.append(cmd))
+    _native.build(defines=['MGX_SOME'], out=str(tmp_path / 'lib.so'), extra=['-some-flag'])
+    assert len(commands) == len(_native._SOURCES) + 1
+    assert all('-some-flag' in cmd for cmd in commands)
+    assert all('-DMGX_SOME' in cmd for cmd in commands if '-c' in cmd)
