@@ -16,7 +16,7 @@
  *   - an action that is not open has log p = -inf, takes no part in H and gets gradient 0;
  *   - a row without open actions has log p = -inf for every action, H = 0, no alternatives (-1), gradient 0, and action -1 is drawn;
  *   - a row with a NaN or +inf among the open scores (masked places may hold anything) has NaN for log p, H and the open places'
- *     gradient, no alternatives (-1), and action -1 is drawn.
+ *     gradient (unless nothing flows back into the row), no alternatives (-1), and action -1 is drawn.
  * Sums are held in 32 bits (drawing: in 64), each row's result depends on the row alone and on the rows' number, and repeats bit
  * for bit.
  */
@@ -46,7 +46,8 @@ int mgx_policy_log_probs(int device, int dtype, const void *logits, int64_t rows
                          int64_t workspace_bytes, void *stream);
 /* gradient of sum_r grad_log_prob[r] * log_prob[r] + grad_entropy[r] * entropy[r] to the scores, in their type: grad [rows][n], dense.
  * grad_log_prob / grad_entropy: f32, row r at r * stride (0: one value for all), NULL = zero; the other arguments are the forward
- * call's, stats and entropy its outputs.  A row whose given action is >= n has NaN at its open places, unless its grad_log_prob is 0. */
+ * call's, stats and entropy its outputs.  A row whose given action is >= n has NaN at its open places, unless its grad_log_prob is 0; a row
+ * into which nothing flows back (grad_log_prob 0 or no action given, grad_entropy 0) has gradient 0 whatever its scores. */
 int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride,
                                   const uint8_t *mask, int64_t mask_row_stride, double temperature, const void *actions,
                                   int action_bytes, const float *stats, const float *entropy, const float *grad_log_prob,

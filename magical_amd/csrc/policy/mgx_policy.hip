@@ -477,7 +477,7 @@ template <typename T> struct RowGradient64 {
         : sc(sc_), row(sc_, r), a(actions.at(r)), ref(ref_), log2_s(log2_s_), gl(up.to_log_prob(r, a, sc_.n)), gh(up.to_entropy(r)), h(entropy[r]) {}
     __device__ __forceinline__ T at(int64_t j) const {
         const float x = row.at(j);
-        if (x == NEG_INF) return from_f32<T>(0.0f);
+        if (x == NEG_INF || (gl == 0 && gh == 0)) return from_f32<T>(0.0f);          // (nothing flows back into the row, be its scores what they may)
         // (nothing overflows: the factors are fp32 numbers.  Below 2^-1000 a p makes 0 of them; where it is NaN, so is h)
         const double l2 = ((double)x - ref) * sc.inv_t2_64 - log2_s, factor = (double)gl + (double)gh * (h + l2 * LN_2);
         return from_f32<T>((float)(((j == a ? (double)gl : 0.0) - Exp64(1.0)(fmax(l2, -1000.0)) * factor) * (sc.inv_t2_64 * LN_2)));

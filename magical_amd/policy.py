@@ -58,8 +58,8 @@ def action_log_probs(logits, actions, *, mask=None, temperature=1.0, top=0):
     alternatives of each row (best first, equal logits by the lower index).
 
     logits [..., n]; actions int32 / int64 [...]: a negative one marks a row in which none is given (a padded step: log probability 0,
-    no gradient through it; entropy and alternatives are still there), one >= n gives NaN, and NaN as gradient unless nothing flows
-    back through its log probability.  top: 0 ... min(n, 64).
+    no gradient through it, whatever the row's logits; entropy and alternatives are still there), one >= n gives NaN, and NaN as gradient
+    unless nothing flows back through its log probability.  top: 0 ... min(n, 64).
     Differentiable to the logits through log_prob and entropy (once, backwards; logits or upstream gradients with a forward-mode tangent
     are refused, NotImplementedError); the gradient has the logits' type and is 0 wherever an action is not open.  Returns ActionLogProbs.
     Refuses wrong types (TypeError), shapes, devices and ranges (ValueError), and to be traced (torch.jit.trace: NotImplementedError)."""

@@ -338,3 +338,36 @@ def test_a_development_builds_flags_reach_the_compiler_and_the_linker(monkeypatc
     assert len(commands) == len(_native._SOURCES) + 1
     assert all('-some-flag' in cmd for cmd in commands)
     assert all('-DMGX_SOME' in cmd for cmd in commands if '-c' in cmd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('n,rows', GRADIENT_SHAPES)
+def test_padded_rows_of_nonsense_have_no_gradient(n, rows, dtype):
+    """A row into which nothing flows back -- a padded step whose entropy is not asked for, a row that a loss leaves out -- has gradient 0, whatever its
+    logits: NaN there would reach every weight behind them."""
+    import torch
+    import magical_amd as m
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(rows, n, generator=g)
+    x[0] = float('nan')
+    x[1, n // 2] = float('nan')
+    x[2, 0] = float('inf')
+    x[3, n - 1] = float('nan')
+    x[4, n - 1] = float('nan')
+    actions = torch.randint(0, n, (rows,), generator=g)
+    actions[:3] = -1
+    used = torch.ones(rows, dtype=torch.bool)
+    used[3] = False
+    leaf = x.to(_torch_type(dtype)).cuda().requires_grad_(True)
+    out = m.action_log_probs(leaf, actions.cuda())
+    assert torch.equal(out.log_prob[:3], torch.zeros(3, device='cuda')) and torch.isnan(out.log_prob[3:5]).all() and torch.isnan(out.entropy[:5]).all()
+    used, zero = used.cuda(), torch.zeros((), device='cuda')
+    for with_entropy in (False, True):
+        loss = torch.where(used, out.log_prob, zero).sum()
+        if with_entropy:
+            loss = loss + torch.where(used & (torch.arange(rows, device='cuda') > 2), out.entropy, zero).sum()
+        grad, = torch.autograd.grad(loss, leaf, retain_graph=True)
+        assert (grad[:4] == 0).all() and torch.isnan(grad[4]).all() and torch.isfinite(grad[5:]).all()
+    grad, = torch.autograd.grad(out.log_prob.sum() + out.entropy.sum(), leaf)
+    assert torch.isnan(grad[:5]).all() and torch.isfinite(grad[5:]).all()
