@@ -14,12 +14,15 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
+#include <unordered_set>
+#include <vector>
 
 #include "../../../include/mgx_policy.h"
 
@@ -156,6 +159,48 @@ struct Upstream {
     }
 };
 
+// A gradient arrives on the stream of the forward call that it belongs to, a leaf's on that on which an earlier call first asked for it, as long as
+// results of such calls are alive.  A captured backward pass would have to wait for that stream, and the default stream cannot take part in a
+// capture: torch ends the process.  Refused before: where the logits are such a leaf by the captured forward call, else (a network's weights) by the
+// backward pass, as soon as it gets here, for whatever it is going to reach behind this node.
+bool capturing(c10::Device device) {
+    const c10::DeviceGuard guard(device);
+    return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+bool on_default_stream(torch::autograd::Node &node) {
+    const auto stream = node.stream();
+    return stream && stream->id() == c10::hip::getDefaultHIPStream(stream->device_index()).id();
+}
+void refuse_captured_backward_beside_eager_graph(const torch::autograd::Node &node, c10::Device device) {
+    if (!capturing(device)) return;
+    const auto *reached = torch::autograd::get_current_graph_task_exec_info();          // (none or empty: every node)
+    std::unordered_set<const torch::autograd::Node *> seen;
+    std::vector<const torch::autograd::Node *> left{&node};
+    while (!left.empty()) {
+        const auto *from = left.back();
+        left.pop_back();
+        for (const torch::autograd::Edge &edge : from->next_edges()) {
+            torch::autograd::Node *const to = edge.function.get();
+            if (!to || !seen.insert(to).second) continue;
+            if (reached && !reached->empty()) {
+                const auto it = reached->find(to);
+                if (it == reached->end() || !it->second.should_execute()) continue;
+            }
+            if (on_default_stream(*to))
+                throw MgxError("something behind the logits (a network's weight, the logits themselves) still belongs to results of earlier calls on the "
+                               "default stream: free these results before the forward and the backward pass are captured, both of them");
+            left.push_back(to);
+        }
+    }
+}
+void refuse_capture_beside_eager_graph(const Tensor &logits) {
+    if (!logits.is_leaf() || !logits.is_cuda()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(logits);
+    if (accumulator && on_default_stream(*accumulator) && capturing(logits.device()))
+        throw MgxError("logits that need a gradient still belong to results of earlier calls on the default stream: free these results before this "
+                       "call is captured, or give logits.detach()");
+}
+
 // The backward pass's node.  (A custom Function keeps the same, with a dictionary and checks that cost 2 us a call.)
 struct LogProbsBackward : torch::autograd::Node {
     SavedVariable logits, actions, mask, stats, entropy;
@@ -166,6 +211,7 @@ struct LogProbsBackward : torch::autograd::Node {
         if (!grads[0].defined() && !grads[1].defined()) return out;
         refuse_tangent(grads[0]);
         refuse_tangent(grads[1]);
+        refuse_captured_backward_beside_eager_graph(*this, (grads[0].defined() ? grads[0] : grads[1]).device());
         std::lock_guard<std::mutex> lock(mutex_);
         const Tensor x = logits.unpack(), a = actions.unpack(), m = mask.unpack(), st = stats.unpack(), h = entropy.unpack(shared_from_this());
         const bool differentiated = at::GradMode::is_enabled();
@@ -192,19 +238,6 @@ struct LogProbsBackward : torch::autograd::Node {
     }
     std::string name() const override { return "ActionLogProbsBackward"; }
 };
-
-// A leaf's gradient arrives on the stream on which an earlier call first asked for it, as long as results of such calls are alive.  A captured
-// backward pass would have to wait for that stream, and the default stream cannot take part in a capture: torch ends the process.
-void refuse_capture_beside_eager_graph(const Tensor &logits) {
-    if (!logits.is_leaf()) return;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(logits);
-    if (!accumulator || !logits.is_cuda()) return;
-    const auto earlier = accumulator->stream();
-    if (!earlier || earlier->id() != c10::hip::getDefaultHIPStream(logits.device().index()).id()) return;
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
-        throw MgxError("logits that need a gradient still belong to results of earlier calls on the default stream: free these results before this "
-                       "call is captured, or give logits.detach()");
-}
 
 Forward forward_with_graph(const Tensor &logits, const Tensor &actions, const OptTensor &mask, double temperature, int64_t top) {
     Forward f;

@@ -15,10 +15,10 @@ softmax(logits / temperature), temperature in 1e-37 ... 1e37, over the actions t
 float32 whatever the logits' type.  Rows with nothing open give log probability -inf, entropy 0 and action -1 with gradient 0; rows with NaN
 or +inf among the open logits give NaN and action -1.  Calls run on torch's current stream of the logits' device.
 
-Calls, and the backward pass, can be captured into a HIP graph and replayed.  While a backward pass is captured, no results of earlier calls
-on the same leaves (a logits tensor, a network's weights) and the default stream may be alive: torch would make that stream part of the
-capture, which it cannot be, and end the process.  Where the logits are such a leaf themselves the call is refused (MgxError); a network's
-weights are for the caller to see to.
+Calls, and the backward pass with its forward call, can be captured into a HIP graph and replayed.  While a backward pass is captured, no
+results of earlier calls on the same leaves (a logits tensor, a network's weights) and the default stream may be alive: torch would make that
+stream part of the capture, which it cannot be, and end the process.  Where the backward pass would come to such a leaf by way of these
+operators it is refused (MgxError; where the logits are one themselves, the forward call).
 """
 from typing import TYPE_CHECKING, NamedTuple, Optional
 

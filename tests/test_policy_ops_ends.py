@@ -371,3 +371,45 @@ def test_padded_rows_of_nonsense_have_no_gradient(n, rows, dtype):
         assert (grad[:4] == 0).all() and torch.isnan(grad[4]).all() and torch.isfinite(grad[5:]).all()
     grad, = torch.autograd.grad(out.log_prob.sum() + out.entropy.sum(), leaf)
     assert torch.isnan(grad[:5]).all() and torch.isfinite(grad[5:]).all()
+
+
+@pytest.mark.gpu
+def test_a_captured_backward_pass_beside_an_eager_graph_of_the_weights_is_refused():
+    """Torch would end the process where it comes to a weight that an eager graph still holds; what does not come there goes on."""
+    import gc
+    import torch
+    import magical_amd as m
+    refused = m._native.MgxError
+    g = torch.Generator(device='cuda').manual_seed(0)
+    feats, weight = torch.randn(9, 12, generator=g, device='cuda'), torch.randn(12, 18, generator=g, device='cuda').requires_grad_(True)
+    a = torch.arange(9, device='cuda')
+    alive = m.action_log_probs(feats @ weight, a)
+    logits = feats @ weight
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(refused, match='default stream'):
+            m.action_log_probs(feats @ weight, a).log_prob.sum().backward()
+        with pytest.raises(refused, match='default stream'):
+            torch.autograd.grad(m.action_log_probs(feats @ weight, a).entropy.sum(), weight)
+        with pytest.raises(refused, match='default stream'):          # (a graph whose first half is an eager one)
+            torch.autograd.grad(m.action_log_probs(logits, a).log_prob.sum(), weight)
+        inner = feats @ weight
+        to_logits, = torch.autograd.grad(m.action_log_probs(inner, a).log_prob.sum(), inner)
+    assert weight.grad is None
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+    want, = torch.autograd.grad(alive.log_prob.sum(), weight)
+    leaf = logits.detach().requires_grad_(True)
+    assert torch.equal(to_logits, torch.autograd.grad(m.action_log_probs(leaf, a).log_prob.sum(), leaf)[0])
+    del alive, logits, inner, to_logits
+    gc.collect()          # (what the refusals' tracebacks still hold)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(m.action_log_probs(feats @ weight, a).log_prob.sum(), weight)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
