@@ -413,3 +413,38 @@ def test_a_captured_backward_pass_beside_an_eager_graph_of_the_weights_is_refuse
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_step_policy_with_masks_temperatures_and_generators():
+    import torch
+    import magical_amd as m
+    n_envs = 64
+    env, twin = (m.make('MoveToCorner-Demo-LoRes4E-v0', n_envs=n_envs, device='cuda:0') for _ in range(2))
+    env.reset(), twin.reset()
+    g = torch.Generator(device='cuda').manual_seed(5)
+    logits = torch.randn(n_envs, 18, generator=g, device='cuda') * 2
+    per_env = torch.rand(n_envs, 18, generator=g, device='cuda') < 0.5
+    per_env[3] = False
+    for mask in (None, per_env, per_env[0], per_env.any(1, keepdim=True)):
+        for temperature in (1.0, 0.3, 5.0):
+            for x in (logits, logits.half(), logits.clone().requires_grad_(True)):
+                ours, theirs = torch.Generator(device='cuda').manual_seed(9), torch.Generator(device='cuda').manual_seed(9)
+                obs, _, _, info = env.step_policy(x, mask=mask, temperature=temperature, generator=ours)
+                u = torch.rand(n_envs, generator=theirs, device='cuda')
+                want = m.sample_actions(x, u, mask=mask, temperature=temperature)
+                assert torch.equal(info['action'], want.action) and torch.equal(info['action_log_prob'], want.log_prob)
+                assert torch.equal(info['action_entropy'], want.entropy) and not info['action_log_prob'].requires_grad
+                twin_obs, _, _, _ = twin.step(want.action.clamp(min=0))
+                assert torch.equal(obs, twin_obs)
+                if mask is not None:
+                    full = mask.expand(n_envs, 18)
+                    assert ((info['action'] == -1) == ~full.any(1)).all()
+                    assert full[info['action'] >= 0].gather(1, info['action'][info['action'] >= 0, None].long()).all()
+    for bad in (dict(mask=per_env[:5]), dict(temperature=0.0), dict(uniforms=torch.rand(3, device='cuda'))):
+        with pytest.raises(ValueError):
+            env.step_policy(logits, **bad)
+    with pytest.raises(TypeError):
+        env.step_policy(logits, mask=per_env.float())
+    env.close()
+    twin.close()
