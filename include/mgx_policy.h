@@ -17,8 +17,8 @@
  *   - a row without open actions has log p = -inf for every action, H = 0, no alternatives (-1), gradient 0, and action -1 is drawn;
  *   - a row with a NaN or +inf among the open scores (masked places may hold anything) has NaN for log p, H and the open places'
  *     gradient (unless nothing flows back into the row), no alternatives (-1), and action -1 is drawn.
- * Sums are held in 32 bits (drawing: in 64), each row's result depends on the row alone and on the rows' number, and repeats bit
- * for bit.
+ * Sums are held in 32 bits (drawing: in 64).  Each row's result depends on the row alone, and its last bits on how many rows and alternatives are
+ * asked for, which decides how a row is shared out; it repeats bit for bit.
  */
 #ifndef MGX_POLICY_H
 #define MGX_POLICY_H
@@ -53,7 +53,8 @@ int mgx_policy_log_probs_backward(int device, int dtype, const void *logits, int
                                   int action_bytes, const float *stats, const float *entropy, const float *grad_log_prob,
                                   int64_t grad_log_prob_stride, const float *grad_entropy, int64_t grad_entropy_stride, void *grad,
                                   void *stream);
-/* one action per row: the first j with p_0 + ... + p_j > u, u = uniforms[r] (f32 or f64: uniform_bytes 4 or 8) in [0, 1); a u below 0
+/* one action per row: the first j with p_0 + ... + p_j > u (in 64 bits: only a u within some n * 2^-53 of a border between two actions may fall on
+ * either side of it, by how a row is shared out), u = uniforms[r] (f32 or f64: uniform_bytes 4 or 8) in [0, 1); a u below 0
  * or NaN counts as 0, a u of 1 or more draws the last action that can be drawn.  A probability below 2^-990 is none.  action: i32 [rows]; log_prob, entropy: f32 [rows]
  * (either may be NULL). */
 int mgx_policy_sample(int device, int dtype, const void *logits, int64_t rows, int64_t n, int64_t row_stride, const uint8_t *mask,

@@ -68,7 +68,8 @@ def action_log_probs(logits, actions, *, mask=None, temperature=1.0, top=0):
 
 def sample_actions(logits, uniforms, *, mask=None, temperature=1.0):
     """One action per row, drawn from softmax(logits / temperature) by the given random numbers: the first action j with
-    p_0 + ... + p_j > u, the sums in 64 bits, so that it does not depend on how they are split.  uniforms: float32 / float64 [...] in
-    [0, 1), one a row (`torch.rand`); numbers outside are taken as the nearest end.  Returns SampledActions (no gradient, of any mode: for
-    that, give the drawn actions to `action_log_probs`).  Other refusals are those of `action_log_probs`."""
+    p_0 + ... + p_j > u, the sums in 64 bits (a u within some n * 2^-53 of a border between two actions can fall on either side of it, by the
+    number of rows; a repeated call draws the same).  uniforms: float32 / float64 [...] in [0, 1), one a row (`torch.rand`); numbers outside
+    are taken as the nearest end.  Returns SampledActions (no gradient, of any mode: for that, give the drawn actions to
+    `action_log_probs`).  Other refusals are those of `action_log_probs`."""
     return SampledActions(*(_ops or _load()).sample(logits, uniforms, mask, temperature))
