@@ -14,8 +14,9 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_PKG, 'csrc')
 LIB_PATH = os.environ.get('MGX_LIB_PATH') or os.path.join(_PKG, 'libmagical_hip.so')      # (override: development builds with other -D knobs)
 _SOURCES = ['mgx_api.hip', 'mgx_world.cpp', 'policy/mgx_policy.hip']
-# the operators on action scores are compiled without packed fp32 instructions: some of their forms have given wrong results on this
-# hardware now and then.  (The engine's sources keep their code generation: without them its fp32 results and speed change.)
+# the operators on action scores are compiled without packed fp32 instructions, which the compiler makes of ordinary float code and on some of
+# whose forms no result here is to rest.  (The engine's sources keep their code generation: without them its fp32 trajectories change bits and
+# its headline loses 1.8 %, profiles/policy_ops_kernel_times.txt.)
 _SOURCE_FLAGS = {'policy/mgx_policy.hip': ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
 # ... and their binding to torch tensors, a Python extension module of its own (host code)
 POLICY_OPS_PATH = os.path.join(_PKG, '_policy_torch.so')

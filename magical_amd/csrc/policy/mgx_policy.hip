@@ -1,4 +1,7 @@
 // mgx_policy.hip -- the operators of include/mgx_policy.h: what lies between a policy's action scores and the engine's actions.
+//
+// Times in these comments, unless one says otherwise: of a call among ten of its kind in a captured graph, on the same scores, the median, on an MI355X;
+// scores that fit the 256 MB cache in front of the memory come from there in part.  A copy of 1 GiB moves 5.1 TB/s on it.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,8 +26,8 @@ template <typename T> struct Scores {
     float inv_t, inv_t2;        // 1 / temperature, log2(e) / temperature: exponentials are taken to the base 2, as the hardware does
     double inv_t2_64;
     // Two scores may be further apart than the largest fp32 number (3e38 and -3e38).  Over a T of up to 1e36 their quotient is one whose exponential is 0
-    // all the same; over a larger one the difference is taken of their halves (unit 1 / 2, else 1), in one operation.  (From what is there: two more
-    // arguments cost 983040 x 18 fp32 0.7 us of 17.)
+    // all the same; over a larger one the difference is taken of their halves (unit 1 / 2, else 1), in one operation.  (Told by what is there already:
+    // two more arguments made 983040 x 18 fp32 17.9 us of 17.2.)
     __host__ __device__ __forceinline__ bool by_halves() const { return __builtin_bit_cast(uint32_t, inv_t2) < __builtin_bit_cast(uint32_t, 1.44e-36f); }
     // one score's (v - ref) / T as a result, which is to be finite over smaller T too: always by halves
     __device__ __forceinline__ float over_t(float v, float ref) const { return 2.0f * (fmaf(v, 0.5f, -0.5f * ref) * inv_t); }
@@ -321,9 +324,9 @@ struct Exp64 {
 
 // ---------------------------------------------------------------------------------------------------------------- short rows
 // A row stays in the registers of G lanes (1 ... 64), E scores a lane: one read of the scores, all sums by lane exchanges, no barrier.  What
-// bounds it: memory (983040 x 18 fp32: 16 us where its 86 MB take 17 at a copy's rate; backward 28 where its 161 MB take 31: part of them lies
+// bounds it: memory (983040 x 18 fp32: 17.1 us where its 86 MB take 17 at a copy's rate; backward 27 where its 161 MB take 31: part of them lies
 // in the cache), from some dozen scores a row on the vector unit, which issues some 15 instructions a score, 20 with a mask (61440 x 324 bf16
-// with a mask: 15 us, 12 of them issued, where memory would take 8; backward 25, 16 issued, 16 of memory).  Lane g holds pieces of W
+// with a mask: 15.4 us, 12 of them issued, where memory would take 8; backward 22.8, 16 issued, 16 of memory).  Lane g holds pieces of W
 // neighbouring scores (16 bytes, or 4 scores): x[e] is score place(g, e).
 template <int G, int E, int W> struct Spread {
     static __device__ __forceinline__ int place(int g, int e) { return e / W * (G * W) + g * W + e % W; }
@@ -359,7 +362,7 @@ template <int UNIT> __device__ __forceinline__ void store_run(void *out, const u
 }
 
 // Rows in one lane put their alternatives together in LDS, as k_backward_lane does with the gradients (288296 x 18 fp16, a lane storing its own: 5
-// alternatives 12.4 us, 8 19.6, 18 56; by way of LDS 12.2, 15.9, 27).
+// alternatives 11.9 us, 8 17.9, 18 56; by way of LDS 12.4, 15.9, 28).
 template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_log_probs_short(Scores<T> sc, Actions actions, int top, float *log_prob, float *entropy,
                                                            float *top_log_probs, int32_t *top_actions) {
@@ -464,7 +467,7 @@ struct Upstream {          // gradients to the log probabilities and entropies, 
 // The gradient is p (c0 + c1 log2 p), with log2 p no lower than LEAST_LOG2: p is 0 there in fp32, so is the product, and -inf stays out of it.  That takes
 // moderate c0 and c1: of larger ones (a gradient to the entropy over a tiny temperature) the product with log2 p overflows, and 0 x inf is NaN, or what
 // fp32 has no exponential for is no longer nothing; and NaN has to stay out of the places that are not open.  Rows with such factors are worked out
-// place by place in 64 bits.
+// place by place in 64 bits (983040 x 18 fp32 57 us for 28, 1024 x 104976 bf16 277 for 67).
 constexpr float LEAST_LOG2 = -256.0f, MODERATE = 0x1p40f;
 __device__ __forceinline__ bool moderate(float c0, float c1) { return fabsf(c0) <= MODERATE && fabsf(c1) <= MODERATE; }
 // (All that the row's factors were made of is read again, so that nothing stays in registers for it.)
@@ -528,8 +531,8 @@ __global__ __launch_bounds__(BLOCK) void k_backward_short(Scores<T> sc, Actions 
 }
 
 // Up to 32 scores a row, a lane each.  The gradients of a wavefront's 64 rows are one run of memory: they are put together in LDS and stored in 16-byte
-// vectors, neighbours by neighbours (a lane storing its own row writes 16 bytes every 72: 59 us where this takes 30; four lanes a row, a score
-// a store: 38; 983040 rows of 18 fp32).
+// vectors, neighbours by neighbours (983040 rows of 18 fp32: 28 us; a lane storing its own row writes 16 bytes every 72: 130; four lanes a row, a
+// score a store: 37).
 template <typename T, int G, int E, int W>
 __global__ __launch_bounds__(BLOCK) void k_backward_lane(Scores<T> sc, Actions actions, const float *entropy, Upstream up, T *grad, bool stream) {
     static_assert(G == 1);
@@ -653,10 +656,11 @@ __global__ __launch_bounds__(BLOCK) void k_sample_short(Scores<T> sc, const void
 
 // ----------------------------------------------------------------------------------------------------------------- long rows
 // A wavefront or workgroup goes over a row, or over one part of it where there are few rows, in tiles of U 16-byte vectors a lane: running
-// maximum, sum and weighted sum per lane, joined at the end; every score is read once.  What bounds it: memory (1024 x 104976 bf16: 44 us,
-// 4.9 TB/s; backward 72 us, 6.0 TB/s), with masks and alternatives the vector unit too (4096 x 5832 bf16, a mask, five alternatives: 22 us,
-// 13 of them issued, where memory would take 14), and with few rows two launches (7 x 50021 fp32, 20 alternatives: 8 and 5 us).  Loading the next tile ahead of
-// the present one's arithmetic made it slower (58 -> 64 and 22 -> 28 us): registers, and other wavefronts hide the loads already.
+// maximum, sum and weighted sum per lane, joined at the end; every score is read once.  What bounds it: memory (1024 x 104976 bf16, 215 MB: 37.6 us, part
+// of them from the cache, 43 ... 46 after other work; backward 66, 67 ... 74 after other work, for 430 MB), with masks and alternatives the vector unit
+// too (4096 x 5832 bf16, a mask, five alternatives: 22 us, 13 of them issued, where memory would take 14), and with few rows two launches, each a
+// chain of load, exchange and rank (7 x 50021 fp32, 20 alternatives: 8 and 5 us under the profiler).  Loading the next tile ahead of the present one's
+// arithmetic made it slower when it was tried (58 -> 64 and 22 -> 28 us): registers, and other wavefronts hide the loads already.
 
 // ROW_WAVES: wavefronts that go over the tile together (1, or the workgroup's 4)
 template <typename T, int ROW_WAVES, int VECTORS = 4> struct Tile {
@@ -719,7 +723,7 @@ struct Top {
     __device__ Top(uint64_t *lds, int k_) : keys(lds), k(k_) {}
     // Before the first offers: x are N scores that each lane is going to offer, the best of some each.  The k-th best of these 64 N bounds the
     // k-th best of all from below; found bit by bit (16 of them: the bound may be lower), it keeps most of the scores out that would not last.
-    // For one alternative it is the best of them.  (32768 x 2500 bf16: 52 us, bit by bit 59.)
+    // For one alternative it is the best of them.  (32768 x 2500 bf16: 47 us, bit by bit 54.)
     template <int N> __device__ __forceinline__ void expect(const float (&x)[N]) {
         if (k == 1) {
             const float most = group_max<64>(lane_max(x));
@@ -1006,7 +1010,7 @@ __global__ __launch_bounds__(BLOCK) void k_backward_long(Scores<T> sc, Actions a
 
 // ---- drawing: the row's segments of 64 vectors (one a lane), each with its own maximum and 64-bit sums, then the one segment the target lies in,
 // read once more.  What bounds it: the 64-bit exponentials, 20 instructions each (4096 x 5832 bf16: 28 us, of which the vector unit issues
-// for 21; memory would take 9); with few rows two launches (16 x 104976 fp32: 6 and 6 us).  32 bits would not do: a border between two actions is off by
+// for 21; memory would take 9); with few rows two launches (16 x 104976 fp32: 11.0 us).  32 bits would not do: a border between two actions is off by
 // some 2^-24 there, and with ten thousand actions a random number lies that close to one every thousandth time.
 struct Segment {
     double s, t;        // sums of the exponentials, and of these times their differences to the maximum
@@ -1235,19 +1239,19 @@ template <typename... P, typename... A> int launch(void (*kernel)(P...), int64_t
 }
 
 // Gradients of this size go past the caches: a quarter of the 256 MB that memory has in front of it would be filled with what is read
-// once, much later, and written back while the next kernels read.  1024 x 104976 bf16 (215 MB): backward 84 -> 72 us, and the forward
-// pass after it 58 -> 44; 983040 x 18 fp32 (71 MB): 29.4 -> 28.2 and 20.9 -> 17.2; 61440 x 324 bf16 (40 MB): no difference.
+// once, much later, and written back while the next kernels read.  1024 x 104976 bf16 (215 MB): backward 78 -> 67 us, forward and
+// backward in turn 113 -> 103; 983040 x 18 fp32 (71 MB): 28.2 -> 27.0 and 44.7 -> 44.2; 61440 x 324 bf16 (40 MB): no difference.
 constexpr int64_t STREAM_BYTES = 64 << 20;
 // Rows of up to 2 KB of scores stay in a few lanes' registers.  Measured against a wavefront a row that goes over it in tiles, 65536 rows (log
-// probabilities / with five alternatives / draws, us): 600 bf16 23 / 57 / 84 against 36 / 79 / 116, 1000 bf16 30 / 72 / 105 against 38 / 81 /
-// 116; 1500 bf16 53 / 117 / 170 against 53 / 96 / 151, 1000 fp32 52 / 100 / 151 against 53 / 74 / 118.
+// probabilities / with five alternatives / draws, us): 600 bf16 24 / 58 / 75 against 37 / 75 / 117, 1000 bf16 30 / 73 / 90 against 37 / 76 / 118;
+// longer ones, as they are now, against registers (log probabilities / draws): 1500 bf16 45 / 139 against 44 / 126, 1000 fp32 45 / 108 against 44 / 120.
 template <typename T> constexpr bool is_short(int64_t n) { return n * (int64_t)sizeof(T) <= 2048; }
 // The backward pass, which needs no second look, keeps rows of up to 2048 scores there, and needs nothing of the forward pass for them (65536
-// x 1500: bf16 77 us, fp32 149; in tiles, from the forward pass's statistics, 198 and 217).
+// x 1500: bf16 69 us, fp32 134; in tiles, from the forward pass's statistics, 77 and 168).
 constexpr int BACKWARD_SHORT_MAX = 2048;
 template <int G_, int E_, int W_> struct Shape { static constexpr int G = G_, E = E_, W = W_; };
-// f(lanes a row, scores a lane, scores a load): up to 32 scores in one lane (no exchanges at all: 983040 x 18 fp32 20 us, over four lanes 24;
-// 61 rows 3.4, over four lanes 3.0; drawing 983040 x 18 bf16 38 us, over four lanes 49); beyond, the fewest lanes that hold the row in four
+// f(lanes a row, scores a lane, scores a load): up to 32 scores in one lane (no exchanges at all: 983040 x 18 fp32 17.1 us, over four lanes 23.4;
+// 61 rows 3.1, over four lanes 2.8; drawing 983040 x 18 bf16 32 us, over four lanes 54); beyond, the fewest lanes that hold the row in four
 // pieces of W scores each, or 64 lanes with up to MOST pieces.
 template <int W, int G, int MOST, typename F> int by_pieces(int64_t n, F f) {
     const int64_t c = (n + G * W - 1) / (G * W);
@@ -1286,10 +1290,10 @@ template <typename F> int by_length_32(int64_t n, F f) {
 template <typename T, int LONGEST, typename F> int by_length(int64_t n, F f) {
     return n <= 32 ? by_length_32(n, f) : by_lanes<16 / sizeof(T), LONGEST>(n, f);
 }
-// Drawing for up to 16384 rows, which do not fill the GPU: short rows over four lanes.  (64-bit exponentials one after the other: 4096 x 18 fp32 4.4 us, in
-// one lane 5.2; 65536 x 18 7.2, in one lane 5.6.)
-// Beyond 32 scores, 16 a lane at most, whatever their type: more leave too few registers for two wavefronts' exponentials to overlap (51738 x 616 fp16, 20
-// a lane 72 us, 10 a lane 65; 46394 x 242, 16 a lane 23.3, 8 a lane 21.7).
+// Drawing for up to 16384 rows, which do not fill the GPU: short rows over four lanes.  (64-bit exponentials one after the other: 4096 x 18 fp32 4.2 us, in
+// one lane 5.0; 65536 x 18 6.4, in one lane 5.2.)
+// Beyond 32 scores, 16 a lane at most, whatever their type; with 32 of 16 bits in fewer lanes there is less overlap of wavefronts' exponentials and fewer
+// exchanges (46394 x 242 fp16 20.0 us against 22.2; 51738 x 616 60.8 against 56.6).
 template <typename T, typename F> int by_length_to_draw(int64_t rows, int64_t n, F f) {
     if (n > 32) return by_lanes<4, 2048 / sizeof(T)>(n, f);
     if (rows > 16384 || n < 8) return by_length_32(n, f);
@@ -1297,9 +1301,9 @@ template <typename T, typename F> int by_length_to_draw(int64_t rows, int64_t n,
 }
 // How a long row is shared out: a wavefront a row (no exchange between wavefronts) where these are many or the rows not that long, else a
 // workgroup, or several where that leaves CUs without one (no more than the row has tiles).  Measured (log probabilities / with five
-// alternatives, us; wavefront against workgroup): 512 x 2500 bf16 5.1 / 7.6 against 5.1 / 7.4, 2048 x 2500 5.3 / 8.9 against 6.9 / 14.4;
-// 512 x 5832 5.5 / 10.3 against 5.0 / 7.9, 2048 x 5832 8.2 / 13.4 against 9.9 / 17.4, 4096 x 5832 12.2 / 18.0 against 15.1 / 28.7; 1024 x 20000
-// 14.9 / 29.5 against 12.0 / 18.3, 2048 x 20000 18.8 / 33.7 against 19.4 / 31.0, 4096 x 20000 32.6 / 50.0 against 35.0 / 60.5.
+// alternatives, us; wavefront against workgroup): 512 x 2500 bf16 4.5 against 4.4, 2048 x 2500 5.2 / 8.1 against 7.1 / 13.7; 512 x 5832 5.8 / 9.7
+// against 4.8 / 7.9, 2048 x 5832 7.5 / 11.8 against 8.3 / 15.3, 4096 x 5832 13.0 / 17.3 against 15.6 / 27.9; 1024 x 20000 15.3 / 26.2 against 12.4 /
+// 17.7, 2048 x 20000 19.3 / 30.3 against 20.3 / 30.4, 4096 x 20000 29.9 / 41.9 against 31.9 / 49.6.
 struct Split {
     int row_waves, parts, part_tiles;
 };
@@ -1311,18 +1315,18 @@ template <typename T> Split split(int64_t rows, int64_t n) {
     return {WAVES, (int)((tiles + each - 1) / each), (int)each};
 }
 // The backward pass of a longer row has a tile of a wavefront's or of a workgroup's size for each wavefront or workgroup; smaller tiles leave less of the last one empty.
-// Measured (us): 32768 x 2500 bf16 93 against 132, 16384 x 5832 76 against 86, 8192 x 20000 124 against 126, 3000 x 40001 99 against 96, 1024 x
-// 104976 86 against 81.
-// Up to two wavefront's tiles, halves of them (16-bit scores alone are that short here): 32768 x 2100 bf16 88 -> 67, x 2500 89 -> 70, x 4000 112 -> 110; longer rows 75.6 -> 76.9
-// (16384 x 5832), 60 -> 62 (750 x 50021 by workgroups), and quarters 83, 89, 149.
+// Measured (us): 32768 x 2500 bf16 75 against 100, 16384 x 5832 61 against 69, 8192 x 20000 113 against 120, 3000 x 40001 76 against 74, 1024 x
+// 104976 67 either way.
+// Up to two wavefront's tiles, halves of them (16-bit scores alone are that short here): 32768 x 2100 bf16 76 -> 57, x 2500 75 -> 58, x 4000 90 -> 91; longer
+// rows 61 -> 65 (16384 x 5832); quarters, when they were tried, 1.2 ... 1.4 times halves.
 template <typename T> bool backward_by_waves(int64_t n) { return Tile<T, 1>::count(n) <= 12; }
 // Short rows' alternatives come one after the other, a pass over the registers each; from nine on, of rows of some length, a wavefront a row that
-// collects and ranks them is faster (7 x 1000 fp32, 20 of them: 5.6 us against 14.6 in passes).
+// collects and ranks them is faster (7 x 500 fp32, 20 of them: 5.6 us against 13.2 in passes).
 template <typename T> bool in_lanes(int64_t n, int top) { return is_short<T>(n) && !(n > 256 && top > 8); }
 template <typename T> int n_segments(int64_t n) { return (int)((n + 64 * (16 / sizeof(T)) - 1) / (64 * (16 / sizeof(T)))); }
 // Drawing: a wavefront a row up to 12 tiles where there are rows enough, else a workgroup a tile and a second kernel.  Measured (us; the first against the
-// second): 16 x 2500 bf16 7.7 against 9.9; 16 x 5832 11.4 against 9.9, 1024 x 5832 12.1 against 14.4, 4096 x 5832 28 against 44; 1024 x 20000
-// 33 against 27, 2048 x 20000 45 against 48, 4096 x 20000 80 against 94; fp32, 20 tiles: 2048 x 20000 76 against 57.
+// second): 16 x 2500 bf16 8.2 against 8.6; 16 x 5832 12.1 against 9.3, 1024 x 5832 12.7 against 14.0, 4096 x 5832 28 against 43; 1024 x 20000
+// 32 against 28, 2048 x 20000 43 against 48, 4096 x 20000 73 against 89; longer rows, fp32, 2048 x 20000 52 by the second (76 against 57 when the rule was made).
 template <typename T> bool sample_by_waves(int64_t rows, int64_t n) {
     const int64_t tiles = Tile<T, 1>::count(n);
     return tiles <= 2 || (tiles <= 4 && rows >= 512) || (tiles <= 12 && rows >= 2048);          // (at most 48 segments: a lane each)
